@@ -168,6 +168,48 @@ class FmhaArgs(Structure):
     ]
 
 
+class QkNormRopeArgs(Structure):
+    _fields_ = [
+        ("q", c_void_p), ("k", c_void_p), ("q_out", c_void_p), ("k_out", c_void_p),
+        ("dq_out", c_void_p), ("dk_out", c_void_p),
+        ("q_weight", c_void_p), ("k_weight", c_void_p), ("dq_weight", c_void_p), ("dk_weight", c_void_p),
+        ("cos", c_void_p), ("sin", c_void_p), ("positions", c_void_p), ("workspace", c_void_p),
+        ("batch", c_int64), ("tokens", c_int64), ("heads_q", c_int64), ("heads_kv", c_int64),
+        ("q_stride_b", c_int64), ("q_stride_h", c_int64), ("q_stride_t", c_int64),
+        ("k_stride_b", c_int64), ("k_stride_h", c_int64), ("k_stride_t", c_int64),
+        ("qo_stride_b", c_int64), ("qo_stride_h", c_int64), ("qo_stride_t", c_int64),
+        ("ko_stride_b", c_int64), ("ko_stride_h", c_int64), ("ko_stride_t", c_int64),
+        ("dq_stride_b", c_int64), ("dq_stride_h", c_int64), ("dq_stride_t", c_int64),
+        ("dk_stride_b", c_int64), ("dk_stride_h", c_int64), ("dk_stride_t", c_int64),
+        ("position_stride_b", c_int64), ("position_stride_t", c_int64),
+        ("table_rows", c_int64), ("table_stride", c_int64), ("workspace_bytes", c_int64),
+        ("head_dim", c_int32), ("rotary_dim", c_int32), ("interleaved", c_int32),
+        ("positions_are_int64", c_int32), ("dtype", c_int32), ("weight_dtype", c_int32), ("eps", c_float),
+    ]
+
+
+class PagedKvAppendArgs(Structure):
+    _fields_ = [
+        ("k", c_void_p), ("v", c_void_p), ("q", c_void_p), ("q_out", c_void_p),
+        ("k_cache", c_void_p), ("v_cache", c_void_p), ("q_weight", c_void_p), ("k_weight", c_void_p),
+        ("cos", c_void_p), ("sin", c_void_p), ("positions", c_void_p),
+        ("page_table", c_void_p), ("cache_lens", c_void_p), ("new_lens", c_void_p),
+        ("batch", c_int64), ("tokens", c_int64), ("heads_q", c_int64), ("heads_kv", c_int64),
+        ("k_stride_b", c_int64), ("k_stride_h", c_int64), ("k_stride_t", c_int64),
+        ("v_stride_b", c_int64), ("v_stride_h", c_int64), ("v_stride_t", c_int64),
+        ("q_stride_b", c_int64), ("q_stride_h", c_int64), ("q_stride_t", c_int64),
+        ("qo_stride_b", c_int64), ("qo_stride_h", c_int64), ("qo_stride_t", c_int64),
+        ("kc_stride_p", c_int64), ("kc_stride_h", c_int64), ("kc_stride_s", c_int64),
+        ("vc_stride_p", c_int64), ("vc_stride_h", c_int64), ("vc_stride_s", c_int64),
+        ("position_stride_b", c_int64), ("position_stride_t", c_int64),
+        ("table_rows", c_int64), ("table_stride", c_int64),
+        ("num_pages", c_int64), ("page_table_stride", c_int64), ("page_size", c_int32), ("max_pages", c_int32),
+        ("head_dim", c_int32), ("rotary_dim", c_int32), ("interleaved", c_int32),
+        ("positions_are_int64", c_int32), ("dtype", c_int32), ("weight_dtype", c_int32),
+        ("zero_padding", c_int32), ("eps", c_float),
+    ]
+
+
 class PeerGatherArgs(Structure):
     _fields_ = [
         ("shards", POINTER(c_void_p)), ("dst", c_void_p),
@@ -215,6 +257,10 @@ SIGNATURES = {
     "b200k_peer_barrier": (c_int, [POINTER(c_void_p), c_int32, c_int32, c_void_p, c_int32, c_void_p]),
     "b200k_fmha_fwd": (c_int, [POINTER(FmhaArgs), c_void_p]),
     "b200k_fmha_workspace_bytes": (c_int64, [POINTER(FmhaArgs)]),
+    "b200k_qk_norm_rope": (c_int, [POINTER(QkNormRopeArgs), c_void_p]),
+    "b200k_qk_norm_rope_backward": (c_int, [POINTER(QkNormRopeArgs), c_void_p]),
+    "b200k_qk_norm_rope_backward_workspace_bytes": (c_int64, [POINTER(QkNormRopeArgs)]),
+    "b200k_paged_kv_append": (c_int, [POINTER(PagedKvAppendArgs), c_void_p]),
     "b200k_sf_swizzle": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int32,
                                  c_void_p, c_int32, c_void_p]),
 }
@@ -304,6 +350,11 @@ def tensor_map_cache_stats() -> tuple[int, int, int]:
 
 def raise_on_device_error() -> None:
     code, info = device_status()
+    if code == INVALID_ARG:
+        what = {80: "a position outside the rotation table (token {})",
+                81: "a page of sequence {} outside the page table or the cache"}
+        role, detail = (info >> 8) & 0xff, (info >> 16) & 0xffff
+        raise B200KError(code, what.get(role, f"index of kind {role} out of range ({{}})").format(detail))
     if code != 0:
         raise B200KError(code, f"device-side wait gave up (role {(info >> 8) & 0xff}, "
                                f"detail {(info >> 16) & 0xffff})")

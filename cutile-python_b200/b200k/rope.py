@@ -1,0 +1,210 @@
+"""Norm of every query and key head and rotation by position, one pass; with its gradient.
+
+The operators between a projection GEMM and ``cutile_fmha``: both take and give the attention
+wrappers' (Batch, Heads, SeqLen, Dim) views, so queries and keys may lie side by side in one
+(Batch, SeqLen, Heads, Dim) projection.  No counterpart among the reference's samples.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+
+
+def rope_table(max_positions: int, rotary_dim: int, theta: float = 10000.0,
+               device: torch.device | str | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """cos, sin of position * theta^(-2 i / rotary_dim), each (max_positions, rotary_dim / 2)
+    float32.  The angles are taken in float64: at position 10^5 a float32 angle is already
+    off by 4e-3."""
+    if max_positions <= 0 or rotary_dim <= 0 or rotary_dim % 2:
+        raise ValueError("max_positions must be positive, rotary_dim positive and even")
+    inv = theta ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64, device=device) / rotary_dim)
+    angle = torch.arange(max_positions, dtype=torch.float64, device=device)[:, None] * inv
+    return angle.cos().float(), angle.sin().float()
+
+
+def rows_view(t: torch.Tensor) -> torch.Tensor:
+    """The tensor itself where its rows are contiguous, else a copy that has them so."""
+    return t if t.stride(-1) == 1 else t.contiguous()
+
+
+def check_no_grad(name: str, instead: str, *tensors) -> None:
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{name} is not recorded by autograd: call it under torch.no_grad(){instead}")
+
+
+def check_out(t: torch.Tensor, like: torch.Tensor, name: str) -> torch.Tensor:
+    if t.shape != like.shape or t.dtype != like.dtype or t.device != like.device:
+        raise ValueError(f"{name} must have the shape, dtype and device of its input")
+    if t.numel() and t.stride(-1) != 1 or any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
+        raise ValueError(f"{name} must have contiguous rows that do not overlap")
+    return t
+
+
+def check_table(cos: torch.Tensor, sin: torch.Tensor, dim: int, device: torch.device):
+    """(cos, sin, rotary_dim) with equal row strides."""
+    if cos.ndim != 2 or cos.shape != sin.shape:
+        raise ValueError("cos and sin must both be (positions, rotary_dim / 2)")
+    if cos.dtype != torch.float32 or sin.dtype != torch.float32:
+        raise TypeError("cos and sin must be float32")
+    if cos.device != device or sin.device != device:
+        raise ValueError("cos and sin must be on the device of the rows")
+    rotary = 2 * cos.shape[1]
+    if rotary > dim or rotary % 16:
+        raise ValueError(f"rotary_dim must be a multiple of 16 up to the head dimension (got {rotary} of {dim})")
+    if cos.shape[0] == 0:
+        raise ValueError("the rotation table has no positions")
+    if (cos.stride() != sin.stride() or cos.stride(1) != 1 or cos.stride(0) % 4
+            or (cos.data_ptr() | sin.data_ptr()) % 16):
+        cos, sin = (torch.empty(cos.shape, dtype=torch.float32, device=device).copy_(t) for t in (cos, sin))
+    return cos, sin, rotary
+
+
+def check_positions(positions: torch.Tensor | None, batch: int, tokens: int, device: torch.device):
+    """(pointer, batch stride, token stride, is int64)"""
+    if positions is None:
+        return None, 0, 0, 0
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise TypeError("positions must be int32 or int64")
+    if positions.device != device:
+        raise ValueError("positions must be on the device of the rows")
+    if positions.shape == (tokens,):
+        stride_b, stride_t = 0, positions.stride(0)
+    elif positions.shape == (batch, tokens):
+        stride_b, stride_t = positions.stride()
+    else:
+        raise ValueError(f"positions must be ({tokens},) or ({batch}, {tokens}), got {tuple(positions.shape)}")
+    return positions.data_ptr(), stride_b, stride_t, int(positions.dtype == torch.int64)
+
+
+def check_weights(dim: int, dtype: torch.dtype, device: torch.device, *weights) -> torch.dtype:
+    """The weights' dtype (the rows' where there are none)."""
+    found = None
+    for w in weights:
+        if w is None:
+            continue
+        if w.shape != (dim,):
+            raise ValueError(f"norm weights must be ({dim},), got {tuple(w.shape)}")
+        if w.device != device:
+            raise ValueError("norm weights must be on the device of the rows")
+        if w.dtype not in (dtype, torch.float32):
+            raise TypeError("norm weights must have the rows' dtype or be float32")
+        if w.stride(0) != 1 and dim > 1:
+            raise ValueError("norm weights must be contiguous")
+        if found is not None and w.dtype != found:
+            raise TypeError("both norm weights must have one dtype")
+        found = w.dtype
+    return found or dtype
+
+
+def _check_rows(q: torch.Tensor, k: torch.Tensor) -> None:
+    if q.ndim != 4 or k.ndim != 4:
+        raise ValueError("q and k must be 4D (Batch, Heads, SeqLen, Dim).")
+    if q.shape[0] != k.shape[0] or q.shape[2:] != k.shape[2:]:
+        raise ValueError("q and k must agree in Batch, SeqLen and Dim.")
+    if q.device != k.device or not q.is_cuda:
+        raise ValueError("q and k must be on the same CUDA device.")
+    if q.dtype != k.dtype:
+        raise ValueError("q and k must have the same data type.")
+    if q.dtype not in (torch.float16, torch.bfloat16, torch.float32):
+        raise TypeError("q and k must be float16, bfloat16 or float32")
+    if q.shape[3] % 8 or not 0 < q.shape[3] <= 256:
+        raise ValueError("the head dimension must be a multiple of 8 up to 256")
+
+
+def launch(entry: str, args: ctypes.Structure, device: torch.device) -> None:
+    """Calls an entry point on the device's current stream."""
+    fn = getattr(_lib.lib(), entry)
+    index = device.index
+    if index is None or torch.cuda.current_device() == index:
+        code = fn(ctypes.byref(args), _lib.stream_ptr(device))
+    else:
+        with torch.cuda.device(device):
+            code = fn(ctypes.byref(args), _lib.stream_ptr(device))
+    if code < 0:
+        _lib.check(code)
+
+
+def _fill(a, q, k, q_out, k_out, q_weight, k_weight, cos, sin, positions, eps, interleaved):
+    batch, heads, tokens, dim = q.shape
+    cos, sin, rotary = check_table(cos, sin, dim, q.device)
+    weight_dtype = check_weights(dim, q.dtype, q.device, q_weight, k_weight)
+    a.q, a.k, a.q_out, a.k_out = q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr()
+    a.q_weight, a.k_weight = _lib.ptr(q_weight), _lib.ptr(k_weight)
+    a.cos, a.sin = cos.data_ptr(), sin.data_ptr()
+    a.table_rows, a.table_stride = cos.shape[0], cos.stride(0)
+    a.positions, a.position_stride_b, a.position_stride_t, a.positions_are_int64 = check_positions(
+        positions, batch, tokens, q.device)
+    a.batch, a.tokens, a.heads_q, a.heads_kv = batch, tokens, heads, k.shape[1]
+    a.q_stride_b, a.q_stride_h, a.q_stride_t, _ = q.stride()
+    a.k_stride_b, a.k_stride_h, a.k_stride_t, _ = k.stride()
+    a.qo_stride_b, a.qo_stride_h, a.qo_stride_t, _ = q_out.stride()
+    a.ko_stride_b, a.ko_stride_h, a.ko_stride_t, _ = k_out.stride()
+    a.head_dim, a.rotary_dim, a.interleaved = dim, rotary, 1 if interleaved else 0
+    a.dtype, a.weight_dtype, a.eps = _lib.dtype_enum(q.dtype), _lib.dtype_enum(weight_dtype), eps
+    return cos, sin
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor,
+                 q_weight: torch.Tensor | None, k_weight: torch.Tensor | None,
+                 cos: torch.Tensor, sin: torch.Tensor,
+                 positions: torch.Tensor | None = None, *,
+                 eps: float = 1e-6, interleaved: bool = False,
+                 q_out: torch.Tensor | None = None,
+                 k_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Every row of q (Batch, Heads, SeqLen, Dim) and k (Batch, KV_Heads, SeqLen, Dim), float16,
+    bfloat16 or float32, divided by its root mean square, times the (Dim,) weight, with its
+    first rotary_dim = 2 * cos.shape[1] values turned by the token's position: one launch, each
+    row read and written once, fp32 inside.
+
+    A weight of None leaves that norm out (rotation alone).  ``cos`` / ``sin`` are tables by
+    position (``rope_table``); ``positions`` is (SeqLen,) or (Batch, SeqLen), None = 0, 1, 2, ...
+    Pairs are (i, i + rotary_dim / 2), or neighbours with ``interleaved``.  ``q_out`` / ``k_out``
+    may be q / k themselves.  A position outside the table gives NaN rows, and
+    ``raise_on_device_error()`` names it."""
+    _check_rows(q, k)
+    check_no_grad("qk_norm_rope", " and take gradients from qk_norm_rope_backward", q, k, q_weight, k_weight)
+    qo = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else check_out(q_out, q, "q_out")
+    ko = torch.empty(k.shape, dtype=k.dtype, device=k.device) if k_out is None else check_out(k_out, k, "k_out")
+    q, k = rows_view(q), rows_view(k)
+    a = _lib.QkNormRopeArgs()
+    keep = _fill(a, q, k, qo, ko, q_weight, k_weight, cos, sin, positions, eps, interleaved)  # noqa: F841
+    launch("b200k_qk_norm_rope", a, q.device)
+    return qo, ko
+
+
+def qk_norm_rope_backward(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
+                          q_weight: torch.Tensor | None, k_weight: torch.Tensor | None,
+                          cos: torch.Tensor, sin: torch.Tensor,
+                          positions: torch.Tensor | None = None, *,
+                          eps: float = 1e-6, interleaved: bool = False):
+    """Gradients (of q, of k, of q_weight, of k_weight) from the gradients ``dq``, ``dk`` of
+    qk_norm_rope's outputs and its inputs (in-place outputs lose them).  The weights' gradients
+    are summed in fp32 over all rows in a fixed order and rounded to the weights' dtype; None
+    for a weight of None."""
+    _check_rows(q, k)
+    check_no_grad("qk_norm_rope_backward", "", dq, dk, q, k, q_weight, k_weight)
+    for g, x, name in ((dq, q, "dq"), (dk, k, "dk")):
+        if g.shape != x.shape or g.dtype != x.dtype or g.device != x.device:
+            raise ValueError(f"{name} must have the shape, dtype and device of {name[1]}")
+    q_in, k_in = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k))
+    q, k, dq, dk = rows_view(q), rows_view(k), rows_view(dq), rows_view(dk)
+    a = _lib.QkNormRopeArgs()
+    keep = _fill(a, q, k, q_in, k_in, q_weight, k_weight, cos, sin, positions, eps, interleaved)  # noqa: F841
+    a.dq_out, a.dk_out = dq.data_ptr(), dk.data_ptr()
+    a.dq_stride_b, a.dq_stride_h, a.dq_stride_t, _ = dq.stride()
+    a.dk_stride_b, a.dk_stride_h, a.dk_stride_t, _ = dk.stride()
+    dqw, dkw = (None if w is None else torch.empty_like(w) for w in (q_weight, k_weight))
+    a.dq_weight, a.dk_weight = _lib.ptr(dqw), _lib.ptr(dkw)
+    workspace = None
+    if dqw is not None or dkw is not None:
+        with torch.cuda.device(q.device):
+            size = _lib.lib().b200k_qk_norm_rope_backward_workspace_bytes(ctypes.byref(a))
+        workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
+        a.workspace, a.workspace_bytes = workspace.data_ptr(), size
+    launch("b200k_qk_norm_rope_backward", a, q.device)
+    return q_in, k_in, dqw, dkw

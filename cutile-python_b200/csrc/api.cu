@@ -228,7 +228,8 @@ int b200k_device_status(int* code, int* info) {
     int zero = 0;
     cudaMemcpy(word, &zero, sizeof(int), cudaMemcpyHostToDevice);
   }
-  if (code) *code = (value & 0xff) ? B200K_TIMEOUT : B200K_OK;
+  const int kind = value & 0xff;   // 1: a wait gave up, 2: an index out of range (common.cuh)
+  if (code) *code = kind == 0 ? B200K_OK : (kind == 2 ? B200K_INVALID_ARG : B200K_TIMEOUT);
   if (info) *info = value & ~0xff;
   return B200K_OK;
 }

@@ -10,8 +10,8 @@
  *     them alive until the stream has passed the call; array arguments must not alias),
  *   - returns 0 or a negative b200k_status; b200k_last_error() gives the message.
  *
- * Device-side trouble (a pipeline wait that ran out of its time budget) is recorded
- * in a per-device status word that b200k_device_status() reads after the caller has
+ * Device-side trouble (a pipeline wait that ran out of its time budget, an index out of
+ * range) is recorded in a per-device status word that b200k_device_status() reads after the caller has
  * synchronised the stream.
  */
 #ifndef B200K_H_
@@ -56,8 +56,11 @@ typedef enum {
 const char* b200k_version(void);
 const char* b200k_last_error(void);             /* thread-local message of the last failure */
 int b200k_sm_count(void);                       /* SMs of the current device, <0 on error */
-/* Reads and clears the current device's status word.  *code is 0 or B200K_TIMEOUT,
- * *info packs (role << 8 | detail << 16) of the wait that gave up. */
+/* Reads and clears the current device's status word.  *code is 0, B200K_TIMEOUT or (an index
+ * in device memory that lies outside what it points into: a position, a page)
+ * B200K_INVALID_ARG; *info packs (role << 8 | detail << 16) of the wait that gave up or of
+ * the index: role 80 = a position outside the rotation table (detail: token), 81 = a page
+ * outside the page table or the cache (detail: sequence). */
 int b200k_device_status(int* code, int* info);
 /* The one piece of state the library owns: a mutex-guarded cache of encoded TMA tensor maps
  * keyed by (base pointer, data type, dims, strides, box, swizzle), at most 8192 entries of
@@ -579,6 +582,110 @@ int b200k_fmha_fwd(const b200k_fmha_args* args, b200k_stream stream);
  * The keys are split over CTAs that stream K and V once on the CUDA cores; a second kernel
  * merges the partial softmax states.  0 = the path does not apply. */
 int64_t b200k_fmha_workspace_bytes(const b200k_fmha_args* args);
+
+/* ---- norm of queries and keys, rotation by position -----------------------------------
+ * No counterpart among the reference's samples; the operators that stand between a projection
+ * GEMM and the attention above.  Per row x (one head of one token, D values), fp32 throughout,
+ * rounded once:
+ *     n = x * rsqrt(mean(x^2) + eps) * weight        (weight NULL: n = x)
+ *     y = n with its first rotary_dim values turned in pairs by the angles of the token's
+ *         position p: (a, b) -> (a cos - b sin, b cos + a sin), the pairs being
+ *         (i, i + rotary_dim / 2), or (2 i, 2 i + 1) with `interleaved`.
+ * Rows are (batch, heads, tokens, D) through element strides, D contiguous; any alignment
+ * (16-byte aligned bases and strides are read as vectors).  D a multiple of 8 up to 256,
+ * rotary_dim a multiple of 16 up to D (0 = no rotation, the tables may then be NULL).  Either
+ * head count may be 0.  q_out may be q and k_out may be k (same pointer and strides).
+ * `positions` (batch, tokens) int32 or int64 through strides, NULL = 0, 1, 2, ... in every
+ * sequence.  A position outside [0, table_rows) gives NaN rows and is recorded in the status
+ * word. */
+typedef struct {
+  const void* q;                /* (batch, heads_q, tokens, D) */
+  const void* k;                /* (batch, heads_kv, tokens, D) */
+  void* q_out;                  /* forward: rotated rows; backward: gradient of q */
+  void* k_out;
+  const void* dq_out;           /* backward: gradients of the forward's outputs */
+  const void* dk_out;
+  const void* q_weight;         /* (D) each, or NULL */
+  const void* k_weight;
+  void* dq_weight;              /* backward: (D), in weight_dtype; with q_weight, NULL without */
+  void* dk_weight;
+  const float* cos;             /* (table_rows, rotary_dim / 2), row stride table_stride (a multiple */
+  const float* sin;             /*   of 4), 16-byte aligned */
+  const void* positions;
+  void* workspace;              /* backward with weights: 16-byte aligned, contents irrelevant */
+  int64_t batch, tokens, heads_q, heads_kv;
+  int64_t q_stride_b, q_stride_h, q_stride_t;
+  int64_t k_stride_b, k_stride_h, k_stride_t;
+  int64_t qo_stride_b, qo_stride_h, qo_stride_t;
+  int64_t ko_stride_b, ko_stride_h, ko_stride_t;
+  int64_t dq_stride_b, dq_stride_h, dq_stride_t;
+  int64_t dk_stride_b, dk_stride_h, dk_stride_t;
+  int64_t position_stride_b, position_stride_t;
+  int64_t table_rows, table_stride, workspace_bytes;
+  int32_t head_dim, rotary_dim;
+  int32_t interleaved;
+  int32_t positions_are_int64;
+  int32_t dtype;                /* B200K_F16 | BF16 | F32: all rows */
+  int32_t weight_dtype;         /* dtype or B200K_F32 */
+  float eps;
+} b200k_qk_norm_rope_args;
+
+int b200k_qk_norm_rope(const b200k_qk_norm_rope_args* args, b200k_stream stream);
+
+/* Gradients of the above from dq_out / dk_out (the norm is recomputed from q / k): q_out and
+ * k_out receive the gradients of q and k, dq_weight and dk_weight those of the weights, summed
+ * in fp32 over all rows in an order that does not change from run to run. */
+int b200k_qk_norm_rope_backward(const b200k_qk_norm_rope_args* args, b200k_stream stream);
+int64_t b200k_qk_norm_rope_backward_workspace_bytes(const b200k_qk_norm_rope_args* args);
+
+/* ---- paged key/value cache ------------------------------------------------------------
+ * A cache is (num_pages, heads_kv, page_size, D) through the strides (page, head, slot): both
+ * (page, head, slot, D) and (page, slot, head, D) storage.  Token p of sequence b lies in slot
+ * p % page_size of page page_table[b][p / page_size].  cache_lens[b] tokens are there before
+ * the call; the call's token t of sequence b is token cache_lens[b] + t, for
+ * t < new_lens[b] (NULL = all `tokens`); the rest of a sequence's `tokens` rows is padding.
+ *
+ * b200k_paged_kv_append stores K (normed when k_weight is given, rotated when rotary_dim > 0,
+ * as above) and V of the call's tokens into the cache and, with q, writes the normed and
+ * rotated queries to q_out in the same launch.  positions NULL = cache_lens[b] + t.  Slots of
+ * padding tokens are left as they are; their q_out rows too, or become zero with
+ * `zero_padding`.  A token whose page is outside [0, num_pages) or behind max_pages is not
+ * stored and is recorded in the status word.  Tokens that share a slot (two sequences with the
+ * same page) leave one of the two. */
+typedef struct {
+  const void* k;                /* (batch, heads_kv, tokens, D) */
+  const void* v;
+  const void* q;                /* (batch, heads_q, tokens, D) or NULL */
+  void* q_out;
+  void* k_cache;
+  void* v_cache;
+  const void* q_weight;         /* (D) or NULL */
+  const void* k_weight;
+  const float* cos;             /* as in b200k_qk_norm_rope_args */
+  const float* sin;
+  const void* positions;
+  const int32_t* page_table;    /* (batch, max_pages), row stride page_table_stride */
+  const int32_t* cache_lens;    /* (batch) */
+  const int32_t* new_lens;      /* (batch) or NULL */
+  int64_t batch, tokens, heads_q, heads_kv;
+  int64_t k_stride_b, k_stride_h, k_stride_t;
+  int64_t v_stride_b, v_stride_h, v_stride_t;
+  int64_t q_stride_b, q_stride_h, q_stride_t;
+  int64_t qo_stride_b, qo_stride_h, qo_stride_t;
+  int64_t kc_stride_p, kc_stride_h, kc_stride_s;
+  int64_t vc_stride_p, vc_stride_h, vc_stride_s;
+  int64_t position_stride_b, position_stride_t;
+  int64_t table_rows, table_stride;
+  int64_t num_pages, page_table_stride;
+  int32_t page_size, max_pages;
+  int32_t head_dim, rotary_dim, interleaved, positions_are_int64;
+  int32_t dtype;                /* B200K_F16 | BF16 */
+  int32_t weight_dtype;
+  int32_t zero_padding;
+  float eps;
+} b200k_paged_kv_append_args;
+
+int b200k_paged_kv_append(const b200k_paged_kv_append_args* args, b200k_stream stream);
 
 #ifdef __cplusplus
 }

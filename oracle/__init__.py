@@ -10,10 +10,12 @@ falling back to anything here.
 Pinning: oracle/quantize.py and oracle/moe.py are checked bit-for-bit against outputs of
 the reference's own functions (tests/golden/*.npz, generated by tests/golden/make_golden.py
 from the reference checkout) and against the reference's known-answer docstring cases;
-the NVFP4 quantiser has no counterpart in the reference and is "parity unpinned".
+the NVFP4 quantiser and oracle/rope.py have no counterpart in the reference and are "parity
+unpinned".
 """
 from .formats import *  # noqa: F401,F403
 from .quantize import *  # noqa: F401,F403
 from .matmul import *  # noqa: F401,F403
 from .moe import *  # noqa: F401,F403
 from .attention import *  # noqa: F401,F403
+from .rope import *  # noqa: F401,F403
