@@ -11,7 +11,7 @@ from .block_scaled import (block_quantize, cutile_block_scaled_matmul,  # noqa: 
                            swizzle_32_4_4)
 from .fmha import cutile_fmha, cutile_fmha_into  # noqa: F401
 from .rope import qk_norm_rope, qk_norm_rope_backward, rope_table  # noqa: F401
-from .paged import paged_kv_append  # noqa: F401
+from .paged import paged_attention, paged_kv_append  # noqa: F401
 from .moe import (cutile_moe, cutile_moe_mxfp8, invoke_fused_moe_kernel,  # noqa: F401
                   invoke_silu_and_mul_kernel, moe_align_device, moe_align_tile_size_torch,
                   quantize_expert_weights)

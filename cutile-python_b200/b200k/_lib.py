@@ -210,6 +210,23 @@ class PagedKvAppendArgs(Structure):
     ]
 
 
+class PagedAttentionArgs(Structure):
+    _fields_ = [
+        ("q", c_void_p), ("k_cache", c_void_p), ("v_cache", c_void_p), ("out", c_void_p),
+        ("page_table", c_void_p), ("cache_lens", c_void_p), ("new_lens", c_void_p), ("tree_mask", c_void_p),
+        ("workspace", c_void_p),
+        ("batch", c_int64), ("tokens", c_int64), ("heads_q", c_int64), ("heads_kv", c_int64),
+        ("q_stride_b", c_int64), ("q_stride_h", c_int64), ("q_stride_t", c_int64),
+        ("o_stride_b", c_int64), ("o_stride_h", c_int64), ("o_stride_t", c_int64),
+        ("kc_stride_p", c_int64), ("kc_stride_h", c_int64), ("kc_stride_s", c_int64),
+        ("vc_stride_p", c_int64), ("vc_stride_h", c_int64), ("vc_stride_s", c_int64),
+        ("mask_stride_b", c_int64), ("mask_stride_t", c_int64), ("mask_stride_j", c_int64),
+        ("num_pages", c_int64), ("page_table_stride", c_int64), ("workspace_bytes", c_int64),
+        ("page_size", c_int32), ("max_pages", c_int32), ("head_dim", c_int32), ("dtype", c_int32),
+        ("zero_padding", c_int32), ("qk_scale", c_float),
+    ]
+
+
 class PeerGatherArgs(Structure):
     _fields_ = [
         ("shards", POINTER(c_void_p)), ("dst", c_void_p),
@@ -261,6 +278,8 @@ SIGNATURES = {
     "b200k_qk_norm_rope_backward": (c_int, [POINTER(QkNormRopeArgs), c_void_p]),
     "b200k_qk_norm_rope_backward_workspace_bytes": (c_int64, [POINTER(QkNormRopeArgs)]),
     "b200k_paged_kv_append": (c_int, [POINTER(PagedKvAppendArgs), c_void_p]),
+    "b200k_paged_attention": (c_int, [POINTER(PagedAttentionArgs), c_void_p]),
+    "b200k_paged_attention_workspace_bytes": (c_int64, [POINTER(PagedAttentionArgs)]),
     "b200k_sf_swizzle": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int32,
                                  c_void_p, c_int32, c_void_p]),
 }

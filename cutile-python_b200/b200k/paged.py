@@ -1,13 +1,21 @@
-"""A key/value cache in pages: appending a step's tokens.
+"""A key/value cache in pages: appending a step's tokens, attention over what is there.
 
 Caches are (Pages, KV_Heads, Page_Size, Dim) views - (page, head, slot, Dim) storage, or
 (page, slot, head, Dim) storage seen through ``transpose(1, 2)``.  ``page_table`` (Batch,
 Max_Pages) names the pages of each sequence in order; ``cache_lens`` (Batch,) counts the tokens
 a sequence had before this step; ``new_lens`` (Batch,), where sequences bring different numbers
-of tokens, says how many of the step's SeqLen rows are real.  
+of tokens, says how many of the step's SeqLen rows are real.  The same tensors serve both calls:
+
+    q = paged_kv_append(k, v, k_cache, v_cache, page_table, cache_lens, cos, sin, q=q, ...)
+    out = paged_attention(q, k_cache, v_cache, page_table, cache_lens, ...)
+    cache_lens += 1                       # or by the drafts that were accepted
+
 No counterpart among the reference's samples.
 """
 from __future__ import annotations
+
+import ctypes
+import math
 
 import torch
 
@@ -119,3 +127,81 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
     a.dtype, a.weight_dtype, a.eps = _lib.dtype_enum(k.dtype), _lib.dtype_enum(weight_dtype), eps
     launch("b200k_paged_kv_append", a, device)
     return qo
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                    page_table: torch.Tensor, cache_lens: torch.Tensor, *,
+                    new_lens: torch.Tensor | None = None, tree_mask: torch.Tensor | None = None,
+                    qk_scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """softmax(qk_scale * q K^T) V of a step's queries q (Batch, Heads, SeqLen, Dim) over the
+    cache, after ``paged_kv_append`` of the same step: query t of sequence b reads the
+    cache_lens[b] tokens that were there before and those of the step's tokens j for which
+    ``tree_mask`` ((SeqLen, SeqLen) or (Batch, SeqLen, SeqLen), bool) is True at [t, j]; without a
+    mask the tokens j <= t.  One token per sequence is a decode step, a mask of ancestors
+    scores a tree of drafts.
+
+    float16 or bfloat16, heads a multiple of the cache's, Dim a multiple of 8 up to 128, pages
+    of a multiple of 8 tokens, qk_scale positive (None: 1 / sqrt(Dim)).  A query that sees no token gives zeros.  Slots that hold none of
+    the sequence's tokens are never used.  Rows behind new_lens[b] are padding: they stay as
+    they are in a given ``out`` and are zero in one made here."""
+    if q.ndim != 4:
+        raise ValueError("q must be 4D (Batch, Heads, SeqLen, Dim).")
+    if not q.is_cuda:
+        raise ValueError("q must be on a CUDA device.")
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError("paged_attention supports float16 and bfloat16")
+    batch, heads, tokens, dim = q.shape
+    device = q.device
+    check_no_grad("paged_attention", "", q, k_cache, v_cache)
+    heads_kv = k_cache.shape[1] if k_cache.ndim == 4 else 0
+    _check_cache(k_cache, v_cache, page_table, cache_lens, new_lens, batch, heads_kv, dim, q.dtype, device)
+    if heads_kv == 0 or heads % heads_kv:
+        raise ValueError("the number of query heads must be a multiple of the cache's heads.")
+    if dim % 8 or not 0 < dim <= 128:
+        raise ValueError("the head dimension must be a multiple of 8 up to 128")
+    if k_cache.shape[2] % 8:
+        raise ValueError("pages must hold a multiple of 8 tokens")
+    qk_scale = 1.0 / math.sqrt(dim) if qk_scale is None else float(qk_scale)
+    if not 0.0 < qk_scale < 3.0e38:
+        raise ValueError("qk_scale must be positive and finite")
+    a = _lib.PagedAttentionArgs()
+    for c, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        if c.data_ptr() % 16 or any(s % 8 for s in c.stride()[:3]):
+            raise ValueError(f"{name} must start on a 16-byte boundary with strides of whole 16-byte units")
+    if tree_mask is not None:
+        if tree_mask.dtype != torch.bool:
+            raise TypeError("tree_mask must be bool")
+        if tree_mask.device != device:
+            raise ValueError("tree_mask must be on the device of the queries.")
+        if tree_mask.shape == (tokens, tokens):
+            a.mask_stride_t, a.mask_stride_j = tree_mask.stride()
+        elif tree_mask.shape == (batch, tokens, tokens):
+            a.mask_stride_b, a.mask_stride_t, a.mask_stride_j = tree_mask.stride()
+        else:
+            raise ValueError(f"tree_mask must be ({tokens}, {tokens}) or ({batch}, {tokens}, {tokens}), "
+                             f"got {tuple(tree_mask.shape)}")
+        a.tree_mask = tree_mask.data_ptr()
+    a.zero_padding = 1 if out is None else 0
+    out = torch.empty(q.shape, dtype=q.dtype, device=device) if out is None else check_out(out, q, "out")
+    q = rows_view(q)
+    a.q, a.k_cache, a.v_cache, a.out = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr()
+    a.page_table, a.cache_lens, a.new_lens = page_table.data_ptr(), cache_lens.data_ptr(), _lib.ptr(new_lens)
+    a.batch, a.tokens, a.heads_q, a.heads_kv = batch, tokens, heads, heads_kv
+    a.q_stride_b, a.q_stride_h, a.q_stride_t, _ = q.stride()
+    a.o_stride_b, a.o_stride_h, a.o_stride_t, _ = out.stride()
+    a.kc_stride_p, a.kc_stride_h, a.kc_stride_s, _ = k_cache.stride()
+    a.vc_stride_p, a.vc_stride_h, a.vc_stride_s, _ = v_cache.stride()
+    a.num_pages, a.page_size = k_cache.shape[0], k_cache.shape[2]
+    a.max_pages, a.page_table_stride = page_table.shape[1], page_table.stride(0)
+    a.head_dim, a.dtype = dim, _lib.dtype_enum(q.dtype)
+    a.qk_scale = qk_scale
+    if torch.cuda.current_device() == device.index:
+        size = _lib.lib().b200k_paged_attention_workspace_bytes(ctypes.byref(a))
+    else:
+        with torch.cuda.device(device):
+            size = _lib.lib().b200k_paged_attention_workspace_bytes(ctypes.byref(a))
+    # made per call: calls on other streams and other captured graphs have their own
+    workspace = torch.empty(size, dtype=torch.uint8, device=device)
+    a.workspace, a.workspace_bytes = workspace.data_ptr(), size
+    launch("b200k_paged_attention", a, device)
+    return out

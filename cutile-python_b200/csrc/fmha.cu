@@ -21,6 +21,7 @@
 #include "common.cuh"
 #include "fmha_decode.h"
 #include "host.h"
+#include "softmax.cuh"
 
 namespace b200k {
 
@@ -28,7 +29,6 @@ constexpr int kFmhaBM = 128;
 constexpr int kFmhaBN = 128;
 constexpr int kFmhaThreads = 192;
 constexpr int kFmhaTmemCols = 256;
-constexpr float kRescaleThreshold = 8.0f;  // log2 units
 
 struct FmhaParams {
   void* out;
@@ -41,45 +41,6 @@ struct FmhaParams {
   int input_pos;
   int* status;
 };
-
-__device__ __forceinline__ float fmax3(float a, float b, float c) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
-
-// Every kFmhaPolyEvery-th pair of scores takes its exp2 on the FMA pipe (a degree-3
-// polynomial after splitting off the integer part) instead of the special-function unit,
-// which is the busiest pipe of the softmax.  Relative error 7.5e-5, far below the rounding
-// of P to 16 bits.  0 disables the polynomial path.
-#ifndef B200K_FMHA_POLY
-#define B200K_FMHA_POLY 4
-#endif
-constexpr int kFmhaPolyEvery = B200K_FMHA_POLY;
-
-__device__ __forceinline__ float2 exp2_poly_pair(float2 x) {
-  const float2 magic = make_float2(12582912.0f, 12582912.0f);       // 1.5 * 2^23
-  const float2 neg_magic = make_float2(-12582912.0f, -12582912.0f);
-  x.x = fmaxf(x.x, -125.0f);
-  x.y = fmaxf(x.y, -125.0f);
-  const float2 t = __fadd2_rn(x, magic);            // integer part lands in the low mantissa bits
-  const float2 i = __fadd2_rn(t, neg_magic);
-  const float2 f = __fadd2_rn(x, make_float2(-i.x, -i.y));   // in [-0.5, 0.5]
-  float2 p = __ffma2_rn(make_float2(0.05517164617776871f, 0.05517164617776871f), f,
-                        make_float2(0.2426111251115799f, 0.2426111251115799f));
-  p = __ffma2_rn(p, f, make_float2(0.6932609677314758f, 0.6932609677314758f));
-  p = __ffma2_rn(p, f, make_float2(0.9999280571937561f, 0.9999280571937561f));
-  float2 r;
-  r.x = __int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23));
-  r.y = __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23));
-  return r;
-}
-
-__device__ __forceinline__ float fast_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 // One softmax warp group (4 warps, one query row per thread) working on the 128-row query
 // tile that starts at row q0 of (batch b, head h): for each of its n_kv key tiles it reads S

@@ -687,6 +687,46 @@ typedef struct {
 
 int b200k_paged_kv_append(const b200k_paged_kv_append_args* args, b200k_stream stream);
 
+/* Attention of the call's tokens over the cache, after b200k_paged_kv_append has stored them:
+ * token t of sequence b reads the cache_lens[b] tokens that were there and those tokens j <
+ * new_lens[b] of the call for which tree_mask[b][t][j] is not 0 (NULL: j <= t), so that a tree
+ * of drafted tokens, a chunk of a prompt and a single token are the same call.
+ *   out = sum_p softmax_p(qk_scale * q . k_p) v_p        (a row that sees no key gives 0)
+ * qk_scale is positive.  What lies in slots that no token of the sequence occupies is never
+ * used, whatever it is.  A page outside [0, num_pages) counts as zeros, lengths beyond the page
+ * table as its end; both are recorded in the status word.
+ * Query head h reads key/value head h / (heads_q / heads_kv).  D a multiple of 8 up to 128;
+ * page_size a multiple of 8; cache bases and strides multiples of 16 bytes.  Padding rows of
+ * out are left as they are, or become zero with `zero_padding`. */
+typedef struct {
+  const void* q;                /* (batch, heads_q, tokens, D) */
+  const void* k_cache;
+  const void* v_cache;
+  void* out;                    /* (batch, heads_q, tokens, D) */
+  const int32_t* page_table;
+  const int32_t* cache_lens;
+  const int32_t* new_lens;      /* or NULL */
+  const uint8_t* tree_mask;     /* (batch, tokens, tokens) through strides, or NULL */
+  void* workspace;              /* see b200k_paged_attention_workspace_bytes; 16-byte aligned */
+  int64_t batch, tokens, heads_q, heads_kv;
+  int64_t q_stride_b, q_stride_h, q_stride_t;
+  int64_t o_stride_b, o_stride_h, o_stride_t;
+  int64_t kc_stride_p, kc_stride_h, kc_stride_s;
+  int64_t vc_stride_p, vc_stride_h, vc_stride_s;
+  int64_t mask_stride_b, mask_stride_t, mask_stride_j;
+  int64_t num_pages, page_table_stride, workspace_bytes;
+  int32_t page_size, max_pages;
+  int32_t head_dim;
+  int32_t dtype;                /* B200K_F16 | BF16 */
+  int32_t zero_padding;
+  float qk_scale;
+} b200k_paged_attention_args;
+
+int b200k_paged_attention(const b200k_paged_attention_args* args, b200k_stream stream);
+/* Scratch for partial results of sequences that several CTAs share; contents irrelevant before
+ * and after the call, not to be shared by calls that may run at the same time. */
+int64_t b200k_paged_attention_workspace_bytes(const b200k_paged_attention_args* args);
+
 #ifdef __cplusplus
 }
 #endif

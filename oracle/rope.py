@@ -114,11 +114,15 @@ def paged_attention_ref(q, k_cache, v_cache, page_table, cache_lens, new_lens=No
         for h in range(hq):
             hk = h // (hq // hkv)
             keys, values = (c[pages, hk, at % size].double() for c in (k_cache, v_cache))
-            for t in range(n):
+            if bool(torch.isfinite(keys).all() and torch.isfinite(values).all()):
+                score = q[b, h, :n].double() @ keys.T * scale
+                p = torch.softmax(score.masked_fill(~sees, -math.inf), dim=1)
+                p[~sees.any(1)] = 0.0
+                out[b, h, :n], mag[b, h, :n] = p @ values, p @ values.abs()
+                continue
+            for t in range(n):               # only what the query sees takes part, row by row
                 who = sees[t]
-                if not bool(who.any()):
-                    continue
-                p = torch.softmax(keys[who] @ q[b, h, t].double() * scale, dim=0)
-                out[b, h, t] = p @ values[who]
-                mag[b, h, t] = p @ values[who].abs()
+                if bool(who.any()):
+                    p = torch.softmax(keys[who] @ q[b, h, t].double() * scale, dim=0)
+                    out[b, h, t], mag[b, h, t] = p @ values[who], p @ values[who].abs()
     return out, mag
