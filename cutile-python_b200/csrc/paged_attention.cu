@@ -390,8 +390,15 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         const uint32_t ph = it & 1;
         const int key0 = j * kPaBN;
         const bool edge = key0 + kPaBN > seq.have;       // the step's tokens, or slots behind the last one
+        if (!mbar_wait(bar(S_FULL), ph, abort_flag)) {
+          report_status(p.status, 96, j);
+          *abort_flag = 1;
+          ok = false;
+          break;
+        }
         if (edge) {
-          // row `row` of V: cleared where no token lies, and where a token of the step that some
+          // (S_FULL also says that P V of the last tile is done: only now is V_FULL's phase this
+          // tile's, and V this tile's rows.)  Row `row` of V is cleared where no token lies, and where a token of the step that some
           // query may not see is not finite (added by hand in the epilogue)
           if (!mbar_wait(bar(V_FULL), ph, abort_flag)) {
             report_status(p.status, 95, j);
@@ -420,12 +427,6 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
           __syncwarp();
           if (lane == 0) mbar_arrive(bar(EDGE_DONE));
           ++edges;
-        }
-        if (!mbar_wait(bar(S_FULL), ph, abort_flag)) {
-          report_status(p.status, 96, j);
-          *abort_flag = 1;
-          ok = false;
-          break;
         }
         tc_fence_after_sync();
         if (any_live) {                                   // a warp of padding rows only keeps step

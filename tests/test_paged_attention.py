@@ -173,6 +173,22 @@ def test_many_short_sequences(device_ok):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("b,hq,hkv,t,d,lens,tree", [
+    (16, 32, 8, 1, 128, [3333 + 67 * i for i in range(16)], False),     # a dozen tiles a CTA
+    (12, 8, 2, 16, 128, [5000 + 131 * i for i in range(12)], True),
+    (9, 8, 2, 60, 64, [4100 - 77 * i for i in range(9)], True)])        # two row tiles
+def test_many_tiles_in_a_row(b, hq, hkv, t, d, lens, tree, device_ok):
+    # long runs inside one CTA: the last tile's rows of V are cleared only after the tile before
+    # has been used
+    c = Cache(b, hq, hkv, t, d, torch.bfloat16, 32, lens)
+    mask = _tree(b, t) if tree else None
+    first = c.run(tree_mask=mask)
+    c.check(first, mask)
+    for _ in range(3):
+        assert torch.equal(c.run(tree_mask=mask), first)
+
+
+@pytest.mark.gpu
 def test_masks_that_leave_rows_empty(device_ok):
     for lens in ([0, 0], [0, 200]):
         c = Cache(2, 4, 2, 6, 64, torch.bfloat16, 16, lens)
