@@ -353,6 +353,50 @@ class LaunchCache:
             check(code)
 
 
+def layout(*tensors) -> tuple:
+    """What a wrapper's checks and argument struct depend on: everything about the tensors but
+    their addresses and contents."""
+    return tuple([None if t is None else (t.shape, t.stride(), t.dtype, t.device, t.requires_grad)
+                  for t in tensors])
+
+
+class LayoutPlans:
+    """Checked calls of one entry point, remembered by the layouts (and scalars) that passed:
+    the argument struct with all but its pointers filled in, as bytes, plus what else the
+    wrapper derived.  A call copies the struct and sets its own pointers, so threads and streams
+    share nothing.  Checking and filling in forty fields costs 10 us of a 20 us call, the
+    lookup 3."""
+
+    def __init__(self, entry_name: str, struct: type, limit: int = 1024):
+        self.entry_name, self.struct, self.limit = entry_name, struct, limit
+        self.plans: dict = {}
+        self.fn = None
+
+    def get(self, key):
+        return self.plans.get(key)
+
+    def put(self, key, args, *extra):
+        if len(self.plans) >= self.limit:
+            self.plans.clear()
+        plan = self.plans[key] = (bytes(args), *extra)
+        return plan
+
+    def args(self, plan):
+        return self.struct.from_buffer_copy(plan[0])
+
+    def launch(self, args, device: torch.device) -> None:
+        if self.fn is None:
+            self.fn = getattr(lib(), self.entry_name)
+        index = device.index
+        if torch.cuda.current_device() == index:
+            code = self.fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(index))
+        else:
+            with torch.cuda.device(device):
+                code = self.fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(index))
+        if code < 0:
+            check(code)
+
+
 def device_status() -> tuple[int, int]:
     """(code, info) of the current device's status word; synchronise the stream first."""
     code, info = c_int(0), c_int(0)

@@ -20,8 +20,11 @@ import math
 import torch
 
 from . import _lib
-from .rope import (check_no_grad, check_out, check_positions, check_table, check_weights, launch,
-                   rows_view)
+from .rope import (aligned_table, check_no_grad, check_out, check_positions, check_table, check_weights,
+                   empty_rows, rows_view)
+
+_APPEND = _lib.LayoutPlans("b200k_paged_kv_append", _lib.PagedKvAppendArgs)
+_ATTENTION = _lib.LayoutPlans("b200k_paged_attention", _lib.PagedAttentionArgs)
 
 
 def _check_cache(k_cache, v_cache, page_table, cache_lens, new_lens, batch, heads, dim, dtype, device):
@@ -73,6 +76,38 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
     new_lens[b] are padding: their cache slots stay as they are, as do their rows of a given
     ``q_out``; in a q_out made here they are zero.  A token whose page lies outside the table
     or the cache is not stored, and ``raise_on_device_error()`` names its sequence."""
+    k, v, q = rows_view(k), rows_view(v), rows_view(q)
+    cos, sin = aligned_table(cos, sin)
+    key = (_lib.layout(k, v, q, k_cache, v_cache, page_table, cache_lens, cos, sin, q_weight, k_weight, positions,
+                       new_lens, q_out), eps, interleaved, torch.is_grad_enabled())
+    plan = _APPEND.get(key)
+    if plan is None:
+        plan = _APPEND.put(key, _append_args(k, v, k_cache, v_cache, page_table, cache_lens, cos, sin, q, q_weight,
+                                             k_weight, positions, new_lens, eps, interleaved, q_out))
+    a = _APPEND.args(plan)
+    a.k, a.v, a.k_cache, a.v_cache = k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
+    a.page_table, a.cache_lens = page_table.data_ptr(), cache_lens.data_ptr()
+    if new_lens is not None:
+        a.new_lens = new_lens.data_ptr()
+    if cos is not None:
+        a.cos, a.sin = cos.data_ptr(), sin.data_ptr()
+    if k_weight is not None:
+        a.k_weight = k_weight.data_ptr()
+    if positions is not None:
+        a.positions = positions.data_ptr()
+    if q is not None:
+        if q_out is None:
+            q_out = empty_rows(q)
+        a.q, a.q_out = q.data_ptr(), q_out.data_ptr()
+        if q_weight is not None:
+            a.q_weight = q_weight.data_ptr()
+    _APPEND.launch(a, k.device)
+    return q_out
+
+
+def _append_args(k, v, k_cache, v_cache, page_table, cache_lens, cos, sin, q, q_weight, k_weight, positions,
+                 new_lens, eps, interleaved, q_out):
+    """Checks a call; every field of it but the pointers."""
     if k.ndim != 4 or k.shape != v.shape:
         raise ValueError("k and v must both be 4D (Batch, KV_Heads, SeqLen, Dim).")
     if not k.is_cuda or v.device != k.device:
@@ -92,30 +127,21 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
     if q is None and (q_weight is not None or q_out is not None):
         raise ValueError("q_weight and q_out need q")
     a = _lib.PagedKvAppendArgs()
-    rotary = 0
     if cos is not None:
-        cos, sin, rotary = check_table(cos, sin, dim, device)
-        a.cos, a.sin = cos.data_ptr(), sin.data_ptr()
+        a.rotary_dim = check_table(cos, sin, dim, device)
         a.table_rows, a.table_stride = cos.shape[0], cos.stride(0)
     weight_dtype = check_weights(dim, k.dtype, device, q_weight, k_weight)
-    a.positions, a.position_stride_b, a.position_stride_t, a.positions_are_int64 = check_positions(
-        positions, batch, tokens, device)
-    qo = None
+    a.position_stride_b, a.position_stride_t, a.positions_are_int64 = check_positions(positions, batch, tokens, device)
     if q is not None:
         if q.ndim != 4 or (q.shape[0], q.shape[2], q.shape[3]) != (batch, tokens, dim):
             raise ValueError("q must be (Batch, Heads, SeqLen, Dim) like k.")
         if q.device != device or q.dtype != k.dtype:
             raise ValueError("q must have the device and data type of k.")
-        qo = torch.empty(q.shape, dtype=q.dtype, device=device) if q_out is None else check_out(q_out, q, "q_out")
-        q = rows_view(q)
-        a.q, a.q_out, a.q_weight, a.heads_q = q.data_ptr(), qo.data_ptr(), _lib.ptr(q_weight), q.shape[1]
+        a.zero_padding = 1 if q_out is None else 0
+        qo = empty_rows(q) if q_out is None else check_out(q_out, q, "q_out")
+        a.heads_q = q.shape[1]
         a.q_stride_b, a.q_stride_h, a.q_stride_t, _ = q.stride()
         a.qo_stride_b, a.qo_stride_h, a.qo_stride_t, _ = qo.stride()
-        a.zero_padding = 1 if q_out is None else 0
-    k, v = rows_view(k), rows_view(v)
-    a.k, a.v, a.k_cache, a.v_cache = k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
-    a.k_weight = _lib.ptr(k_weight)
-    a.page_table, a.cache_lens, a.new_lens = page_table.data_ptr(), cache_lens.data_ptr(), _lib.ptr(new_lens)
     a.batch, a.tokens, a.heads_kv = batch, tokens, heads
     a.k_stride_b, a.k_stride_h, a.k_stride_t, _ = k.stride()
     a.v_stride_b, a.v_stride_h, a.v_stride_t, _ = v.stride()
@@ -123,10 +149,9 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
     a.vc_stride_p, a.vc_stride_h, a.vc_stride_s, _ = v_cache.stride()
     a.num_pages, a.page_size = k_cache.shape[0], k_cache.shape[2]
     a.max_pages, a.page_table_stride = page_table.shape[1], page_table.stride(0)
-    a.head_dim, a.rotary_dim, a.interleaved = dim, rotary, 1 if interleaved else 0
+    a.head_dim, a.interleaved = dim, 1 if interleaved else 0
     a.dtype, a.weight_dtype, a.eps = _lib.dtype_enum(k.dtype), _lib.dtype_enum(weight_dtype), eps
-    launch("b200k_paged_kv_append", a, device)
-    return qo
+    return a
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -144,6 +169,34 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     of a multiple of 8 tokens, qk_scale positive (None: 1 / sqrt(Dim)).  A query that sees no token gives zeros.  Slots that hold none of
     the sequence's tokens are never used.  Rows behind new_lens[b] are padding: they stay as
     they are in a given ``out`` and are zero in one made here."""
+    q = rows_view(q)
+    key = (_lib.layout(q, k_cache, v_cache, page_table, cache_lens, new_lens, tree_mask, out), qk_scale,
+           torch.is_grad_enabled())
+    plan = _ATTENTION.get(key)
+    if plan is None:
+        a = _attention_args(q, k_cache, v_cache, page_table, cache_lens, new_lens, tree_mask, qk_scale, out)
+        with torch.cuda.device(q.device):
+            a.workspace_bytes = _lib.lib().b200k_paged_attention_workspace_bytes(ctypes.byref(a))
+        plan = _ATTENTION.put(key, a, a.workspace_bytes)
+    if (k_cache.data_ptr() | v_cache.data_ptr()) % 16:
+        raise ValueError("the caches must start on 16-byte boundaries")
+    if out is None:
+        out = empty_rows(q)
+    # made per call: calls on other streams and other captured graphs have their own
+    workspace = torch.empty(plan[1], dtype=torch.uint8, device=q.device)
+    a = _ATTENTION.args(plan)
+    a.q, a.k_cache, a.v_cache, a.out = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr()
+    a.page_table, a.cache_lens, a.workspace = page_table.data_ptr(), cache_lens.data_ptr(), workspace.data_ptr()
+    if new_lens is not None:
+        a.new_lens = new_lens.data_ptr()
+    if tree_mask is not None:
+        a.tree_mask = tree_mask.data_ptr()
+    _ATTENTION.launch(a, q.device)
+    return out
+
+
+def _attention_args(q, k_cache, v_cache, page_table, cache_lens, new_lens, tree_mask, qk_scale, out):
+    """Checks a call; every field of it but the pointers."""
     if q.ndim != 4:
         raise ValueError("q must be 4D (Batch, Heads, SeqLen, Dim).")
     if not q.is_cuda:
@@ -164,10 +217,10 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     qk_scale = 1.0 / math.sqrt(dim) if qk_scale is None else float(qk_scale)
     if not 0.0 < qk_scale < 3.0e38:
         raise ValueError("qk_scale must be positive and finite")
-    a = _lib.PagedAttentionArgs()
     for c, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-        if c.data_ptr() % 16 or any(s % 8 for s in c.stride()[:3]):
-            raise ValueError(f"{name} must start on a 16-byte boundary with strides of whole 16-byte units")
+        if any(s % 8 for s in c.stride()[:3]):
+            raise ValueError(f"{name} must have strides of whole 16-byte units")
+    a = _lib.PagedAttentionArgs()
     if tree_mask is not None:
         if tree_mask.dtype != torch.bool:
             raise TypeError("tree_mask must be bool")
@@ -180,28 +233,14 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         else:
             raise ValueError(f"tree_mask must be ({tokens}, {tokens}) or ({batch}, {tokens}, {tokens}), "
                              f"got {tuple(tree_mask.shape)}")
-        a.tree_mask = tree_mask.data_ptr()
     a.zero_padding = 1 if out is None else 0
-    out = torch.empty(q.shape, dtype=q.dtype, device=device) if out is None else check_out(out, q, "out")
-    q = rows_view(q)
-    a.q, a.k_cache, a.v_cache, a.out = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr()
-    a.page_table, a.cache_lens, a.new_lens = page_table.data_ptr(), cache_lens.data_ptr(), _lib.ptr(new_lens)
+    o = empty_rows(q) if out is None else check_out(out, q, "out")
     a.batch, a.tokens, a.heads_q, a.heads_kv = batch, tokens, heads, heads_kv
     a.q_stride_b, a.q_stride_h, a.q_stride_t, _ = q.stride()
-    a.o_stride_b, a.o_stride_h, a.o_stride_t, _ = out.stride()
+    a.o_stride_b, a.o_stride_h, a.o_stride_t, _ = o.stride()
     a.kc_stride_p, a.kc_stride_h, a.kc_stride_s, _ = k_cache.stride()
     a.vc_stride_p, a.vc_stride_h, a.vc_stride_s, _ = v_cache.stride()
     a.num_pages, a.page_size = k_cache.shape[0], k_cache.shape[2]
     a.max_pages, a.page_table_stride = page_table.shape[1], page_table.stride(0)
-    a.head_dim, a.dtype = dim, _lib.dtype_enum(q.dtype)
-    a.qk_scale = qk_scale
-    if torch.cuda.current_device() == device.index:
-        size = _lib.lib().b200k_paged_attention_workspace_bytes(ctypes.byref(a))
-    else:
-        with torch.cuda.device(device):
-            size = _lib.lib().b200k_paged_attention_workspace_bytes(ctypes.byref(a))
-    # made per call: calls on other streams and other captured graphs have their own
-    workspace = torch.empty(size, dtype=torch.uint8, device=device)
-    a.workspace, a.workspace_bytes = workspace.data_ptr(), size
-    launch("b200k_paged_attention", a, device)
-    return out
+    a.head_dim, a.dtype, a.qk_scale = dim, _lib.dtype_enum(q.dtype), qk_scale
+    return a

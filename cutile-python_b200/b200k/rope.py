@@ -25,9 +25,9 @@ def rope_table(max_positions: int, rotary_dim: int, theta: float = 10000.0,
     return angle.cos().float(), angle.sin().float()
 
 
-def rows_view(t: torch.Tensor) -> torch.Tensor:
+def rows_view(t: torch.Tensor | None) -> torch.Tensor | None:
     """The tensor itself where its rows are contiguous, else a copy that has them so."""
-    return t if t.stride(-1) == 1 else t.contiguous()
+    return t if t is None or t.stride(-1) == 1 or not t.numel() else t.contiguous()
 
 
 def check_no_grad(name: str, instead: str, *tensors) -> None:
@@ -45,8 +45,8 @@ def check_out(t: torch.Tensor, like: torch.Tensor, name: str) -> torch.Tensor:
     return t
 
 
-def check_table(cos: torch.Tensor, sin: torch.Tensor, dim: int, device: torch.device):
-    """(cos, sin, rotary_dim) with equal row strides."""
+def check_table(cos: torch.Tensor, sin: torch.Tensor, dim: int, device: torch.device) -> int:
+    """rotary_dim of a pair of tables."""
     if cos.ndim != 2 or cos.shape != sin.shape:
         raise ValueError("cos and sin must both be (positions, rotary_dim / 2)")
     if cos.dtype != torch.float32 or sin.dtype != torch.float32:
@@ -58,16 +58,13 @@ def check_table(cos: torch.Tensor, sin: torch.Tensor, dim: int, device: torch.de
         raise ValueError(f"rotary_dim must be a multiple of 16 up to the head dimension (got {rotary} of {dim})")
     if cos.shape[0] == 0:
         raise ValueError("the rotation table has no positions")
-    if (cos.stride() != sin.stride() or cos.stride(1) != 1 or cos.stride(0) % 4
-            or (cos.data_ptr() | sin.data_ptr()) % 16):
-        cos, sin = (torch.empty(cos.shape, dtype=torch.float32, device=device).copy_(t) for t in (cos, sin))
-    return cos, sin, rotary
+    return rotary
 
 
 def check_positions(positions: torch.Tensor | None, batch: int, tokens: int, device: torch.device):
-    """(pointer, batch stride, token stride, is int64)"""
+    """(batch stride, token stride, is int64)"""
     if positions is None:
-        return None, 0, 0, 0
+        return 0, 0, 0
     if positions.dtype not in (torch.int32, torch.int64):
         raise TypeError("positions must be int32 or int64")
     if positions.device != device:
@@ -78,7 +75,7 @@ def check_positions(positions: torch.Tensor | None, batch: int, tokens: int, dev
         stride_b, stride_t = positions.stride()
     else:
         raise ValueError(f"positions must be ({tokens},) or ({batch}, {tokens}), got {tuple(positions.shape)}")
-    return positions.data_ptr(), stride_b, stride_t, int(positions.dtype == torch.int64)
+    return stride_b, stride_t, int(positions.dtype == torch.int64)
 
 
 def check_weights(dim: int, dtype: torch.dtype, device: torch.device, *weights) -> torch.dtype:
@@ -116,28 +113,29 @@ def _check_rows(q: torch.Tensor, k: torch.Tensor) -> None:
         raise ValueError("the head dimension must be a multiple of 8 up to 256")
 
 
-def launch(entry: str, args: ctypes.Structure, device: torch.device) -> None:
-    """Calls an entry point on the device's current stream."""
-    fn = getattr(_lib.lib(), entry)
-    index = device.index
-    if index is None or torch.cuda.current_device() == index:
-        code = fn(ctypes.byref(args), _lib.stream_ptr(device))
-    else:
-        with torch.cuda.device(device):
-            code = fn(ctypes.byref(args), _lib.stream_ptr(device))
-    if code < 0:
-        _lib.check(code)
+def empty_rows(like: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(like, memory_format=torch.contiguous_format)
+
+
+def aligned_table(cos, sin):
+    """The tables themselves, or 16-byte aligned copies of a common layout."""
+    if cos is None or sin is None or ((cos.data_ptr() | sin.data_ptr()) % 16 == 0 and cos.stride() == sin.stride()
+                                      and cos.stride(-1) == 1 and cos.stride(0) % 4 == 0):
+        return cos, sin
+    return tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t) for t in (cos, sin))
+
+
+_FORWARD = _lib.LayoutPlans("b200k_qk_norm_rope", _lib.QkNormRopeArgs)
+_BACKWARD = _lib.LayoutPlans("b200k_qk_norm_rope_backward", _lib.QkNormRopeArgs)
 
 
 def _fill(a, q, k, q_out, k_out, q_weight, k_weight, cos, sin, positions, eps, interleaved):
+    """Every field of a checked call but its pointers."""
     batch, heads, tokens, dim = q.shape
-    cos, sin, rotary = check_table(cos, sin, dim, q.device)
+    rotary = check_table(cos, sin, dim, q.device)
     weight_dtype = check_weights(dim, q.dtype, q.device, q_weight, k_weight)
-    a.q, a.k, a.q_out, a.k_out = q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr()
-    a.q_weight, a.k_weight = _lib.ptr(q_weight), _lib.ptr(k_weight)
-    a.cos, a.sin = cos.data_ptr(), sin.data_ptr()
     a.table_rows, a.table_stride = cos.shape[0], cos.stride(0)
-    a.positions, a.position_stride_b, a.position_stride_t, a.positions_are_int64 = check_positions(
+    a.position_stride_b, a.position_stride_t, a.positions_are_int64 = check_positions(
         positions, batch, tokens, q.device)
     a.batch, a.tokens, a.heads_q, a.heads_kv = batch, tokens, heads, k.shape[1]
     a.q_stride_b, a.q_stride_h, a.q_stride_t, _ = q.stride()
@@ -146,7 +144,17 @@ def _fill(a, q, k, q_out, k_out, q_weight, k_weight, cos, sin, positions, eps, i
     a.ko_stride_b, a.ko_stride_h, a.ko_stride_t, _ = k_out.stride()
     a.head_dim, a.rotary_dim, a.interleaved = dim, rotary, 1 if interleaved else 0
     a.dtype, a.weight_dtype, a.eps = _lib.dtype_enum(q.dtype), _lib.dtype_enum(weight_dtype), eps
-    return cos, sin
+
+
+def _point(a, q, k, q_out, k_out, q_weight, k_weight, cos, sin, positions):
+    a.q, a.k, a.q_out, a.k_out = q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr()
+    a.cos, a.sin = cos.data_ptr(), sin.data_ptr()
+    if q_weight is not None:
+        a.q_weight = q_weight.data_ptr()
+    if k_weight is not None:
+        a.k_weight = k_weight.data_ptr()
+    if positions is not None:
+        a.positions = positions.data_ptr()
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor,
@@ -166,14 +174,27 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor,
     Pairs are (i, i + rotary_dim / 2), or neighbours with ``interleaved``.  ``q_out`` / ``k_out``
     may be q / k themselves.  A position outside the table gives NaN rows, and
     ``raise_on_device_error()`` names it."""
-    _check_rows(q, k)
-    check_no_grad("qk_norm_rope", " and take gradients from qk_norm_rope_backward", q, k, q_weight, k_weight)
-    qo = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else check_out(q_out, q, "q_out")
-    ko = torch.empty(k.shape, dtype=k.dtype, device=k.device) if k_out is None else check_out(k_out, k, "k_out")
     q, k = rows_view(q), rows_view(k)
-    a = _lib.QkNormRopeArgs()
-    keep = _fill(a, q, k, qo, ko, q_weight, k_weight, cos, sin, positions, eps, interleaved)  # noqa: F841
-    launch("b200k_qk_norm_rope", a, q.device)
+    cos, sin = aligned_table(cos, sin)
+    key = (_lib.layout(q, k, q_weight, k_weight, cos, sin, positions, q_out, k_out), eps, interleaved,
+           torch.is_grad_enabled())
+    plan = _FORWARD.get(key)
+    qo, ko = q_out, k_out
+    if plan is None:
+        _check_rows(q, k)
+        check_no_grad("qk_norm_rope", " and take gradients from qk_norm_rope_backward", q, k, q_weight, k_weight)
+        qo = empty_rows(q) if q_out is None else check_out(q_out, q, "q_out")
+        ko = empty_rows(k) if k_out is None else check_out(k_out, k, "k_out")
+        a = _lib.QkNormRopeArgs()
+        _fill(a, q, k, qo, ko, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+        plan = _FORWARD.put(key, a)
+    if qo is None:
+        qo = empty_rows(q)
+    if ko is None:
+        ko = empty_rows(k)
+    a = _FORWARD.args(plan)
+    _point(a, q, k, qo, ko, q_weight, k_weight, cos, sin, positions)
+    _FORWARD.launch(a, q.device)
     return qo, ko
 
 
@@ -186,25 +207,38 @@ def qk_norm_rope_backward(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k
     qk_norm_rope's outputs and its inputs (in-place outputs lose them).  The weights' gradients
     are summed in fp32 over all rows in a fixed order and rounded to the weights' dtype; None
     for a weight of None."""
-    _check_rows(q, k)
-    check_no_grad("qk_norm_rope_backward", "", dq, dk, q, k, q_weight, k_weight)
-    for g, x, name in ((dq, q, "dq"), (dk, k, "dk")):
-        if g.shape != x.shape or g.dtype != x.dtype or g.device != x.device:
-            raise ValueError(f"{name} must have the shape, dtype and device of {name[1]}")
-    q_in, k_in = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k))
     q, k, dq, dk = rows_view(q), rows_view(k), rows_view(dq), rows_view(dk)
-    a = _lib.QkNormRopeArgs()
-    keep = _fill(a, q, k, q_in, k_in, q_weight, k_weight, cos, sin, positions, eps, interleaved)  # noqa: F841
+    cos, sin = aligned_table(cos, sin)
+    key = (_lib.layout(dq, dk, q, k, q_weight, k_weight, cos, sin, positions), eps, interleaved,
+           torch.is_grad_enabled())
+    plan = _BACKWARD.get(key)
+    if plan is None:
+        _check_rows(q, k)
+        check_no_grad("qk_norm_rope_backward", "", dq, dk, q, k, q_weight, k_weight)
+        for g, x, name in ((dq, q, "dq"), (dk, k, "dk")):
+            if g.shape != x.shape or g.dtype != x.dtype or g.device != x.device:
+                raise ValueError(f"{name} must have the shape, dtype and device of {name[1]}")
+        a = _lib.QkNormRopeArgs()
+        _fill(a, q, k, empty_rows(q), empty_rows(k), q_weight, k_weight, cos, sin, positions, eps, interleaved)
+        a.dq_stride_b, a.dq_stride_h, a.dq_stride_t, _ = dq.stride()
+        a.dk_stride_b, a.dk_stride_h, a.dk_stride_t, _ = dk.stride()
+        if q_weight is not None or k_weight is not None:
+            with torch.cuda.device(q.device):
+                a.workspace_bytes = _lib.lib().b200k_qk_norm_rope_backward_workspace_bytes(ctypes.byref(a))
+        plan = _BACKWARD.put(key, a, a.workspace_bytes)
+    q_in, k_in = empty_rows(q), empty_rows(k)
+    a = _BACKWARD.args(plan)
+    _point(a, q, k, q_in, k_in, q_weight, k_weight, cos, sin, positions)
     a.dq_out, a.dk_out = dq.data_ptr(), dk.data_ptr()
-    a.dq_stride_b, a.dq_stride_h, a.dq_stride_t, _ = dq.stride()
-    a.dk_stride_b, a.dk_stride_h, a.dk_stride_t, _ = dk.stride()
-    dqw, dkw = (None if w is None else torch.empty_like(w) for w in (q_weight, k_weight))
-    a.dq_weight, a.dk_weight = _lib.ptr(dqw), _lib.ptr(dkw)
-    workspace = None
-    if dqw is not None or dkw is not None:
-        with torch.cuda.device(q.device):
-            size = _lib.lib().b200k_qk_norm_rope_backward_workspace_bytes(ctypes.byref(a))
-        workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
-        a.workspace, a.workspace_bytes = workspace.data_ptr(), size
-    launch("b200k_qk_norm_rope_backward", a, q.device)
+    dqw = dkw = workspace = None
+    if q_weight is not None:
+        dqw = torch.empty_like(q_weight)
+        a.dq_weight = dqw.data_ptr()
+    if k_weight is not None:
+        dkw = torch.empty_like(k_weight)
+        a.dk_weight = dkw.data_ptr()
+    if plan[1]:
+        workspace = torch.empty(plan[1], dtype=torch.uint8, device=q.device)
+        a.workspace = workspace.data_ptr()
+    _BACKWARD.launch(a, q.device)
     return q_in, k_in, dqw, dkw
