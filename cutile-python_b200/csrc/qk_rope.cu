@@ -27,6 +27,8 @@ namespace {
 
 constexpr int kRopeThreads = 128;
 constexpr int kMaxHeads = 65536;
+constexpr int kBackwardStages = 5;      // rows of 16-bit values on their way to a lane group
+constexpr int kBackwardMinBlocks = 4;
 
 // One tensor of a call: (batch, heads, tokens, D) rows in, rows out.
 struct RopeSide {
@@ -38,6 +40,7 @@ struct RopeSide {
   int64_t x_b, x_h, x_t, dy_b, dy_h, dy_t, y_b, y_h, y_t;   // elements; paged output: page, head, slot
   int heads;
   int chunks;            // ceil(heads / heads per group)
+  int log_per;           // backward: log2 of the heads per group
   int rotate;
   int paged;
   int zero_padding;      // tokens behind new_lens[b] give zero rows (else they are left alone)
@@ -82,70 +85,110 @@ template <typename T> struct Oct {
   uint4 q[kWords];
 };
 
-template <typename T, bool VEC>
-__device__ __forceinline__ Oct<T> load_oct(const T* p) {
-  Oct<T> o;
-  if constexpr (VEC) {
+// A lane's sixteen values as the pairs (lo, hi) that a rotation turns, two pairs to a register
+// pair: fp32 products and sums are issued two at a time.  Half split: lo is the first vector, hi
+// the second.  Interleaved: lo the even, hi the odd elements of both.
+struct Pairs {
+  float2 lo[4], hi[4];
+};
+template <bool INTER>
+__device__ __forceinline__ Pairs to_pairs(const float (&a)[8], const float (&b)[8]) {
+  Pairs r;
 #pragma unroll
-    for (int i = 0; i < Oct<T>::kWords; ++i) o.q[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
-  } else {
-    T* e = reinterpret_cast<T*>(&o);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = p[i];
+  for (int k = 0; k < 4; ++k) {
+    if constexpr (INTER) {
+      const float* e = k < 2 ? a + 4 * k : b + 4 * (k - 2);
+      r.lo[k] = make_float2(e[0], e[2]);
+      r.hi[k] = make_float2(e[1], e[3]);
+    } else {
+      r.lo[k] = make_float2(a[2 * k], a[2 * k + 1]);
+      r.hi[k] = make_float2(b[2 * k], b[2 * k + 1]);
+    }
   }
-  return o;
+  return r;
 }
-
-template <typename T, bool VEC>
-__device__ __forceinline__ void store_oct(T* p, const float (&f)[8]) {
-  Oct<T> o;
-  T* e = reinterpret_cast<T*>(&o);
+template <bool INTER>
+__device__ __forceinline__ void from_pairs(const Pairs& r, float (&a)[8], float (&b)[8]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) e[i] = rope_from_f32<T>(f[i]);
-  if constexpr (VEC) {
-#pragma unroll
-    for (int i = 0; i < Oct<T>::kWords; ++i) reinterpret_cast<uint4*>(p)[i] = o.q[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) p[i] = e[i];
+  for (int k = 0; k < 4; ++k) {
+    if constexpr (INTER) {
+      float* e = k < 2 ? a + 4 * k : b + 4 * (k - 2);
+      e[0] = r.lo[k].x; e[1] = r.hi[k].x; e[2] = r.lo[k].y; e[3] = r.hi[k].y;
+    } else {
+      a[2 * k] = r.lo[k].x; a[2 * k + 1] = r.lo[k].y;
+      b[2 * k] = r.hi[k].x; b[2 * k + 1] = r.hi[k].y;
+    }
   }
 }
 
 template <typename T>
 __device__ __forceinline__ void unpack_oct(const Oct<T>& o, float (&f)[8]) {
-  const T* e = reinterpret_cast<const T*>(&o);
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&o);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = rope_to_f32<T>(e[i]);
-}
-
-template <typename T>
-__device__ __forceinline__ void load_weight(const RopeParams& p, const void* w, int col, float (&f)[8]) {
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] = __uint_as_float(w[i] << 16);
+      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  } else {
+    const T* e = reinterpret_cast<const T*>(&o);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    f[i] = p.w_is_f32 ? static_cast<const float*>(w)[col + i]
-                      : rope_to_f32<T>(static_cast<const T*>(w)[col + i]);
+    for (int i = 0; i < 8; ++i) f[i] = rope_to_f32<T>(e[i]);
   }
 }
 
-// A pair of the lane's values turned by (c, s); `back` turns the other way.
-__device__ __forceinline__ void turn(float& a, float& b, float c, float s) {
-  const float ta = a * c - b * s;
-  b = b * c + a * s;
-  a = ta;
-}
-
-// The lane's pairs: half split (lo[i], hi[i]); interleaved (lo[2i], lo[2i+1]), (hi[2i], hi[2i+1]).
-__device__ __forceinline__ void rotate_lane(float (&lo)[8], float (&hi)[8], const float (&c)[8], const float (&s)[8],
-                                            int interleaved) {
-  if (interleaved) {
+template <typename T, bool VEC>
+__device__ __forceinline__ void store_oct(T* p, const float (&f)[8]) {
+  Oct<T> o;
+  uint32_t* w = reinterpret_cast<uint32_t*>(&o);
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      turn(lo[2 * i], lo[2 * i + 1], c[i], s[i]);
-      turn(hi[2 * i], hi[2 * i + 1], c[4 + i], s[4 + i]);
-    }
+    for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(f[i]);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) turn(lo[i], hi[i], c[i], s[i]);
+    for (int i = 0; i < 4; ++i)
+      w[i] = std::is_same<T, __half>::value ? pack_f16x2(f[2 * i], f[2 * i + 1]) : pack_bf16x2(f[2 * i], f[2 * i + 1]);
+  }
+  if constexpr (VEC) {
+#pragma unroll
+    for (int i = 0; i < Oct<T>::kWords; ++i) reinterpret_cast<uint4*>(p)[i] = o.q[i];
+  } else {
+    const T* e = reinterpret_cast<const T*>(&o);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p[i] = e[i];
+  }
+}
+
+// Norm weights of a lane's columns; zeros where it has none.
+template <typename T, bool INTER, typename Columns>
+__device__ __forceinline__ Pairs load_weights(const void* w, int w_is_f32, const Columns& col) {
+  float a[8], b[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    a[i] = b[i] = 0.f;
+    if (w_is_f32) {
+      if (col.has_lo) a[i] = static_cast<const float*>(w)[col.lo + i];
+      if (col.has_hi) b[i] = static_cast<const float*>(w)[col.hi + i];
+    } else {
+      if (col.has_lo) a[i] = rope_to_f32<T>(static_cast<const T*>(w)[col.lo + i]);
+      if (col.has_hi) b[i] = rope_to_f32<T>(static_cast<const T*>(w)[col.hi + i]);
+    }
+  }
+  return to_pairs<INTER>(a, b);
+}
+
+// Cosines and sines of the lane's pairs; with `minus` the negated sines.
+struct Angles {
+  float2 c[4], s[4], minus[4];
+};
+// (lo, hi) -> (lo c - hi s, hi c + lo s); BACK turns the other way.
+template <bool BACK>
+__device__ __forceinline__ void rotate_pairs(Pairs& r, const Angles& g) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float2 lo = r.lo[k], hi = r.hi[k];
+    r.lo[k] = __ffma2_rn(lo, g.c[k], __fmul2_rn(hi, BACK ? g.s[k] : g.minus[k]));
+    r.hi[k] = __ffma2_rn(hi, g.c[k], __fmul2_rn(lo, BACK ? g.minus[k] : g.s[k]));
   }
 }
 
@@ -163,12 +206,13 @@ struct LaneColumns {
   bool rotated;
 };
 
+template <bool INTER>
 __device__ __forceinline__ LaneColumns lane_columns(const RopeParams& p, int unit) {
   LaneColumns c;
   c.rotated = unit < p.pairs;
   if (c.rotated) {
-    c.lo = p.interleaved ? unit * 16 : unit * 8;
-    c.hi = p.interleaved ? unit * 16 + 8 : unit * 8 + p.rotary / 2;
+    c.lo = INTER ? unit * 16 : unit * 8;
+    c.hi = INTER ? unit * 16 + 8 : unit * 8 + p.rotary / 2;
     c.has_lo = c.has_hi = true;
   } else {
     c.lo = p.rotary + (unit - p.pairs) * 16;
@@ -179,40 +223,109 @@ __device__ __forceinline__ LaneColumns lane_columns(const RopeParams& p, int uni
   return c;
 }
 
-// Cosines and sines of a token's position for the lane's pairs.  A position outside the table
-// is recorded in the status word and gives NaN rows: nothing is read out of range.
-__device__ __forceinline__ void load_angles(const RopeParams& p, int64_t b, int64_t t, const LaneColumns& col, int unit,
-                                            float (&c)[8], float (&s)[8]) {
-  int64_t pos;
+__device__ __forceinline__ int64_t position_of(const RopeParams& p, int64_t b, int64_t t) {
   if (p.positions != nullptr) {
     const int64_t at = b * p.pos_b + t * p.pos_t;
-    pos = p.pos_is_i64 ? static_cast<const int64_t*>(p.positions)[at] : static_cast<const int*>(p.positions)[at];
-  } else {
-    pos = (p.cache_lens != nullptr ? p.cache_lens[b] : 0) + t;
+    return p.pos_is_i64 ? static_cast<const int64_t*>(p.positions)[at] : static_cast<const int*>(p.positions)[at];
   }
+  return (p.cache_lens != nullptr ? p.cache_lens[b] : 0) + t;
+}
+
+// Cosines and sines of a position for the lane's pairs.  A position outside the table is recorded
+// in the status word and gives NaN rows: nothing is read out of range.
+__device__ __forceinline__ void load_angles(const RopeParams& p, int64_t pos, int64_t t, int unit, Angles& g) {
   if (pos < 0 || pos >= p.table_rows) {
     if (unit == 0) report_bad_index(p.status, kRolePosition, static_cast<int>(t));
+    const float nan = __int_as_float(0x7fc00000);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = s[i] = __int_as_float(0x7fc00000);
+    for (int k = 0; k < 4; ++k) g.c[k] = g.s[k] = g.minus[k] = make_float2(nan, nan);
     return;
   }
-  const float* cr = p.cos + pos * p.table_stride + unit * 8;
-  const float* sr = p.sin + pos * p.table_stride + unit * 8;
+  const float4* cr = reinterpret_cast<const float4*>(p.cos + pos * p.table_stride + unit * 8);
+  const float4* sr = reinterpret_cast<const float4*>(p.sin + pos * p.table_stride + unit * 8);
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const float4 cv = reinterpret_cast<const float4*>(cr)[i];
-    const float4 sv = reinterpret_cast<const float4*>(sr)[i];
-    c[4 * i] = cv.x; c[4 * i + 1] = cv.y; c[4 * i + 2] = cv.z; c[4 * i + 3] = cv.w;
-    s[4 * i] = sv.x; s[4 * i + 1] = sv.y; s[4 * i + 2] = sv.z; s[4 * i + 3] = sv.w;
+    const float4 c = cr[i], s = sr[i];
+    g.c[2 * i] = make_float2(c.x, c.y);
+    g.c[2 * i + 1] = make_float2(c.z, c.w);
+    g.s[2 * i] = make_float2(s.x, s.y);
+    g.s[2 * i + 1] = make_float2(s.z, s.w);
+    g.minus[2 * i] = make_float2(-s.x, -s.y);
+    g.minus[2 * i + 1] = make_float2(-s.z, -s.w);
   }
 }
 
-// Forward.  grid.x: one block per kRopeThreads / GS tokens; grid.y: (side, chunk of heads).
-// U rows are requested together before the first is used.
-template <typename T, int GS, bool VEC>
+// A lane's two vectors of a row (zeros where it has none), fetched into its own slots of shared
+// memory: [vector][16-byte piece][thread], so neighbouring threads hit neighbouring banks.  With
+// VEC the copies are asynchronous and cost no registers while they are in flight; a thread waits
+// for its own copies only, so no barrier is needed.
+template <typename T, bool VEC>
+__device__ __forceinline__ void stage_row(uint4* slot, const T* row, const LaneColumns& col, bool on) {
+  constexpr int kWords = Oct<T>::kWords;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const bool has = on && (half == 0 ? col.has_lo : col.has_hi);
+    const T* src = row + (half == 0 ? col.lo : col.hi);
+    if constexpr (VEC) {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) {
+        const uint32_t dst = smem_u32(slot + (half * kWords + i) * kRopeThreads);
+        // a source size of 0 fills the slot with zeros and reads nothing
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst),
+                     "l"(reinterpret_cast<uint64_t>(reinterpret_cast<const uint4*>(has ? src : row) + (has ? i : 0))),
+                     "r"(has ? 16 : 0)
+                     : "memory");
+      }
+    } else {
+      Oct<T> o = {};
+      T* e = reinterpret_cast<T*>(&o);
+      if (has) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = src[i];
+      }
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) slot[(half * kWords + i) * kRopeThreads] = o.q[i];
+    }
+  }
+}
+__device__ __forceinline__ void stage_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void stage_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+template <typename T, bool INTER>
+__device__ __forceinline__ Pairs read_staged(const uint4* slot) {
+  Oct<T> a, b;
+#pragma unroll
+  for (int i = 0; i < Oct<T>::kWords; ++i) {
+    a.q[i] = slot[i * kRopeThreads];
+    b.q[i] = slot[(Oct<T>::kWords + i) * kRopeThreads];
+  }
+  float x[8], y[8];
+  unpack_oct<T>(a, x);
+  unpack_oct<T>(b, y);
+  return to_pairs<INTER>(x, y);
+}
+template <typename T, bool INTER, bool VEC>
+__device__ __forceinline__ void store_pairs(T* row, const LaneColumns& col, const Pairs& r) {
+  float a[8], b[8];
+  from_pairs<INTER>(r, a, b);
+  if (col.has_lo) store_oct<T, VEC>(row + col.lo, a);
+  if (col.has_hi) store_oct<T, VEC>(row + col.hi, b);
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+// Forward.  grid.x: one block per kRopeThreads / GS tokens; grid.y: (side, chunk of heads).  All
+// rows of the chunk are requested at once, then normed and rotated batch by batch as they come.
+template <typename T> struct ForwardRows {          // heads a group walks; 16 KB of shared memory
+  static constexpr int kMax = sizeof(T) == 4 ? 2 : 4;
+};
+
+template <typename T, int GS, bool INTER, bool VEC>
 __global__ void __launch_bounds__(kRopeThreads)
 qk_rope_kernel(const __grid_constant__ RopeParams p) {
-  constexpr int U = sizeof(T) == 4 ? 2 : 4;
+  constexpr int kRows = ForwardRows<T>::kMax, kBatch = kRows / 2;
+  constexpr int kSlot = 2 * Oct<T>::kWords * kRopeThreads;
+  __shared__ uint4 stage[kRows * kSlot];
+  uint4* mine = stage + threadIdx.x;
   const int unit = threadIdx.x % GS;
   const int64_t n = static_cast<int64_t>(blockIdx.x) * (kRopeThreads / GS) + threadIdx.x / GS;
   int chunk = blockIdx.y, which = 0;
@@ -220,8 +333,19 @@ qk_rope_kernel(const __grid_constant__ RopeParams p) {
   const RopeSide& sd = p.side[which];
   const bool live = n < p.total_tokens;
   const int64_t b = live ? n / p.tokens : 0, t = live ? n - b * p.tokens : 0;
-  const LaneColumns col = lane_columns(p, unit);
+  const LaneColumns col = lane_columns<INTER>(p, unit);
   const bool padded = live && p.new_lens != nullptr && t >= p.new_lens[b];
+
+  const T* x = static_cast<const T*>(sd.x) + b * sd.x_b + t * sd.x_t;
+  const int h_begin = chunk * p.heads_per_group;
+  const int rows = min(sd.heads - h_begin, p.heads_per_group);   // at most kRows
+#pragma unroll
+  for (int u = 0; u < kRows; ++u) {
+    const bool on = live && !padded && u < rows;
+    stage_row<T, VEC>(mine + u * kSlot, x + (on ? h_begin + u : 0) * sd.x_h, col, on);
+    if (u == kBatch - 1) stage_commit();
+  }
+  stage_commit();
 
   // where this token's rows go
   int64_t out = b * sd.y_b + t * sd.y_t;
@@ -238,171 +362,196 @@ qk_rope_kernel(const __grid_constant__ RopeParams p) {
       out = page * sd.y_b + (at - entry * p.page_size) * sd.y_t;
     }
   }
-  const bool read = store && !padded;
-
-  float c[8], s[8], wlo[8], whi[8];
-  const bool rotate = sd.rotate != 0 && col.rotated && read;
-  if (rotate) load_angles(p, b, t, col, unit, c, s);
+  Angles angles;
+  const bool rotate = sd.rotate != 0 && col.rotated && store && !padded;
+  if (rotate) load_angles(p, position_of(p, b, t), t, unit, angles);
   const bool norm = sd.w != nullptr;
-  if (norm) {
-    if (col.has_lo) load_weight<T>(p, sd.w, col.lo, wlo);
-    if (col.has_hi) load_weight<T>(p, sd.w, col.hi, whi);
-  }
+  Pairs w;
+  if (norm) w = load_weights<T, INTER>(sd.w, p.w_is_f32, col);
 
-  const T* x = static_cast<const T*>(sd.x) + b * sd.x_b + t * sd.x_t;
-  T* y = static_cast<T*>(sd.y) + out;
-  const int h_end = min(sd.heads, (chunk + 1) * p.heads_per_group);
-  for (int h0 = chunk * p.heads_per_group; h0 < h_end; h0 += U) {
-    Oct<T> lo[U], hi[U];
+  T* y = static_cast<T*>(sd.y) + out + h_begin * sd.y_h;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const bool on = read && h0 + u < h_end;
-      lo[u] = hi[u] = Oct<T>{};
-      if (on && col.has_lo) lo[u] = load_oct<T, VEC>(x + (h0 + u) * sd.x_h + col.lo);
-      if (on && col.has_hi) hi[u] = load_oct<T, VEC>(x + (h0 + u) * sd.x_h + col.hi);
-    }
+  for (int batch = 0; batch < 2; ++batch) {
+    if (batch == 0) stage_wait<1>();
+    else stage_wait<0>();
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float a[8], d[8];
-      unpack_oct<T>(lo[u], a);
-      unpack_oct<T>(hi[u], d);
+    for (int v = 0; v < kBatch; ++v) {
+      const int u = batch * kBatch + v;
+      if (u >= rows) break;                      // the same for the whole block
+      Pairs r = read_staged<T, INTER>(mine + u * kSlot);
       if (norm) {
-        float sq = 0.f;
+        float2 sq = both(0.f), sq2 = both(0.f);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sq += a[i] * a[i] + d[i] * d[i];
-        const float r = rsqrtf(group_sum<GS>(sq) * p.inv_dim + p.eps);
+        for (int k = 0; k < 4; ++k) {
+          sq = __ffma2_rn(r.lo[k], r.lo[k], sq);
+          sq2 = __ffma2_rn(r.hi[k], r.hi[k], sq2);
+        }
+        sq = __fadd2_rn(sq, sq2);
+        const float2 inv = both(rsqrtf(group_sum<GS>(sq.x + sq.y) * p.inv_dim + p.eps));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          a[i] *= r * wlo[i];
-          d[i] *= r * whi[i];
+        for (int k = 0; k < 4; ++k) {
+          r.lo[k] = __fmul2_rn(r.lo[k], __fmul2_rn(inv, w.lo[k]));
+          r.hi[k] = __fmul2_rn(r.hi[k], __fmul2_rn(inv, w.hi[k]));
         }
       }
-      if (rotate) rotate_lane(a, d, c, s, p.interleaved);
+      if (rotate) rotate_pairs<false>(r, angles);
       if (padded) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) a[i] = d[i] = 0.f;
+        for (int k = 0; k < 4; ++k) r.lo[k] = r.hi[k] = both(0.f);
       }
-      if (store && h0 + u < h_end) {
-        T* row = y + (h0 + u) * sd.y_h;
-        if (col.has_lo) store_oct<T, VEC>(row + col.lo, a);
-        if (col.has_hi) store_oct<T, VEC>(row + col.hi, d);
-      }
+      if (store) store_pairs<T, INTER, VEC>(y + u * sd.y_h, col, r);
     }
   }
 }
 
-// Backward.  Block-strided over (token, chunk of heads) of one side; every lane sums its
-// columns' weight gradient over its rows in fp32, the block's groups are summed through shared
-// memory in a fixed order and the block leaves one partial row: the result does not depend on
-// the order in which blocks run.
-template <typename T, int GS, bool VEC>
-__global__ void __launch_bounds__(kRopeThreads)
+// Backward.  Block-strided over (token, chunk of heads) of one side, kStages rows of x and dy
+// ahead of the row in hand; every lane sums its columns' weight gradient over its rows in fp32,
+// the block's groups are summed through shared memory in a fixed order and the block leaves one
+// partial row: the result does not depend on the order in which blocks run.
+template <typename T, int GS, bool INTER, bool VEC>
+__global__ void __launch_bounds__(kRopeThreads, kBackwardMinBlocks)
 qk_rope_backward_kernel(const __grid_constant__ RopeParams p) {
-  constexpr int U = 2;
+  constexpr int kStages = sizeof(T) == 4 ? kBackwardStages / 2 : kBackwardStages;
   constexpr int kGroups = kRopeThreads / GS;
+  constexpr int kSlot = 2 * Oct<T>::kWords * kRopeThreads;
+  __shared__ uint4 stage[kStages * 2 * kSlot];
+  __shared__ Pairs weights[GS];
   pdl_launch_dependents();   // the sum of the partial rows may be set up now; it waits for this grid
+  uint4* mine = stage + threadIdx.x;
   const int unit = threadIdx.x % GS, group = threadIdx.x / GS;
   int which = 0;
   while (which + 1 < p.sides && static_cast<int>(blockIdx.x) >= p.side[which + 1].first_block) ++which;
   const RopeSide& sd = p.side[which];
   const int block = blockIdx.x - sd.first_block;
-  const LaneColumns col = lane_columns(p, unit);
+  const LaneColumns col = lane_columns<INTER>(p, unit);
   const bool norm = sd.w != nullptr;
-  float wlo[8] = {}, whi[8] = {};
-  if (norm) {
-    if (col.has_lo) load_weight<T>(p, sd.w, col.lo, wlo);
-    if (col.has_hi) load_weight<T>(p, sd.w, col.hi, whi);
-  }
-  float glo[8] = {}, ghi[8] = {};   // weight gradient of the lane's columns
+  const bool rotated = col.rotated && sd.rotate != 0;
+  Pairs grad;                     // weight gradient of the lane's columns
+#pragma unroll
+  for (int k = 0; k < 4; ++k) grad.lo[k] = grad.hi[k] = both(0.f);
 
+  // row number i of a group: head (i mod 2^k) of the chunk that is its task i / 2^k; the same
+  // number of rows for every group of the block (the sums below are warp-collective)
   const int64_t tasks = p.total_tokens * sd.chunks;
   const int64_t step = static_cast<int64_t>(sd.blocks) * kGroups;
-  // the loop's bound is the same for the lanes of a warp (group_sum is warp-collective)
-  const int64_t rounds = (tasks + step - 1) / step;
-  for (int64_t i = 0; i < rounds; ++i) {
-    const int64_t task = i * step + static_cast<int64_t>(block) * kGroups + group;
-    const bool live = task < tasks;
-    const int64_t n = live ? task / sd.chunks : 0;
-    const int chunk = live ? static_cast<int>(task - n * sd.chunks) : 0;
-    const int64_t b = n / p.tokens, t = n - b * p.tokens;
-    float c[8], s[8];
-    const bool rotate = live && col.rotated;
-    if (rotate) {
-      load_angles(p, b, t, col, unit, c, s);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) s[k] = -s[k];
+  const int64_t first = static_cast<int64_t>(block) * kGroups + group;
+  const int per = 1 << sd.log_per;
+  const int rows = static_cast<int>(((tasks + step - 1) / step) << sd.log_per);
+  struct Place {
+    int64_t b, t;
+    int h, heads;                 // first head, heads of this chunk (0: no such task)
+  };
+  auto place_of = [&](int i) {
+    const int64_t task = static_cast<int64_t>(i >> sd.log_per) * step + first;
+    Place q = {0, 0, 0, 0};
+    if (task < tasks && i < rows) {
+      int64_t n;
+      if (tasks <= 0x7fffffff) {  // 32-bit divisions where they do
+        const uint32_t n32 = static_cast<uint32_t>(task) / static_cast<uint32_t>(sd.chunks);
+        q.b = n32 / static_cast<uint32_t>(p.tokens);
+        n = n32;
+      } else {
+        n = task / sd.chunks;
+        q.b = n / p.tokens;
+      }
+      q.h = static_cast<int>(task - n * sd.chunks) << sd.log_per;
+      q.heads = min(sd.heads - q.h, per);
+      q.t = n - q.b * p.tokens;
     }
-    const T* x = static_cast<const T*>(sd.x) + b * sd.x_b + t * sd.x_t;
-    const T* dy = static_cast<const T*>(sd.dy) + b * sd.dy_b + t * sd.dy_t;
-    T* dx = static_cast<T*>(sd.y) + b * sd.y_b + t * sd.y_t;
-    const int h_begin = chunk * p.heads_per_group;
-    const int h_end = live ? min(sd.heads, h_begin + p.heads_per_group) : h_begin;
-    // as many rounds for every group of the warp: a full chunk's heads, not this chunk's
-    for (int h0 = h_begin; h0 < h_begin + min(p.heads_per_group, sd.heads); h0 += U) {
-      Oct<T> xlo[U], xhi[U], dlo[U], dhi[U];
+    return q;
+  };
+  const T* xs = static_cast<const T*>(sd.x);
+  const T* dys = static_cast<const T*>(sd.dy);
+  int fetch_heads = 0;            // of the chunk that is being requested
+  auto request = [&](int i, uint4* slot) {
+    const int u = i & (per - 1);
+    if (u == 0) {
+      const Place q = place_of(i);
+      fetch_heads = q.heads;
+      xs = static_cast<const T*>(sd.x) + q.b * sd.x_b + q.t * sd.x_t + q.h * sd.x_h;
+      dys = static_cast<const T*>(sd.dy) + q.b * sd.dy_b + q.t * sd.dy_t + q.h * sd.dy_h;
+    }
+    stage_row<T, VEC>(slot, xs, col, u < fetch_heads);
+    stage_row<T, VEC>(slot + kSlot, dys, col, u < fetch_heads);
+    if (u + 1 < fetch_heads) {
+      xs += sd.x_h;
+      dys += sd.dy_h;
+    }
+    stage_commit();
+  };
+  for (int i = 0; i < kStages - 1; ++i) request(i, mine + i * 2 * kSlot);
+  if (norm && threadIdx.x < GS) weights[unit] = load_weights<T, INTER>(sd.w, p.w_is_f32, col);
+  __syncthreads();
+  const Pairs& w = weights[unit];
+
+  int heads = 0;                  // of the chunk in hand
+  Angles angles;
+  T* dx = nullptr;
+  int use = 0, fill = kStages - 1;
+  for (int i = 0; i < rows; ++i) {
+    const int u = i & (per - 1);
+    request(i + kStages - 1, mine + fill * 2 * kSlot);
+    fill = fill + 1 == kStages ? 0 : fill + 1;
+    if (u == 0) {
+      const Place here = place_of(i);
+      heads = here.heads;
+      if (heads > 0 && rotated) load_angles(p, position_of(p, here.b, here.t), here.t, unit, angles);
+      dx = static_cast<T*>(sd.y) + here.b * sd.y_b + here.t * sd.y_t + here.h * sd.y_h;
+    }
+    stage_wait<kStages - 1>();
+    const uint4* slot = mine + use * 2 * kSlot;
+    use = use + 1 == kStages ? 0 : use + 1;
+    Pairs g = read_staged<T, INTER>(slot + kSlot);
+    if (heads > 0 && rotated) rotate_pairs<true>(g, angles);
+    if (norm) {
+      const Pairs x = read_staged<T, INTER>(slot);
+      Pairs gx;
+      float2 sq[2] = {both(0.f), both(0.f)}, dot[2] = {both(0.f), both(0.f)};   // sum x^2, sum x g w
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const bool on = h0 + u < h_end;
-        xlo[u] = xhi[u] = dlo[u] = dhi[u] = Oct<T>{};
-        if (on && col.has_lo) {
-          xlo[u] = load_oct<T, VEC>(x + (h0 + u) * sd.x_h + col.lo);
-          dlo[u] = load_oct<T, VEC>(dy + (h0 + u) * sd.dy_h + col.lo);
-        }
-        if (on && col.has_hi) {
-          xhi[u] = load_oct<T, VEC>(x + (h0 + u) * sd.x_h + col.hi);
-          dhi[u] = load_oct<T, VEC>(dy + (h0 + u) * sd.dy_h + col.hi);
-        }
+      for (int k = 0; k < 4; ++k) {
+        gx.lo[k] = __fmul2_rn(g.lo[k], x.lo[k]);
+        gx.hi[k] = __fmul2_rn(g.hi[k], x.hi[k]);
+        sq[0] = __ffma2_rn(x.lo[k], x.lo[k], sq[0]);
+        sq[1] = __ffma2_rn(x.hi[k], x.hi[k], sq[1]);
+        dot[0] = __ffma2_rn(gx.lo[k], w.lo[k], dot[0]);
+        dot[1] = __ffma2_rn(gx.hi[k], w.hi[k], dot[1]);
       }
+      const float2 sqs = __fadd2_rn(sq[0], sq[1]), dots = __fadd2_rn(dot[0], dot[1]);
+      const float r = rsqrtf(group_sum<GS>(sqs.x + sqs.y) * p.inv_dim + p.eps);
+      const float along = group_sum<GS>(dots.x + dots.y) * p.inv_dim * r * r;   // mean(h u) / (x / u)
+      // rows that are not there are zeros and add nothing
+      const float2 r2 = both(u < heads ? r : 0.f), m2 = both(u < heads ? -r * along : 0.f);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        float gl[8], gh[8];
-        unpack_oct<T>(dlo[u], gl);
-        unpack_oct<T>(dhi[u], gh);
-        if (rotate) rotate_lane(gl, gh, c, s, p.interleaved);
-        if (norm) {
-          float a[8], d[8];
-          unpack_oct<T>(xlo[u], a);
-          unpack_oct<T>(xhi[u], d);
-          float sq = 0.f, dot = 0.f;   // sum x^2, sum x * g * w
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            sq += a[k] * a[k] + d[k] * d[k];
-            dot += a[k] * (gl[k] * wlo[k]) + d[k] * (gh[k] * whi[k]);
-          }
-          const float r = rsqrtf(group_sum<GS>(sq) * p.inv_dim + p.eps);
-          const float along = group_sum<GS>(dot) * p.inv_dim * r * r;   // mean(h u) / (x / u)
-          if (h0 + u < h_end) {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              glo[k] += gl[k] * (a[k] * r);
-              ghi[k] += gh[k] * (d[k] * r);
-            }
-          }
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            gl[k] = r * (gl[k] * wlo[k] - a[k] * along);
-            gh[k] = r * (gh[k] * whi[k] - d[k] * along);
-          }
-        }
-        if (h0 + u < h_end) {
-          T* row = dx + (h0 + u) * sd.y_h;
-          if (col.has_lo) store_oct<T, VEC>(row + col.lo, gl);
-          if (col.has_hi) store_oct<T, VEC>(row + col.hi, gh);
-        }
+      for (int k = 0; k < 4; ++k) {
+        grad.lo[k] = __ffma2_rn(gx.lo[k], r2, grad.lo[k]);
+        grad.hi[k] = __ffma2_rn(gx.hi[k], r2, grad.hi[k]);
+        g.lo[k] = __ffma2_rn(x.lo[k], m2, __fmul2_rn(__fmul2_rn(g.lo[k], w.lo[k]), r2));
+        g.hi[k] = __ffma2_rn(x.hi[k], m2, __fmul2_rn(__fmul2_rn(g.hi[k], w.hi[k]), r2));
       }
+    }
+    if (u < heads) {
+      store_pairs<T, INTER, VEC>(dx, col, g);
+      dx += sd.y_h;
     }
   }
+  stage_wait<0>();
 
   if (!norm) return;   // the same for the whole block
-  __shared__ float sums[kGroups][GS * 16 + 1];
+  float (*sums)[GS * 16 + 1] = reinterpret_cast<float (*)[GS * 16 + 1]>(stage);
+  static_assert(sizeof(stage) >= kGroups * (GS * 16 + 1) * 4, "the stages are reused for the sums");
+  __syncthreads();
+  {
+    float a[8], b[8];
+    from_pairs<INTER>(grad, a, b);
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    sums[group][unit * 16 + k] = glo[k];
-    sums[group][unit * 16 + 8 + k] = ghi[k];
+    for (int k = 0; k < 8; ++k) {
+      sums[group][unit * 16 + k] = a[k];
+      sums[group][unit * 16 + 8 + k] = b[k];
+    }
   }
   __syncthreads();
   for (int i = threadIdx.x; i < GS * 16; i += kRopeThreads) {
-    const LaneColumns lc = lane_columns(p, i / 16);
+    const LaneColumns lc = lane_columns<INTER>(p, i / 16);
     const bool high = (i % 16) >= 8;
     if (high ? lc.has_hi : lc.has_lo) {
       float v = 0.f;
@@ -463,12 +612,12 @@ bool side_vectors(const RopeSide& s, int64_t elem) {
 // Lanes per row: the smallest group whose lanes hold 16 values each.
 int lanes_per_row(int units) { return units <= 4 ? 4 : (units <= 8 ? 8 : 16); }
 
-// Heads a group walks with one token's angles: as many as leave every SM about a thousand
-// threads, at least the rows that are requested together.
-int pick_heads_per_group(int64_t total_tokens, int heads_all, int lanes, int at_least, int sms) {
-  int per = 16;
-  while (per > at_least && total_tokens * lanes * ceil_div(heads_all, per) < static_cast<int64_t>(sms) * 1024) per /= 2;
-  return per < at_least ? at_least : per;
+// Heads a group walks with one token's angles, a power of two: as many as leave every SM about a
+// thousand threads.
+int pick_heads_per_group(int64_t total_tokens, int heads_all, int lanes, int most, int sms) {
+  int per = most;
+  while (per > 1 && total_tokens * lanes * ceil_div(heads_all, per) < static_cast<int64_t>(sms) * 1024) per /= 2;
+  return per;
 }
 
 int fill_geometry(RopeParams& p, int64_t batch, int64_t tokens, int dim, int rotary, int interleaved,
@@ -512,8 +661,13 @@ int fill_geometry(RopeParams& p, int64_t batch, int64_t tokens, int dim, int rot
 
 template <typename T, int GS>
 int launch_rope(const RopeParams& p, bool vec, dim3 grid, cudaStream_t stream) {
-  if (vec) qk_rope_kernel<T, GS, true><<<grid, kRopeThreads, 0, stream>>>(p);
-  else qk_rope_kernel<T, GS, false><<<grid, kRopeThreads, 0, stream>>>(p);
+  if (p.interleaved) {
+    if (vec) qk_rope_kernel<T, GS, true, true><<<grid, kRopeThreads, 0, stream>>>(p);
+    else qk_rope_kernel<T, GS, true, false><<<grid, kRopeThreads, 0, stream>>>(p);
+  } else {
+    if (vec) qk_rope_kernel<T, GS, false, true><<<grid, kRopeThreads, 0, stream>>>(p);
+    else qk_rope_kernel<T, GS, false, false><<<grid, kRopeThreads, 0, stream>>>(p);
+  }
   B200K_CHECK_LAUNCH("qk_rope launch");
   return B200K_OK;
 }
@@ -535,7 +689,8 @@ int launch_forward(RopeParams& p, int dtype, cudaStream_t stream) {
     heads_all += p.side[i].heads;
     vec = vec && side_vectors(p.side[i], dtype == B200K_F32 ? 4 : 2);
   }
-  p.heads_per_group = pick_heads_per_group(p.total_tokens, heads_all, lanes, dtype == B200K_F32 ? 2 : 4, sms);
+  p.heads_per_group = pick_heads_per_group(p.total_tokens, heads_all, lanes,
+                                           dtype == B200K_F32 ? ForwardRows<float>::kMax : ForwardRows<__half>::kMax, sms);
   int64_t chunks = 0;
   for (int i = 0; i < p.sides; ++i) {
     p.side[i].chunks = static_cast<int>(ceil_div(p.side[i].heads, p.heads_per_group));
@@ -551,8 +706,13 @@ int launch_forward(RopeParams& p, int dtype, cudaStream_t stream) {
 
 template <typename T, int GS>
 int launch_backward(const RopeParams& p, bool vec, int grid, cudaStream_t stream) {
-  if (vec) qk_rope_backward_kernel<T, GS, true><<<grid, kRopeThreads, 0, stream>>>(p);
-  else qk_rope_backward_kernel<T, GS, false><<<grid, kRopeThreads, 0, stream>>>(p);
+  if (p.interleaved) {
+    if (vec) qk_rope_backward_kernel<T, GS, true, true><<<grid, kRopeThreads, 0, stream>>>(p);
+    else qk_rope_backward_kernel<T, GS, true, false><<<grid, kRopeThreads, 0, stream>>>(p);
+  } else {
+    if (vec) qk_rope_backward_kernel<T, GS, false, true><<<grid, kRopeThreads, 0, stream>>>(p);
+    else qk_rope_backward_kernel<T, GS, false, false><<<grid, kRopeThreads, 0, stream>>>(p);
+  }
   B200K_CHECK_LAUNCH("qk_rope backward launch");
   return B200K_OK;
 }
@@ -565,7 +725,7 @@ int launch_backward_type(const RopeParams& p, int lanes, bool vec, int grid, cud
 }
 
 // Blocks of the backward pass per SM: enough rows in flight, few partial rows.
-constexpr int kBackwardBlocksPerSM = 6;
+constexpr int kBackwardBlocksPerSM = kBackwardMinBlocks;
 
 }  // namespace
 }  // namespace b200k
@@ -639,7 +799,7 @@ extern "C" int b200k_qk_norm_rope_backward(const b200k_qk_norm_rope_args* a, b20
 
   const int lanes = lanes_per_row(p.units);
   const int groups = kRopeThreads / lanes;
-  p.heads_per_group = pick_heads_per_group(p.total_tokens, static_cast<int>(a->heads_q + a->heads_kv), lanes, 2, sms);
+  const int most = pick_heads_per_group(p.total_tokens, static_cast<int>(a->heads_q + a->heads_kv), lanes, 8, sms);
   WeightGradParams g = {};
   g.dim = p.dim;
   g.out[0] = a->dq_weight;
@@ -669,7 +829,8 @@ extern "C" int b200k_qk_norm_rope_backward(const b200k_qk_norm_rope_args* a, b20
     }
     s.heads = static_cast<int>(heads);
     s.rotate = a->rotary_dim > 0;
-    s.chunks = static_cast<int>(ceil_div(heads, p.heads_per_group));
+    while ((1 << s.log_per) < most && (1 << s.log_per) < heads) ++s.log_per;
+    s.chunks = static_cast<int>(ceil_div(heads, 1 << s.log_per));
     const int64_t need = ceil_div(p.total_tokens * s.chunks, groups);
     int64_t share = budget * rows / (rows_q + rows_k);
     if (share < 1) share = 1;
