@@ -219,6 +219,8 @@ __device__ __forceinline__ LaneColumns lane_columns(const RopeParams& p, int uni
     c.hi = c.lo + 8;
     c.has_lo = unit < p.units;
     c.has_hi = c.has_lo && c.hi < p.dim;
+    if (!c.has_lo) c.lo = 0;
+    if (!c.has_hi) c.hi = 0;
   }
   return c;
 }
@@ -264,22 +266,21 @@ __device__ __forceinline__ void stage_row(uint4* slot, const T* row, const LaneC
   constexpr int kWords = Oct<T>::kWords;
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
-    const bool has = on && (half == 0 ? col.has_lo : col.has_hi);
-    const T* src = row + (half == 0 ? col.lo : col.hi);
+    const bool has = half == 0 ? col.has_lo : col.has_hi;
+    const T* src = row + (half == 0 ? col.lo : col.hi);   // a column of the row also where the lane has none
     if constexpr (VEC) {
 #pragma unroll
       for (int i = 0; i < kWords; ++i) {
         const uint32_t dst = smem_u32(slot + (half * kWords + i) * kRopeThreads);
         // a source size of 0 fills the slot with zeros and reads nothing
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst),
-                     "l"(reinterpret_cast<uint64_t>(reinterpret_cast<const uint4*>(has ? src : row) + (has ? i : 0))),
-                     "r"(has ? 16 : 0)
+                     "l"(reinterpret_cast<uint64_t>(reinterpret_cast<const uint4*>(src) + i)), "r"(has && on ? 16 : 0)
                      : "memory");
       }
     } else {
       Oct<T> o = {};
       T* e = reinterpret_cast<T*>(&o);
-      if (has) {
+      if (has && on) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) e[i] = src[i];
       }
@@ -415,7 +416,7 @@ qk_rope_backward_kernel(const __grid_constant__ RopeParams p) {
   constexpr int kGroups = kRopeThreads / GS;
   constexpr int kSlot = 2 * Oct<T>::kWords * kRopeThreads;
   __shared__ uint4 stage[kStages * 2 * kSlot];
-  __shared__ Pairs weights[GS];
+  __shared__ float4 weights[4][GS];   // [piece][unit]: neighbouring lanes read neighbouring banks
   pdl_launch_dependents();   // the sum of the partial rows may be set up now; it waits for this grid
   uint4* mine = stage + threadIdx.x;
   const int unit = threadIdx.x % GS, group = threadIdx.x / GS;
@@ -480,9 +481,15 @@ qk_rope_backward_kernel(const __grid_constant__ RopeParams p) {
     stage_commit();
   };
   for (int i = 0; i < kStages - 1; ++i) request(i, mine + i * 2 * kSlot);
-  if (norm && threadIdx.x < GS) weights[unit] = load_weights<T, INTER>(sd.w, p.w_is_f32, col);
+  if (norm && threadIdx.x < GS) {
+    const Pairs v = load_weights<T, INTER>(sd.w, p.w_is_f32, col);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      weights[k][unit] = make_float4(v.lo[2 * k].x, v.lo[2 * k].y, v.lo[2 * k + 1].x, v.lo[2 * k + 1].y);
+      weights[2 + k][unit] = make_float4(v.hi[2 * k].x, v.hi[2 * k].y, v.hi[2 * k + 1].x, v.hi[2 * k + 1].y);
+    }
+  }
   __syncthreads();
-  const Pairs& w = weights[unit];
 
   int heads = 0;                  // of the chunk in hand
   Angles angles;
@@ -505,7 +512,15 @@ qk_rope_backward_kernel(const __grid_constant__ RopeParams p) {
     if (heads > 0 && rotated) rotate_pairs<true>(g, angles);
     if (norm) {
       const Pairs x = read_staged<T, INTER>(slot);
-      Pairs gx;
+      Pairs gx, w;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const float4 l = weights[k][unit], h = weights[2 + k][unit];
+        w.lo[2 * k] = make_float2(l.x, l.y);
+        w.lo[2 * k + 1] = make_float2(l.z, l.w);
+        w.hi[2 * k] = make_float2(h.x, h.y);
+        w.hi[2 * k + 1] = make_float2(h.z, h.w);
+      }
       float2 sq[2] = {both(0.f), both(0.f)}, dot[2] = {both(0.f), both(0.f)};   // sum x^2, sum x g w
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
