@@ -14,11 +14,20 @@
 // memory.  A CTA walks its range; an item that lies in one range is finished there, the others
 // leave partial softmax states (row maximum, sum, accumulator) that a second kernel joins in
 // range order.  The split is a function of the lengths alone, so results do not depend on
-// timing.  Two CTAs share an SM: one's softmax overlaps the other's matrix products and loads.
+// timing.
 //
-//   warp 0      TMA producer: one box per run of slots inside a page
-//   warp 1      MMA issuer: S = Q K^T, O += P V (P from tensor memory)
-//   warps 2..5  Q to shared memory, softmax (a row per thread), epilogue
+// One CTA per SM, two softmax groups A and B whose work interleaves on the tensor cores, so that
+// one's softmax overlaps the other's matrix products:
+//   split  (at most 128 rows)   A and B take the item's key tiles in turn, each with its own
+//                               running maximum, sum and O; A joins the two states at the end
+//   pair   (more rows)          A and B are two row tiles of 128, every key tile serves both
+//
+//   warps 0, 10  TMA producers of K and of V: a box per run of slots inside a page, into rings
+//   warp 1       MMA issuer: S_x = Q K^T, O_x += P_x V (P from tensor memory)
+//   warps 2..5   softmax group A, warps 6..9 group B: a query row per thread
+//
+// What a run does once (masks, Q rows that are not aligned, tokens that are not finite) is kept in
+// rolled loops: unrolled, the kernel was 180 KB of code, more than the instruction cache.
 //
 // Slots behind a sequence's last token may hold anything: their scores are masked by index and
 // their rows of V are cleared in shared memory, since 0 * NaN is not 0.
@@ -34,10 +43,19 @@ namespace {
 
 constexpr int kPaBM = 128;             // query rows of a tile
 constexpr int kPaBN = 128;             // keys of a tile
-constexpr int kPaThreads = 192;
-constexpr int kPaTmemCols = 256;
-constexpr int kPaCtasPerSM = 2;
-constexpr int kPaMergeThreads = 128;
+constexpr int kPaThreads = 352;        // K warp, MMA warp, two softmax groups of four warps, V warp
+constexpr int kPaTmemCols = 512;       // S_A, S_B, O_A, O_B; P over S
+constexpr int kPaJoinThreads = 128;
+
+// Rings of K and V tiles in what Q leaves of 224 KB.  V tiles wait for the softmax, so V gets
+// the odd one.
+template <int D, bool PAIR> struct Rings {
+  static constexpr int kTile = 128 * D * 2;
+  static constexpr int kQ = PAIR ? 2 : 1;
+  static constexpr int kTiles = 224 * 1024 / kTile - kQ;
+  static constexpr int kK = kTiles / 2, kV = kTiles - kK;
+  static constexpr int kSmem = 1024 + (kQ + kTiles) * kTile + 1984;
+};
 
 struct PagedParams {
   const uint16_t* q;
@@ -51,7 +69,8 @@ struct PagedParams {
   int64_t q_b, q_h, q_t, o_b, o_h, o_t, kc_p, kc_h, kc_s, vc_p, vc_h, vc_s, mask_b, mask_t, mask_j;
   int64_t page_table_stride, num_pages;
   int batch, tokens, heads_kv, group, dim;
-  int rows, row_tiles, tile_rows;      // tokens * group; tiles of 128 of them; min(rows, 128)
+  int rows, row_tiles;                 // tokens * group; tiles of tile_height of them
+  int tile_height, tile_rows;          // 128 (split) or 256 (pair); rows a tile really has, at most
   int page_size, max_pages, box_rows;
   int ctas;
   int q_vec, o_vec;                    // rows of q / out on 16-byte boundaries
@@ -62,52 +81,55 @@ struct PagedParams {
   int* status;
 };
 
-// Lengths of a sequence, kept inside what its page table can name.
+// Lengths of a sequence, kept inside what its page table can name (at most 2^29 tokens: every count
+// of tokens and of key tiles fits 32 bits).
 struct SeqInfo {
   int have, fresh, len, tiles;         // tokens before the step, of the step, their sum, key tiles
 };
 __device__ __forceinline__ SeqInfo seq_info(const PagedParams& p, int b) {
   SeqInfo s;
-  const int64_t cap = static_cast<int64_t>(p.max_pages) * p.page_size;
-  const int64_t have = p.cache_lens[b];
-  int64_t fresh = p.tokens;
-  if (p.new_lens != nullptr) fresh = max(0, min(p.new_lens[b], p.tokens));
-  s.fresh = static_cast<int>(fresh);
-  s.have = static_cast<int>(max(static_cast<int64_t>(0), min(have, cap)));
-  s.len = static_cast<int>(min(s.have + fresh, cap));
-  if (fresh == 0) s.len = 0;
+  const int cap = p.max_pages * p.page_size;
+  s.fresh = p.new_lens != nullptr ? max(0, min(p.new_lens[b], p.tokens)) : p.tokens;
+  s.have = max(0, min(p.cache_lens[b], cap));
+  s.len = s.fresh == 0 ? 0 : min(s.have + s.fresh, cap);
   s.tiles = (s.len + kPaBN - 1) / kPaBN;
   return s;
 }
 __device__ __forceinline__ bool lengths_fit(const PagedParams& p, int b) {
-  const int64_t have = p.cache_lens[b];
-  const int64_t fresh = p.new_lens != nullptr ? max(0, min(p.new_lens[b], p.tokens)) : p.tokens;
-  return fresh == 0 || (have >= 0 && have + fresh <= static_cast<int64_t>(p.max_pages) * p.page_size);
+  const int fresh = p.new_lens != nullptr ? max(0, min(p.new_lens[b], p.tokens)) : p.tokens;
+  const int have = p.cache_lens[b];
+  return fresh == 0 || (have >= 0 && have <= p.max_pages * p.page_size - fresh);
 }
 
-__device__ __forceinline__ int64_t warp_sum64(int64_t v) {
+__device__ __forceinline__ int warp_sum(int v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
 // Key tiles of the sequences [0, count), warp-collective.
-__device__ __forceinline__ int64_t tiles_before(const PagedParams& p, int count, int lane) {
-  int64_t sum = 0;
+__device__ __forceinline__ int tiles_before(const PagedParams& p, int count, int lane) {
+  int sum = 0;
+#pragma unroll 1
   for (int b = lane; b < count; b += 32) sum += seq_info(p, b).tiles;
-  return warp_sum64(sum);
+  return warp_sum(sum);
 }
 
-// First tile of CTA c's range; the ranges cover `total` tiles.
-__device__ __forceinline__ int64_t range_begin(int c, int64_t total, int ctas) { return c * total / ctas; }
-// The CTA whose range holds tile x.
-__device__ __forceinline__ int range_owner(int64_t x, int64_t total, int ctas) {
-  return static_cast<int>(((x + 1) * ctas - 1) / total);
-}
+// `total` tiles in `ctas` ranges, the first total % ctas of them one tile longer: first tile of
+// range c, and the range that holds tile x.
+struct Ranges {
+  int base, longer;
+  __device__ __forceinline__ Ranges(int total, int ctas) : base(total / ctas), longer(total % ctas) {}
+  __device__ __forceinline__ int begin(int c) const { return c * base + min(c, longer); }
+  __device__ __forceinline__ int owner(int x) const {
+    const int in_longer = longer * (base + 1);
+    return x < in_longer ? x / (base + 1) : longer + (x - in_longer) / base;
+  }
+};
 
 // A CTA's walk over its range: runs of key tiles of one item.
 struct Walk {
-  int64_t left;                        // tiles still to come
+  int left;                            // tiles still to come
   int b, item, tile;                   // sequence; head * row_tiles + row tile; first key tile
 };
 struct Run {
@@ -124,7 +146,7 @@ __device__ __forceinline__ bool next_run(const PagedParams& p, Walk& w, Run& r) 
   r.head = w.item / p.row_tiles;
   r.row_tile = w.item - r.head * p.row_tiles;
   r.first = w.tile;
-  r.last = static_cast<int>(min(static_cast<int64_t>(r.seq.tiles), w.tile + w.left));
+  r.last = min(r.seq.tiles, w.tile + w.left);
   w.left -= r.last - r.first;
   w.tile = 0;
   if (++w.item == p.heads_kv * p.row_tiles) {
@@ -132,6 +154,26 @@ __device__ __forceinline__ bool next_run(const PagedParams& p, Walk& w, Run& r) 
     ++w.b;
   }
   return true;
+}
+
+// A softmax warp's walk and run, in shared memory: what a run needs at its two ends only would
+// otherwise be spilled to local memory, whose lines the 20 KB of L1 beside the tiles do not hold.
+constexpr int kRunWords = 16;
+__device__ __forceinline__ void save_run(volatile int* w, const Walk& k, const Run& r) {
+  w[0] = k.left; w[1] = k.b; w[2] = k.item; w[3] = k.tile;
+  w[4] = r.seq.have; w[5] = r.seq.fresh; w[6] = r.seq.len; w[7] = r.seq.tiles;
+  w[8] = r.b; w[9] = r.head; w[10] = r.row_tile; w[11] = r.first; w[12] = r.last;
+}
+__device__ __forceinline__ Walk saved_walk(volatile int* w) {
+  Walk k;
+  k.left = w[0]; k.b = w[1]; k.item = w[2]; k.tile = w[3];
+  return k;
+}
+__device__ __forceinline__ Run saved_run(volatile int* w) {
+  Run r;
+  r.seq.have = w[4]; r.seq.fresh = w[5]; r.seq.len = w[6]; r.seq.tiles = w[7];
+  r.b = w[8]; r.head = w[9]; r.row_tile = w[10]; r.first = w[11]; r.last = w[12];
+  return r;
 }
 
 // Whether a 16-bit float is an infinity or NaN, for the two halves of a word.
@@ -146,34 +188,100 @@ __device__ __forceinline__ float half_to_float(uint16_t h) {
   else return __half2float(*reinterpret_cast<const __half*>(&h));
 }
 
+// Which of the keys [k0, k0 + 32) a row sees, as bits.  `mask` points at the row's entries.
+__device__ __forceinline__ uint32_t visible_keys(const uint8_t* mask, int64_t mask_j, int have, int fresh, int t, int k0) {
+  const int old = min(32, have - k0);         // tokens from before the step
+  if (old >= 32) return 0xffffffffu;
+  uint32_t bits = old > 0 ? (1u << old) - 1u : 0u;
+  const int draft0 = k0 - have;               // of bit 0
+  if (mask == nullptr) {                      // drafts up to t
+    const int n = min(t, fresh - 1) + 1 - draft0;
+    return n >= 32 ? 0xffffffffu : (n > 0 ? (1u << n) - 1u : 0u);
+  }
+  const int first = max(0, -draft0), last = min(32, fresh - draft0);
+  mask += draft0 * mask_j;
+#pragma unroll 8
+  for (int i = 0; i < 32; ++i)
+    if (i >= first && i < last && mask[i * mask_j] != 0) bits |= 1u << i;
+  return bits;
+}
+
+// A finished row's O in the workspace: adds the share of the step's tokens whose row of V was
+// cleared for being not finite, where the row sees them, and with `whole` writes the output.
+// Such values are a model's failure, but they stay with the rows that see them.
 template <int D, bool BF16>
-__global__ void __launch_bounds__(kPaThreads, kPaCtasPerSM)
+__device__ __forceinline__ void add_cleared_drafts(const PagedParams& p, Run run, int hq, int t, float* acc, float m,
+                                                float inv_l, bool whole) {
+  const uint16_t* q_row = p.q + run.b * p.q_b + hq * p.q_h + t * p.q_t;
+  const int end = min(run.seq.len, run.last * kPaBN);
+  for (int key = max(run.seq.have, run.first * kPaBN); key < end; ++key) {
+    const int draft = key - run.seq.have;
+    const bool sees = p.mask != nullptr ? p.mask[run.b * p.mask_b + t * p.mask_t + draft * p.mask_j] != 0 : draft <= t;
+    const int page = p.page_table[run.b * p.page_table_stride + key / p.page_size];
+    if (!sees || page < 0 || page >= p.num_pages) continue;
+    const uint16_t* v_row = p.v + page * p.vc_p + run.head * p.vc_h + (key % p.page_size) * p.vc_s;
+    bool bad = false;
+#pragma unroll 1
+    for (int k = 0; k < p.dim; ++k) bad = bad || word_not_finite<BF16>(v_row[k]);
+    if (!bad) continue;
+    const uint16_t* k_row = p.k + page * p.kc_p + run.head * p.kc_h + (key % p.page_size) * p.kc_s;
+    float score = 0.f;
+#pragma unroll 1
+    for (int k = 0; k < p.dim; ++k) score += half_to_float<BF16>(q_row[k]) * half_to_float<BF16>(k_row[k]);
+    const float e = fast_exp2(score * p.scale_log2 - m);
+#pragma unroll 1
+    for (int k = 0; k < p.dim; ++k) acc[k] += e * half_to_float<BF16>(v_row[k]);
+  }
+  if (!whole) return;
+  uint16_t* o_row = p.out + run.b * p.o_b + hq * p.o_h + t * p.o_t;
+#pragma unroll 1
+  for (int k = 0; k < p.dim; ++k) {
+    if constexpr (BF16) reinterpret_cast<__nv_bfloat16*>(o_row)[k] = __float2bfloat16_rn(acc[k] * inv_l);
+    else reinterpret_cast<__half*>(o_row)[k] = __float2half_rn(acc[k] * inv_l);
+  }
+}
+
+template <int D, bool BF16, bool PAIR>
+__global__ void __launch_bounds__(kPaThreads, 1)
 paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                        const __grid_constant__ PagedParams p) {
+  using R = Rings<D, PAIR>;
   constexpr int kBoxes = D / 64;            // 64-element (128-byte) slices of the head dim
-  constexpr int kTileBytes = 128 * D * 2;
   constexpr int kBoxBytes = 128 * 128;
+  constexpr int kTileRows = PAIR ? 2 * kPaBM : kPaBM;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (base - smem_u32(smem_raw));
   const uint32_t q_smem = base;
-  const uint32_t k_smem = base + kTileBytes;
-  const uint32_t v_smem = base + 2 * kTileBytes;
-  uint8_t* tail = smem + 3 * kTileBytes;
+  const uint32_t k_smem = q_smem + R::kQ * R::kTile;
+  const uint32_t v_smem = k_smem + R::kK * R::kTile;
+  uint8_t* tail = smem + (R::kQ + R::kTiles) * R::kTile;
   const uint32_t bar0 = smem_u32(tail);
-  enum { Q_FULL = 0, K_FULL, K_EMPTY, V_FULL, V_EMPTY, S_FULL, P_FULL, PV_DONE, EDGE_DONE, NUM_BARS };
+  enum { Q_FULL = 0, Q_EMPTY, S_FULL, P_HALF = S_FULL + 2, P_FULL = P_HALF + 2, PV_DONE = P_FULL + 2,
+         RUN_DONE = PV_DONE + 2, O_READ, K_FULL, K_EMPTY = K_FULL + R::kK, V_FULL = K_EMPTY + R::kK,
+         V_EMPTY = V_FULL + R::kV, NUM_BARS = V_EMPTY + R::kV };
+  static_assert(8 * NUM_BARS <= 384, "barriers fit their place");
   auto bar = [&](int i) { return bar0 + 8u * i; };
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail + 8 * NUM_BARS);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + 8 * NUM_BARS + 8);
-  volatile int* bad_draft = reinterpret_cast<volatile int*>(tail + 8 * NUM_BARS + 16);   // [2], by run parity
-  Walk* walk_start = reinterpret_cast<Walk*>(tail + 8 * NUM_BARS + 32);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail + 384);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + 392);
+  volatile int* bad_draft = reinterpret_cast<volatile int*>(tail + 400);   // [2], by run parity
+  Walk* walk_start = reinterpret_cast<Walk*>(tail + 408);
+  float2* state_b = reinterpret_cast<float2*>(tail + 448);                 // [128] maximum and sum of B's rows
+  volatile int* run_words = reinterpret_cast<volatile int*>(tail + 1472);  // [8 softmax warps][kRunWords]
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
 
   pdl_launch_dependents();   // the joining kernel may be set up now; it waits for this grid
   if (threadIdx.x == 0) {
-    for (int i = 0; i < NUM_BARS; ++i) mbar_init(bar(i), (i == P_FULL || i == Q_FULL || i == EDGE_DONE) ? 4 : 1);
+    for (int i = 0; i < NUM_BARS; ++i) {
+      int count = 1;
+      if (i >= P_HALF && i < PV_DONE) count = 4;
+      if (i == Q_FULL) count = PAIR ? 8 : 4;
+      if (i == RUN_DONE) count = 8;
+      if (i == O_READ) count = 4;
+      mbar_init(bar(i), count);
+    }
     *abort_flag = 0;
     bad_draft[0] = bad_draft[1] = -1;
     fence_barrier_init();
@@ -187,32 +295,32 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
   if (warp == 2) {
     // this CTA's range of key tiles and the item it begins in
     const int per_seq = p.heads_kv * p.row_tiles;
-    const int64_t total = tiles_before(p, p.batch, lane) * per_seq;
+    const Ranges ranges(tiles_before(p, p.batch, lane) * per_seq, p.ctas);
     Walk w;
-    const int64_t begin = range_begin(blockIdx.x, total, p.ctas);
-    w.left = range_begin(blockIdx.x + 1, total, p.ctas) - begin;
+    const int begin = ranges.begin(blockIdx.x);
+    w.left = ranges.begin(blockIdx.x + 1) - begin;
     w.b = 0;
     w.item = 0;
     w.tile = 0;
-    int64_t before = 0;
+    int before = 0;
+#pragma unroll 1
     for (int b0 = 0; b0 < p.batch && w.left > 0; b0 += 32) {
       const int b = b0 + lane;
-      const int64_t mine = b < p.batch ? static_cast<int64_t>(seq_info(p, b).tiles) * per_seq : 0;
-      int64_t upto = mine;
+      const int tiles = b < p.batch ? seq_info(p, b).tiles : 0;
+      const int mine = tiles * per_seq;
+      int upto = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+        const int v = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += v;
       }
       const bool here = begin >= before + upto - mine && begin < before + upto;
-      const uint32_t who = __ballot_sync(0xffffffffu, here);
-      if (who != 0) {
+      if (__any_sync(0xffffffffu, here)) {
         if (here) {
-          const int tiles = static_cast<int>(mine / per_seq);
-          const int64_t in_seq = begin - (before + upto - mine);
+          const int in_seq = begin - (before + upto - mine);
           w.b = b;
-          w.item = static_cast<int>(in_seq / tiles);
-          w.tile = static_cast<int>(in_seq - static_cast<int64_t>(w.item) * tiles);
+          w.item = in_seq / tiles;
+          w.tile = in_seq - w.item * tiles;
           *walk_start = w;
         }
         break;
@@ -221,6 +329,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
     }
     if (w.left <= 0 && lane == 0) *walk_start = w;
     if (blockIdx.x == 0) {
+#pragma unroll 1
       for (int b = lane; b < p.batch; b += 32)
         if (!lengths_fit(p, b)) report_bad_index(p.status, kRolePage, b);
     }
@@ -229,249 +338,360 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
-  const uint32_t tmem_s = tmem_base;          // S: 128 columns; P aliases its first 64
-  const uint32_t tmem_o = tmem_base + 128;    // O: D columns
   constexpr uint32_t kFmt = BF16 ? kFmtBF16 : kFmtF16;
-  Walk walk = *walk_start;
-  Run run;
 
-  if (warp == 0) {
+  if (warp == 0 || warp == kPaThreads / 32 - 1) {
+    // the K producer and the V producer
+    Walk walk = *walk_start;
+    Run run;
+    const bool is_v = warp != 0;
+    const CUtensorMap* tmap = is_v ? &tmap_v : &tmap_k;
+    const int full = is_v ? V_FULL : K_FULL, empty = is_v ? V_EMPTY : K_EMPTY, places = is_v ? R::kV : R::kK;
+    const uint32_t ring = is_v ? v_smem : k_smem;
     const int boxes_per_tile = kPaBN / p.box_rows;
+    const uint32_t box_bytes = p.box_rows * 128u;
     const bool elected = elect_one();
     bool ok = true;
-    int it = 0;                                // key tiles so far, over all runs
+    int place = 0, fills = 0;
+    uint32_t parity = 1;                       // a fresh ring is empty
     while (ok && next_run(p, walk, run)) {
       const int* pages = p.page_table + run.b * p.page_table_stride;
-      for (int j = run.first; j < run.last; ++j, ++it) {
-        const uint32_t ph = it & 1;
-        const int boxes = min(boxes_per_tile, (run.seq.len - j * kPaBN + p.box_rows - 1) / p.box_rows);
-        // lane i: the i-th run of slots, all of one page
-        int page = 0, slot = 0;
-        if (lane < boxes) {
-          const int key = j * kPaBN + lane * p.box_rows;
+      // lane i: the i-th run of slots of a tile, all of one page
+      auto find = [&](int j, int& page, int& slot) {
+        const int key = j * kPaBN + lane * p.box_rows;
+        page = slot = 0;
+        if (lane < boxes_per_tile && key < run.seq.len) {
           const int entry = key / p.page_size;
           slot = key - entry * p.page_size;
           page = pages[entry];
-          if (page < 0 || page >= p.num_pages) {
-            report_bad_index(p.status, kRolePage, run.b);
-            page = static_cast<int>(p.num_pages);   // behind the last page: filled with zeros
+        }
+      };
+      int page, slot;
+      find(run.first, page, slot);
+      for (int j = run.first; j < run.last; ++j) {
+        int next_page = 0, next_slot = 0;
+        if (j + 1 < run.last) find(j + 1, next_page, next_slot);   // on its way while this tile is issued
+        const int boxes = min(boxes_per_tile, (run.seq.len - j * kPaBN + p.box_rows - 1) / p.box_rows);
+        if (lane < boxes && (page < 0 || page >= p.num_pages)) {
+          report_bad_index(p.status, kRolePage, run.b);
+          page = static_cast<int>(p.num_pages);   // behind the last page: filled with zeros
+        }
+        if (!mbar_wait(bar(empty + place), parity, abort_flag)) {
+          report_status(p.status, is_v ? 91 : 90, j);
+          *abort_flag = 1;
+          ok = false;
+          break;
+        }
+        const uint32_t dst = ring + place * R::kTile, done = bar(full + place);
+        if (elected) mbar_arrive_expect_tx(done, static_cast<uint32_t>(boxes) * box_bytes * kBoxes);
+        // warp-uniform coordinates: one elected lane issues box after box (lanes with coordinates
+        // of their own cost three times as much per box)
+#pragma unroll 1
+        for (int i = 0; i < boxes; ++i) {
+          const int pg = __shfl_sync(0xffffffffu, page, i), sl = __shfl_sync(0xffffffffu, slot, i);
+          if (elected) {
+#pragma unroll
+            for (int h = 0; h < kBoxes; ++h)
+              tma_load_4d(dst + h * kBoxBytes + i * box_bytes, tmap, done, h * 64, sl, run.head, pg);
           }
         }
-        const uint32_t bytes = static_cast<uint32_t>(boxes) * p.box_rows * 128u * kBoxes;
-        if (!mbar_wait(bar(K_EMPTY), ph ^ 1, abort_flag)) {
-          report_status(p.status, 90, j);
-          *abort_flag = 1;
-          ok = false;
-          break;
-        }
-        if (elected) mbar_arrive_expect_tx(bar(K_FULL), bytes);
         __syncwarp();
-        if (lane < boxes) {
-#pragma unroll
-          for (int i = 0; i < kBoxes; ++i)
-            tma_load_4d(k_smem + i * kBoxBytes + lane * p.box_rows * 128, &tmap_k, bar(K_FULL), i * 64, slot,
-                        run.head, page);
-        }
-        __syncwarp();
-        if (!mbar_wait(bar(V_EMPTY), ph ^ 1, abort_flag)) {
-          report_status(p.status, 91, j);
-          *abort_flag = 1;
-          mbar_wait(bar(K_FULL), ph, abort_flag);
-          ok = false;
-          break;
-        }
-        if (elected) mbar_arrive_expect_tx(bar(V_FULL), bytes);
-        __syncwarp();
-        if (lane < boxes) {
-#pragma unroll
-          for (int i = 0; i < kBoxes; ++i)
-            tma_load_4d(v_smem + i * kBoxBytes + lane * p.box_rows * 128, &tmap_v, bar(V_FULL), i * 64, slot,
-                        run.head, page);
-        }
-        __syncwarp();
+        ++fills;
+        if (++place == places) { place = 0; parity ^= 1; }
+        page = next_page;
+        slot = next_slot;
       }
     }
-    if (it > 0) {   // no copy of this CTA is in flight when it leaves (bounded, also after a failure)
-      mbar_wait(bar(K_FULL), (it - 1) & 1, abort_flag);
-      mbar_wait(bar(V_FULL), (it - 1) & 1, abort_flag);
-    }
+    // no copy of this warp is in flight when the CTA leaves (bounded, also after a failure): the
+    // last fill of every ring place
+    for (int i = 0; i < places && i < fills; ++i)
+      mbar_wait(bar(full + i), ((fills - 1 - i) / places) & 1, abort_flag);
     __syncwarp();
   } else if (warp == 1) {
+    Walk walk = *walk_start;
+    Run run;
     const bool elected = elect_one();
     constexpr uint32_t idesc_qk = make_idesc(kFmt, kFmt, false, false, kPaBM, kPaBN);
     constexpr uint32_t idesc_pv = make_idesc(kFmt, kFmt, false, true, kPaBM, D);
+    int ks = 0, vs = 0;
+    uint32_t kp = 0, vp = 0, pp[2] = {0, 0};   // ring places and parities; parity of the groups' P
     bool ok = true;
-    int it = 0, runs = 0;
-    for (; ok && next_run(p, walk, run); ++runs) {
+    auto give_up = [&](int role, int detail) {
+      report_status(p.status, role, detail);
+      *abort_flag = 1;
+      ok = false;
+    };
+    // S_x = Q_x K^T: both operands K-major, 16 elements (32 bytes) of the head dim per MMA
+    auto issue_s = [&](int x) {
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        const uint32_t off = (kk / 4) * kBoxBytes;
+        const uint64_t qd = make_smem_desc(q_smem + (PAIR ? x * R::kTile : 0) + off, 16, 1024, kSwizzle128B) + 2 * (kk % 4);
+        const uint64_t kd = make_smem_desc(k_smem + ks * R::kTile + off, 16, 1024, kSwizzle128B) + 2 * (kk % 4);
+        if (elected) umma<kKindF16>(tmem_base + x * 128, qd, kd, idesc_qk, kk > 0 ? 1u : 0u);
+      }
+      if (elected) tc_commit(bar(S_FULL + x));
+    };
+    auto free_k = [&]() {
+      if (elected) tc_commit(bar(K_EMPTY + ks));
+      if (++ks == R::kK) { ks = 0; kp ^= 1; }
+    };
+    // O_x += P_x V in two halves of 64 keys: P from tensor memory, V (keys, D) with D contiguous
+    auto issue_pv = [&](int x, bool first, int j) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        if (!mbar_wait(bar((half == 0 ? P_HALF : P_FULL) + x), pp[x], abort_flag)) {
+          give_up(94, j);
+          return;
+        }
+        tc_fence_after_sync();
+#pragma unroll
+        for (int k4 = 0; k4 < kPaBN / 32; ++k4) {
+          const int kk = half * (kPaBN / 32) + k4;
+          const uint64_t vd = make_smem_desc(v_smem + vs * R::kTile + kk * 2048, kBoxBytes, 1024, kSwizzle128B);
+          if (elected)
+            umma_f16_ts(tmem_base + 256 + x * 128, tmem_base + x * 128 + kk * 8, vd, idesc_pv, (!first || kk > 0) ? 1u : 0u);
+        }
+      }
+      pp[x] ^= 1;
+      if (elected) tc_commit(bar(PV_DONE + x));
+    };
+    auto free_v = [&]() {
+      if (elected) tc_commit(bar(V_EMPTY + vs));
+      if (++vs == R::kV) { vs = 0; vp ^= 1; }
+    };
+    for (int runs = 0; ok && next_run(p, walk, run); ++runs) {
+      const int n = run.last - run.first;
       if (!mbar_wait(bar(Q_FULL), runs & 1, abort_flag)) {
-        report_status(p.status, 92, runs);
-        *abort_flag = 1;
+        give_up(92, runs);
         break;
       }
-      for (int j = run.first; j < run.last; ++j, ++it) {
-        const uint32_t ph = it & 1;
-        if (!mbar_wait(bar(K_FULL), ph, abort_flag)) {
-          report_status(p.status, 93, j);
-          *abort_flag = 1;
-          ok = false;
-          break;
+      // the next S that fits: `ahead` tiles before its P V
+      auto next_s = [&](int i) {
+        if (!mbar_wait(bar(K_FULL + ks), kp, abort_flag)) {
+          give_up(93, i);
+          return;
         }
         tc_fence_after_sync();
-        // S = Q K^T: both operands K-major, 16 elements (32 bytes) of the head dim per MMA
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = (kk / 4) * kBoxBytes;
-          const uint64_t qd = make_smem_desc(q_smem + off, 16, 1024, kSwizzle128B) + 2 * (kk % 4);
-          const uint64_t kd = make_smem_desc(k_smem + off, 16, 1024, kSwizzle128B) + 2 * (kk % 4);
-          if (elected) umma<kKindF16>(tmem_s, qd, kd, idesc_qk, kk > 0 ? 1u : 0u);
+        if (PAIR) {
+          issue_s(0);
+          issue_s(1);
+        } else {
+          issue_s(i & 1);
         }
-        if (elected) {
-          tc_commit(bar(K_EMPTY));
-          tc_commit(bar(S_FULL));
-        }
-        if (!mbar_wait(bar(P_FULL), ph, abort_flag) || !mbar_wait(bar(V_FULL), ph, abort_flag)) {
-          report_status(p.status, 94, j);
-          *abort_flag = 1;
-          ok = false;
+        free_k();
+        if (i == n - 1 && elected) tc_commit(bar(Q_EMPTY));
+      };
+      next_s(0);
+      if (!PAIR && n > 1 && ok) next_s(1);
+      for (int i = 0; i < n && ok; ++i) {
+        if (!mbar_wait(bar(V_FULL + vs), vp, abort_flag)) {
+          give_up(95, i);
           break;
         }
-        tc_fence_after_sync();
-        // O += P V: P from tensor memory, V (keys, D) with D contiguous = MN-major B
-#pragma unroll
-        for (int kk = 0; kk < kPaBN / 16; ++kk) {
-          const uint64_t vd = make_smem_desc(v_smem + kk * 2048, kBoxBytes, 1024, kSwizzle128B);
-          if (elected) umma_f16_ts(tmem_o, tmem_s + kk * 8, vd, idesc_pv, (j > run.first || kk > 0) ? 1u : 0u);
-        }
-        if (elected) {
-          tc_commit(bar(V_EMPTY));
-          tc_commit(bar(PV_DONE));
+        if (PAIR) {
+          // P V (A, i)  S (A, i + 1)  P V (B, i)  S (B, i + 1)
+          const bool more = i + 1 < n;
+          if (more && !mbar_wait(bar(K_FULL + ks), kp, abort_flag)) {
+            give_up(93, i);
+            break;
+          }
+          tc_fence_after_sync();
+          issue_pv(0, i == 0, i);
+          if (ok && more) issue_s(0);
+          if (ok) issue_pv(1, i == 0, i);
+          if (ok && more) issue_s(1);
+          if (ok && more) free_k();
+          if (ok && more && i + 1 == n - 1 && elected) tc_commit(bar(Q_EMPTY));
+          if (ok) free_v();
+        } else {
+          issue_pv(i & 1, i < 2, i);
+          if (ok) free_v();
+          if (ok && i + 2 < n) next_s(i + 2);
         }
       }
     }
     __syncwarp();
   } else {
+    const int x = (warp - 2) >> 2;              // group A or B
     const int quarter = warp & 3;
     const int row = quarter * 32 + lane;
     const uint32_t lane_addr = uint32_t(quarter * 32) << 16;
+    const uint32_t tmem_s = tmem_base + x * 128 + lane_addr;
+    const uint32_t tmem_o = tmem_base + 256 + x * 128 + lane_addr;
     bool ok = true;
-    int it = 0, runs = 0, edges = 0;           // key tiles, runs, tiles with an edge so far
-    for (; ok && next_run(p, walk, run); ++runs) {
-      const SeqInfo seq = run.seq;
-      const int edges_before = edges;
-      const int r = run.row_tile * kPaBM + row;          // row of the item: token * group + head
-      const int t = r / p.group;
-      const int hq = run.head * p.group + (r - t * p.group);
-      const bool live = r < p.rows && t < seq.fresh;
-      const bool any_live = __any_sync(0xffffffffu, live);
-      const uint16_t* q_row = p.q + run.b * p.q_b + hq * p.q_h + t * p.q_t;
-      // Q: this row in 16-byte pieces, in the 128-byte swizzle of the MMA operand.  The last S
-      // of the previous run has been read (S_FULL), so nothing reads the old rows any more.
+    int runs = 0;
+    int tile0 = 0, b_tiles = 0;                 // key tiles of the CTA's earlier runs; B's share of all
+    uint32_t sp = 0;                            // parity of the group's next S (and P V)
+    auto give_up = [&](int role, int detail) {
+      report_status(p.status, role, detail);
+      *abort_flag = 1;
+      ok = false;
+    };
+    volatile int* mine = run_words + (warp - 2) * kRunWords;
+    // the query row this thread has in a run: token and head, and whether there is one
+    struct Place {
+      int t, hq;
+      bool live;
+    };
+    auto place_in = [&](const Run& run) {
+      const int r = run.row_tile * kTileRows + (PAIR ? x * kPaBM : 0) + row;   // token * group + head
+      Place q;
+      q.t = r / p.group;
+      q.hq = run.head * p.group + (r - q.t * p.group);
+      q.live = r < p.rows && q.t < run.seq.fresh;
+      return q;
+    };
+    for (; ok; ++runs) {
+      int n, first_tile, have;
+      bool live, any_live;
+      {
+        Walk walk = runs == 0 ? *walk_start : saved_walk(mine);
+        Run run;
+        if (!next_run(p, walk, run)) break;
+        const Place at = place_in(run);
+        live = at.live;
+        any_live = __any_sync(0xffffffffu, live);
+        n = run.last - run.first;
+        first_tile = run.first;
+        have = run.seq.have;
+        __syncwarp();
+        if (lane == 0) save_run(mine, walk, run);
+        __syncwarp();
+      if (PAIR || x == 1) {
+        // Q: this row in 16-byte pieces, in the 128-byte swizzle of the MMA operand, once the last
+        // S of the run before has read its own.  (Split: B fetches it while A finishes that run.)
+        const uint32_t q_dst = q_smem + (PAIR ? x * R::kTile : 0) + row * 128;
+        const uint16_t* q_row = p.q + run.b * p.q_b + at.hq * p.q_h + at.t * p.q_t;
+        uint4 q4[D / 8];
 #pragma unroll
-      for (int c = 0; c < D / 8; ++c) {
-        uint32_t w[4] = {0u, 0u, 0u, 0u};
-        if (live && c * 8 < p.dim) {
-          if (p.q_vec) {
-            const uint4 x = *reinterpret_cast<const uint4*>(q_row + c * 8);
-            w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
-          } else {
+        for (int c = 0; c < D / 8; ++c) {
+          q4[c] = make_uint4(0u, 0u, 0u, 0u);
+          if (live && p.q_vec && c * 8 < p.dim) q4[c] = *reinterpret_cast<const uint4*>(q_row + c * 8);
+        }
+        __syncwarp();
+        if (runs > 0 && !mbar_wait(bar(Q_EMPTY), (runs - 1) & 1, abort_flag)) {
+          give_up(98, runs);
+          break;
+        }
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c)
+          st_shared_v4(q_dst + (c / 8) * kBoxBytes + (((c % 8) ^ (row & 7)) * 16), q4[c].x, q4[c].y, q4[c].z, q4[c].w);
+        if (!p.q_vec && live) {
+#pragma unroll 1
+          for (int c = 0; c < p.dim / 8; ++c) {
+            uint32_t w[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i)
               w[i] = static_cast<uint32_t>(q_row[c * 8 + 2 * i]) | (static_cast<uint32_t>(q_row[c * 8 + 2 * i + 1]) << 16);
+            st_shared_v4(q_dst + (c / 8) * kBoxBytes + (((c % 8) ^ (row & 7)) * 16), w[0], w[1], w[2], w[3]);
           }
         }
-        st_shared_v4(q_smem + (c / 8) * kBoxBytes + row * 128 + (((c % 8) ^ (row & 7)) * 16), w[0], w[1], w[2], w[3]);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(Q_FULL));
       }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(Q_FULL));
+      }
+      if (!PAIR && x == 1 && runs > 0 && !mbar_wait(bar(O_READ), (runs - 1) & 1, abort_flag)) {
+        give_up(99, runs);                      // A has read this group's O of the run before
+        break;
+      }
 
       float m_used = -INFINITY, l = 0.0f;
-      for (int j = run.first; j < run.last; ++j, ++it) {
-        const uint32_t ph = it & 1;
+      // the run is this warp's no more than to its last P: what others read of it is in place
+      auto leave_run = [&]() {
+        if (!PAIR && x == 1) state_b[row] = make_float2(m_used, l);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(RUN_DONE));
+      };
+      const int i0 = PAIR ? 0 : x, di = PAIR ? 1 : 2;
+      if (i0 >= n) leave_run();                 // B of a single tile
+      for (int i = i0; i < n; i += di) {
+        const int j = first_tile + i;
         const int key0 = j * kPaBN;
-        const bool edge = key0 + kPaBN > seq.have;       // the step's tokens, or slots behind the last one
-        if (!mbar_wait(bar(S_FULL), ph, abort_flag)) {
-          report_status(p.status, 96, j);
-          *abort_flag = 1;
-          ok = false;
+        const bool edge = key0 + kPaBN > have;       // the step's tokens, or slots behind the last one
+        uint32_t sees[4] = {0u, 0u, 0u, 0u};
+        if (edge && live) {
+          const Run run = saved_run(mine);
+          const int t = place_in(run).t;
+          const uint8_t* mask = p.mask == nullptr ? nullptr : p.mask + run.b * p.mask_b + t * p.mask_t;
+#pragma unroll 1
+          for (int w = 0; w < 4; ++w) {                  // rolled: the words move up
+            sees[0] = sees[1];
+            sees[1] = sees[2];
+            sees[2] = sees[3];
+            sees[3] = visible_keys(mask, p.mask_j, have, run.seq.fresh, t, key0 + 32 * w);
+          }
+        }
+        __syncwarp();
+        if (!mbar_wait(bar(S_FULL + x), sp, abort_flag)) {
+          give_up(96, j);
           break;
         }
-        if (edge) {
-          // (S_FULL also says that P V of the last tile is done: only now is V_FULL's phase this
-          // tile's, and V this tile's rows.)  Row `row` of V is cleared where no token lies, and where a token of the step that some
-          // query may not see is not finite (added by hand in the epilogue)
-          if (!mbar_wait(bar(V_FULL), ph, abort_flag)) {
-            report_status(p.status, 95, j);
-            *abort_flag = 1;
-            ok = false;
+        if (edge && (!PAIR || x == 0)) {
+          // Row `row` of V is cleared where no token lies, and where a token of the step that some
+          // query may not see is not finite (added by hand in the epilogue).  S_FULL says that
+          // the P V two tiles back is done, so V_FULL's phase is this tile's or the one before.
+          const int vi = tile0 + i, vs = vi % R::kV;
+          if (!mbar_wait(bar(V_FULL + vs), (vi / R::kV) & 1, abort_flag)) {
+            give_up(95, j);
             break;
           }
+          // (rows lie 128 bytes apart: every lane starts at another 16-byte piece, or all would
+          // meet in the same banks)
+          const uint32_t v_row = v_smem + vs * R::kTile + row * 128;
           const int key = key0 + row;
-          bool clear = key >= seq.len;
-          if (!clear && key >= seq.have && (p.mask != nullptr || p.tokens > 1)) {
-#pragma unroll 4
+          bool clear = key >= mine[6];                    // the sequence's length
+          if (!clear && key >= have && (p.mask != nullptr || p.tokens > 1)) {
+#pragma unroll 2
             for (int c = 0; c < D / 8; ++c) {
-              uint32_t x[4];
-              ld_shared_v4(v_smem + (c / 8) * kBoxBytes + row * 128 + (c % 8) * 16, x);
-              clear = clear || word_not_finite<BF16>(x[0]) || word_not_finite<BF16>(x[1]) ||
-                      word_not_finite<BF16>(x[2]) || word_not_finite<BF16>(x[3]);
+              uint32_t y[4];
+              ld_shared_v4(v_row + (c / 8) * kBoxBytes + ((c ^ row) & 7) * 16, y);
+              clear = clear || word_not_finite<BF16>(y[0]) || word_not_finite<BF16>(y[1]) ||
+                      word_not_finite<BF16>(y[2]) || word_not_finite<BF16>(y[3]);
             }
             if (clear) bad_draft[runs & 1] = runs;
           }
           if (clear) {
-#pragma unroll 4
-            for (int c = 0; c < D / 8; ++c)
-              st_shared_v4(v_smem + (c / 8) * kBoxBytes + row * 128 + (c % 8) * 16, 0u, 0u, 0u, 0u);
+#pragma unroll 2
+            for (int c = 0; c < D / 8; ++c) st_shared_v4(v_row + (c / 8) * kBoxBytes + ((c ^ row) & 7) * 16, 0u, 0u, 0u, 0u);
           }
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) mbar_arrive(bar(EDGE_DONE));
-          ++edges;
         }
         tc_fence_after_sync();
         if (any_live) {                                   // a warp of padding rows only keeps step
-          float s[128];
-          {
-            uint32_t x[128];
-            tmem_ld_32x32b_x128(tmem_s + lane_addr, x);
+          // S in halves of 64 scores, once for the maximum and once for the exponentials: a row of 128
+          // in registers would spill, and local memory is what the L1 beside 224 KB of tiles
+          // serves worst
+          auto load_scores = [&](int half, float (&s)[64]) {
+            uint32_t y[64];
+            tmem_ld_32x32b_x64(tmem_s + half * 64, y);
             tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 128; ++i) s[i] = __uint_as_float(x[i]);
-          }
-          if (edge) {
-            uint32_t sees[4];
+            for (int k = 0; k < 64; ++k) s[k] = __uint_as_float(y[k]);
+            if (edge) {
+              const uint32_t lo = half == 0 ? sees[0] : sees[2], hi = half == 0 ? sees[1] : sees[3];
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              uint32_t bits = 0;
-              const int k0 = key0 + 32 * w;
-              if (k0 + 32 <= seq.have) {
-                bits = 0xffffffffu;
-              } else if (live && k0 < seq.len) {
-                const uint8_t* mrow = p.mask + run.b * p.mask_b + t * p.mask_t;
-#pragma unroll 1
-                for (int i = 0; i < 32; ++i) {
-                  const int key = k0 + i, draft = key - seq.have;
-                  bool v = draft < 0;
-                  if (!v && key < seq.len) v = p.mask != nullptr ? mrow[draft * p.mask_j] != 0 : draft <= t;
-                  bits |= static_cast<uint32_t>(v) << i;
-                }
-              }
-              sees[w] = bits;
+              for (int k = 0; k < 64; ++k)
+                if ((((k < 32 ? lo : hi) >> (k % 32)) & 1u) == 0u) s[k] = -INFINITY;
             }
+          };
+          float mx = -INFINITY;
+#pragma unroll 1
+          for (int half = 0; half < 2; ++half) {
+            float s[64];
+            load_scores(half, s);
+            float m4[4];
 #pragma unroll
-            for (int i = 0; i < 128; ++i)
-              if (((sees[i / 32] >> (i % 32)) & 1u) == 0u) s[i] = -INFINITY;
-            __syncwarp();
+            for (int c = 0; c < 4; ++c) {
+              m4[c] = fmax3(s[16 * c], s[16 * c + 1], s[16 * c + 2]);
+#pragma unroll
+              for (int k = 3; k < 15; k += 2) m4[c] = fmax3(m4[c], s[16 * c + k], s[16 * c + k + 1]);
+              m4[c] = fmaxf(m4[c], s[16 * c + 15]);
+            }
+            mx = fmaxf(mx, fmax3(m4[0], m4[1], fmaxf(m4[2], m4[3])));
           }
-          float mx8[8];
-#pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            float m = fmax3(s[16 * c], s[16 * c + 1], s[16 * c + 2]);
-#pragma unroll
-            for (int i = 3; i < 15; i += 2) m = fmax3(m, s[16 * c + i], s[16 * c + i + 1]);
-            mx8[c] = fmaxf(m, s[16 * c + 15]);
-          }
-          const float mx = fmax3(fmax3(mx8[0], mx8[1], mx8[2]), fmax3(mx8[3], mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7]));
           const float m_new = fmaxf(m_used, mx * p.scale_log2);
           const bool grow = (m_new - m_used > kRescaleThreshold) || (m_used == -INFINITY && m_new > -INFINITY);
           const bool any_grow = __any_sync(0xffffffffu, grow);
@@ -480,127 +700,149 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
             alpha = (m_used == -INFINITY) ? 0.0f : fast_exp2(m_used - m_new);
             m_used = m_new;
           }
-          if (any_grow && j > run.first) {
-            // S_FULL of this tile was committed after P V of the last one, so O is quiescent
+          if (any_grow && i > i0) {
+            // this S was committed after the group's last P V, so O is quiescent
             l *= alpha;
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
-              uint32_t x[32];
-              tmem_ld_32x32b_x32(tmem_o + lane_addr + c * 32, x);
+              uint32_t y[32];
+              tmem_ld_32x32b_x32(tmem_o + c * 32, y);
               tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * alpha);
-              tmem_st_32x32b_x32(tmem_o + lane_addr + c * 32, x);
+              for (int k = 0; k < 32; ++k) y[k] = __float_as_uint(__uint_as_float(y[k]) * alpha);
+              tmem_st_32x32b_x32(tmem_o + c * 32, y);
             }
           }
           const float neg_m = (m_used == -INFINITY) ? 0.0f : -m_used;
           const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
           const float2 negm2 = make_float2(neg_m, neg_m);
           float2 sum2[4] = {};
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < 2; ++c) {
+            float s[64];
+            load_scores(c, s);                            // P of the first half lies over scores already used
             uint32_t pk[32];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const float2 x = __ffma2_rn(make_float2(s[c * 64 + 2 * i], s[c * 64 + 2 * i + 1]), scale2, negm2);
-              const float2 e = make_float2(fast_exp2(x.x), fast_exp2(x.y));
-              sum2[i & 3] = __fadd2_rn(sum2[i & 3], e);
+            for (int k = 0; k < 32; ++k) {
+              const float2 y = __ffma2_rn(make_float2(s[2 * k], s[2 * k + 1]), scale2, negm2);
+              const float2 e = make_float2(fast_exp2(y.x), fast_exp2(y.y));
+              sum2[k & 3] = __fadd2_rn(sum2[k & 3], e);
               // P is rounded to the input type: it is the tensor cores' operand
-              pk[i] = BF16 ? pack_bf16x2(e.x, e.y) : pack_f16x2(e.x, e.y);
+              pk[k] = BF16 ? pack_bf16x2(e.x, e.y) : pack_f16x2(e.x, e.y);
             }
-            tmem_st_32x32b_x32(tmem_s + lane_addr + c * 32, pk);
+            tmem_st_32x32b_x32(tmem_s + c * 32, pk);
+            if (c == 0) {                                 // the first 64 keys are enough for half of P V
+              tmem_st_wait();
+              tc_fence_before_sync();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(bar(P_HALF + x));
+            }
           }
           l += ((sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y)) + ((sum2[2].x + sum2[2].y) + (sum2[3].x + sum2[3].y));
           tmem_st_wait();
+        } else {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(P_HALF + x));
         }
+        sp ^= 1;
+        // before the last P: whoever finds the run's products done finds these arrivals made, so
+        // the phases of RUN_DONE cannot lie two apart
+        if (i + di >= n) leave_run();
         tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(P_FULL));
+        if (lane == 0) mbar_arrive(bar(P_FULL + x));
       }
-      // every warp has looked at its rows of V before any reads bad_draft (a tile's V comes after
-      // all four warps have left the tile before it, so the phases cannot lie two apart)
-      if (ok && (!mbar_wait(bar(PV_DONE), (it - 1) & 1, abort_flag) ||
-                 (edges > edges_before && !mbar_wait(bar(EDGE_DONE), (edges - 1) & 1, abort_flag)))) {
-        report_status(p.status, 97, 0);
-        *abort_flag = 1;
-        ok = false;
-      }
+      tile0 += n;
       if (!ok) break;
+      if (!PAIR && x == 1) continue;                      // A finishes the run
+      const bool edges = (first_tile + n) * kPaBN > have;
+      const bool two = !PAIR && n > 1;                    // B has a share of it
+      b_tiles += n / 2;
+      if (!mbar_wait(bar(PV_DONE + x), sp ^ 1, abort_flag) ||
+          (two && !mbar_wait(bar(PV_DONE + 1), (b_tiles - 1) & 1, abort_flag)) ||
+          ((!PAIR || edges) && !mbar_wait(bar(RUN_DONE), runs & 1, abort_flag))) {
+        give_up(97, runs);
+        break;
+      }
       tc_fence_after_sync();
-      if (!any_live) continue;
 
       // the run's result: the output where the run is the whole item, else a partial state
-      const bool whole = run.first == 0 && run.last == seq.tiles;
-      const int64_t slot = (2 * static_cast<int64_t>(blockIdx.x) + (runs == 0 ? 0 : 1)) * p.tile_rows + row;
+      float fa = 1.0f, fb = 0.0f;
+      if (two) {
+        const float2 sb = state_b[row];
+        const float m = fmaxf(m_used, sb.x);
+        fa = (m_used == -INFINITY) ? 0.0f : fast_exp2(m_used - m);
+        fb = (sb.x == -INFINITY) ? 0.0f : fast_exp2(sb.x - m);
+        l = l * fa + sb.y * fb;
+        m_used = m;
+      }
+      const Run run = saved_run(mine);
+      const Place at = place_in(run);
+      const bool whole = run.first == 0 && run.last == run.seq.tiles;
+      const int64_t slot = (2 * static_cast<int64_t>(blockIdx.x) + (runs == 0 ? 0 : 1)) * p.tile_rows +
+                           (PAIR ? x * kPaBM : 0) + row;
       const float inv_l = (l > 0.0f) ? __fdividef(1.0f, l) : (l == 0.0f ? 0.0f : l);
-      uint16_t* o_row = p.out + run.b * p.o_b + hq * p.o_h + t * p.o_t;
-      const bool by_hand = bad_draft[runs & 1] == runs;
+      const bool by_hand = edges && bad_draft[runs & 1] == runs;
+      const bool to_out = whole && !by_hand;
+      uint16_t* o_row = p.out + run.b * p.o_b + at.hq * p.o_h + at.t * p.o_t;
+      float* acc = p.ws_acc + slot * D;
       if (live && !whole) {
         p.ws_ml[2 * slot] = m_used;
         p.ws_ml[2 * slot + 1] = l;
       }
+      if (any_live) {
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          float o[32];
+          {
+            uint32_t y[32];
+            tmem_ld_32x32b_x32(tmem_o + c * 32, y);
+            tmem_ld_wait();
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        float o[32];
-        {
-          uint32_t x[32];
-          tmem_ld_32x32b_x32(tmem_o + lane_addr + c * 32, x);
-          tmem_ld_wait();
+            for (int k = 0; k < 32; ++k) o[k] = __uint_as_float(y[k]);
+            if (two) {                                    // B's O lies in the same lanes
+              tmem_ld_32x32b_x32(tmem_o + 128 + c * 32, y);
+              tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = __uint_as_float(x[i]);
-        }
-        if (live) {
-          if (by_hand) {
-            // tokens of the step whose row of V was cleared for being not finite: their share,
-            // for the rows that see them
-            const int k_end = min(seq.len, run.last * kPaBN);
-            for (int key = max(seq.have, run.first * kPaBN); key < k_end; ++key) {
-              const int draft = key - seq.have;
-              const bool v = p.mask != nullptr ? p.mask[run.b * p.mask_b + t * p.mask_t + draft * p.mask_j] != 0 : draft <= t;
-              const int page = p.page_table[run.b * p.page_table_stride + key / p.page_size];
-              if (!v || page < 0 || page >= p.num_pages) continue;
-              const uint16_t* v_row = p.v + page * p.vc_p + run.head * p.vc_h + (key % p.page_size) * p.vc_s;
-              bool bad = false;
-              for (int i = 0; i < p.dim; ++i) bad = bad || word_not_finite<BF16>(v_row[i]);
-              if (!bad) continue;
-              const uint16_t* k_row = p.k + page * p.kc_p + run.head * p.kc_h + (key % p.page_size) * p.kc_s;
-              float score = 0.f;
-              for (int i = 0; i < p.dim; ++i) score += half_to_float<BF16>(q_row[i]) * half_to_float<BF16>(k_row[i]);
-              const float e = fast_exp2(score * p.scale_log2 - m_used);
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (c * 32 + i < p.dim) o[i] += e * half_to_float<BF16>(v_row[c * 32 + i]);
+              for (int k = 0; k < 32; ++k) o[k] = o[k] * fa + __uint_as_float(y[k]) * fb;
             }
           }
-          if (whole) {
+          if (live && to_out) {
             uint32_t pk[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-              pk[i] = BF16 ? pack_bf16x2(o[2 * i] * inv_l, o[2 * i + 1] * inv_l) : pack_f16x2(o[2 * i] * inv_l, o[2 * i + 1] * inv_l);
+            for (int k = 0; k < 16; ++k)
+              pk[k] = BF16 ? pack_bf16x2(o[2 * k] * inv_l, o[2 * k + 1] * inv_l)
+                           : pack_f16x2(o[2 * k] * inv_l, o[2 * k + 1] * inv_l);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int d0 = c * 32 + 8 * i;
+            for (int k = 0; k < 4; ++k) {
+              const int d0 = c * 32 + 8 * k;
               if (d0 < p.dim) {
                 if (p.o_vec) {
-                  *reinterpret_cast<uint4*>(o_row + d0) = make_uint4(pk[4 * i], pk[4 * i + 1], pk[4 * i + 2], pk[4 * i + 3]);
+                  *reinterpret_cast<uint4*>(o_row + d0) = make_uint4(pk[4 * k], pk[4 * k + 1], pk[4 * k + 2], pk[4 * k + 3]);
                 } else {
 #pragma unroll
-                  for (int k = 0; k < 4; ++k) {
-                    o_row[d0 + 2 * k] = static_cast<uint16_t>(pk[4 * i + k] & 0xffff);
-                    o_row[d0 + 2 * k + 1] = static_cast<uint16_t>(pk[4 * i + k] >> 16);
+                  for (int e = 0; e < 4; ++e) {
+                    o_row[d0 + 2 * e] = static_cast<uint16_t>(pk[4 * k + e] & 0xffff);
+                    o_row[d0 + 2 * e + 1] = static_cast<uint16_t>(pk[4 * k + e] >> 16);
                   }
                 }
               }
             }
-          } else {
-            float4* dst = reinterpret_cast<float4*>(p.ws_acc + slot * D + c * 32);
+          } else if (live) {
+            float4* dst = reinterpret_cast<float4*>(acc + c * 32);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            for (int k = 0; k < 8; ++k) dst[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
           }
+          __syncwarp();
         }
+        if (by_hand && live) add_cleared_drafts<D, BF16>(p, run, at.hq, at.t, acc, m_used, inv_l, whole);
         __syncwarp();
       }
       tc_fence_before_sync();
+      if (!PAIR) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(O_READ));
+      }
     }
     __syncwarp();
   }
@@ -617,22 +859,22 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
 // owns a row: lanes read the partial maxima and sums side by side, then every lane adds up its
 // columns over the partials.
 template <int D, bool BF16>
-__global__ void __launch_bounds__(kPaMergeThreads)
+__global__ void __launch_bounds__(kPaJoinThreads)
 paged_attention_join_kernel(const __grid_constant__ PagedParams p) {
   constexpr int kCols = D / 32;              // columns of a lane
   const int lane = threadIdx.x & 31;
   const int per_seq = p.heads_kv * p.row_tiles;
   const int b = blockIdx.y / per_seq, item = blockIdx.y - b * per_seq;
   const int head = item / p.row_tiles, row_tile = item - head * p.row_tiles;
-  const int row = blockIdx.x * (kPaMergeThreads / 32) + (threadIdx.x >> 5);
-  const int r = row_tile * kPaBM + row;
+  const int row = blockIdx.x * (kPaJoinThreads / 32) + (threadIdx.x >> 5);
+  const int r = row_tile * p.tile_height + row;
   const SeqInfo seq = seq_info(p, b);
-  const int64_t total = tiles_before(p, p.batch, lane) * per_seq;
-  const int64_t first = tiles_before(p, b, lane) * per_seq + static_cast<int64_t>(item) * seq.tiles;
+  const Ranges ranges(tiles_before(p, p.batch, lane) * per_seq, p.ctas);
+  const int first = tiles_before(p, b, lane) * per_seq + item * seq.tiles;
   // the partial states come from the kernel launched just before; every thread waits for it, so
   // that this kernel's end is that one's end too
   pdl_wait();
-  if (row >= kPaBM || r >= p.rows) return;
+  if (row >= p.tile_rows || r >= p.rows) return;
   const int t = r / p.group;
   uint16_t* o_row = p.out + b * p.o_b + static_cast<int64_t>(head * p.group + (r - t * p.group)) * p.o_h + t * p.o_t;
   const int d0 = lane * kCols;
@@ -643,16 +885,16 @@ paged_attention_join_kernel(const __grid_constant__ PagedParams p) {
   if (t < seq.fresh && seq.tiles == 0) {
     store = true;                            // nothing to see: zeros
   } else if (t < seq.fresh) {
-    const int c0 = range_owner(first, total, p.ctas), c1 = range_owner(first + seq.tiles - 1, total, p.ctas);
+    const int c0 = ranges.owner(first), c1 = ranges.owner(first + seq.tiles - 1);
     if (c0 != c1) {
       store = true;
       // only the first of an item's CTAs may have begun with an earlier item
       auto slot = [&](int c) {
-        return (2 * static_cast<int64_t>(c) + (range_begin(c, total, p.ctas) >= first ? 0 : 1)) * p.tile_rows + row;
+        return (2 * static_cast<int64_t>(c) + (ranges.begin(c) >= first ? 0 : 1)) * p.tile_rows + row;
       };
       float m = -INFINITY;
       for (int c = c0 + lane; c <= c1; c += 32)
-        if (range_begin(c, total, p.ctas) < range_begin(c + 1, total, p.ctas)) m = fmaxf(m, p.ws_ml[2 * slot(c)]);
+        if (ranges.begin(c) < ranges.begin(c + 1)) m = fmaxf(m, p.ws_ml[2 * slot(c)]);
 #pragma unroll
       for (int s = 16; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
       float l = 0.f;
@@ -661,14 +903,14 @@ paged_attention_join_kernel(const __grid_constant__ PagedParams p) {
         int64_t at = 0;
         const int c = base + lane;
         // a range may be empty where there are fewer tiles than CTAs
-        if (c <= c1 && range_begin(c, total, p.ctas) < range_begin(c + 1, total, p.ctas)) {
+        if (c <= c1 && ranges.begin(c) < ranges.begin(c + 1)) {
           at = slot(c);
           const float mc = p.ws_ml[2 * at];
           f = (mc == -INFINITY) ? 0.f : exp2f(mc - m);
           l += f * p.ws_ml[2 * at + 1];
         }
         const int n = min(32, c1 - base + 1);
-#pragma unroll 4
+#pragma unroll 2
         for (int k = 0; k < n; ++k) {
           const float fk = __shfl_sync(0xffffffffu, f, k);
           const int64_t ak = __shfl_sync(0xffffffffu, at, k);
@@ -702,13 +944,25 @@ paged_attention_join_kernel(const __grid_constant__ PagedParams p) {
 
 int padded_dim(const b200k_paged_attention_args* a) { return a->head_dim <= 64 ? 64 : 128; }
 
-// CTAs of a call: two per SM, fewer where there cannot be as many key tiles.
+// Rows that share a key/value head, and how they are cut: one 128-row tile ("split"), or tiles of
+// 256 ("pair") where there are more.
+struct Rows {
+  int64_t all, height, tiles, per_tile;
+};
+Rows lay_out_rows(const b200k_paged_attention_args* a) {
+  Rows r;
+  r.all = a->tokens * (a->heads_q / a->heads_kv);
+  r.height = r.all <= kPaBM ? kPaBM : 2 * kPaBM;
+  r.tiles = ceil_div(r.all, r.height);
+  r.per_tile = r.all < r.height ? r.all : r.height;
+  return r;
+}
+
+// CTAs of a call: one per SM, fewer where there cannot be as many key tiles.
 int64_t pick_ctas(const b200k_paged_attention_args* a, int sms) {
-  const int64_t rows = a->tokens * (a->heads_q / a->heads_kv);
-  const int64_t items = a->batch * a->heads_kv * ceil_div(rows, kPaBM);
+  const int64_t items = a->batch * a->heads_kv * lay_out_rows(a).tiles;
   const int64_t most = items * ceil_div(static_cast<int64_t>(a->max_pages) * a->page_size, kPaBN);
-  const int64_t want = static_cast<int64_t>(sms) * kPaCtasPerSM;
-  const int64_t n = most < want ? most : want;
+  const int64_t n = most < sms ? most : sms;
   return n < 1 ? 1 : n;
 }
 
@@ -724,17 +978,19 @@ int check_args(const b200k_paged_attention_args* a) {
     return fail(B200K_INVALID_ARG, "qk_scale must be positive and finite");
   if (a->page_size <= 0 || a->page_size % 8 != 0)
     return fail(B200K_UNSUPPORTED, "page_size must be a positive multiple of 8 (got %d)", a->page_size);
-  const int64_t limit = int64_t(1) << 30;
+  const int64_t limit = int64_t(1) << 29;   // sums of two such counts fit 32 bits
   if (a->tokens * a->heads_q > limit || static_cast<int64_t>(a->max_pages) * a->page_size > limit ||
-      a->num_pages >= limit || a->batch * a->heads_kv > 65535)
+      a->num_pages >= limit || a->batch > limit || a->heads_kv > limit ||
+      a->batch * a->heads_kv > 65535 ||
+      a->batch * a->heads_kv * lay_out_rows(a).tiles * ceil_div(static_cast<int64_t>(a->max_pages) * a->page_size, kPaBN) > limit)
     return fail(B200K_UNSUPPORTED, "more rows, pages or sequences than the kernel counts");
   return B200K_OK;
 }
 
-template <int D, bool BF16>
-int launch_paged(const CUtensorMap& tk, const CUtensorMap& tv, const PagedParams& p, int64_t items, cudaStream_t stream) {
-  constexpr int kSmem = 1024 + 3 * 128 * D * 2 + 256;
-  auto kernel = paged_attention_kernel<D, BF16>;
+template <int D, bool BF16, bool PAIR>
+int launch_paged_as(const CUtensorMap& tk, const CUtensorMap& tv, const PagedParams& p, int64_t items, cudaStream_t stream) {
+  constexpr int kSmem = Rings<D, PAIR>::kSmem;
+  auto kernel = paged_attention_kernel<D, BF16, PAIR>;
   static bool configured[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -746,11 +1002,17 @@ int launch_paged(const CUtensorMap& tk, const CUtensorMap& tv, const PagedParams
   }
   kernel<<<p.ctas, kPaThreads, kSmem, stream>>>(tk, tv, p);
   B200K_CHECK_LAUNCH("paged attention launch");
-  const dim3 grid(static_cast<unsigned>(ceil_div(p.tile_rows, kPaMergeThreads / 32)), static_cast<unsigned>(items));
-  const cudaError_t e = launch_after_predecessor(paged_attention_join_kernel<D, BF16>, grid, dim3(kPaMergeThreads), 0,
+  const dim3 grid(static_cast<unsigned>(ceil_div(p.tile_rows, kPaJoinThreads / 32)), static_cast<unsigned>(items));
+  const cudaError_t e = launch_after_predecessor(paged_attention_join_kernel<D, BF16>, grid, dim3(kPaJoinThreads), 0,
                                                  stream, p);
   if (e != cudaSuccess) return fail(B200K_CUDA_ERROR, "paged attention join launch: %s", cudaGetErrorString(e));
   return B200K_OK;
+}
+
+template <int D, bool BF16>
+int launch_paged(const CUtensorMap& tk, const CUtensorMap& tv, const PagedParams& p, int64_t items, cudaStream_t stream) {
+  return p.tile_height == kPaBM ? launch_paged_as<D, BF16, false>(tk, tv, p, items, stream)
+                                : launch_paged_as<D, BF16, true>(tk, tv, p, items, stream);
 }
 
 }  // namespace
@@ -764,9 +1026,7 @@ extern "C" int64_t b200k_paged_attention_workspace_bytes(const b200k_paged_atten
     return 0;
   const int sms = current_sm_count();
   if (sms <= 0) return 0;
-  const int64_t rows = a->tokens * (a->heads_q / a->heads_kv);
-  const int64_t tile_rows = rows < kPaBM ? rows : kPaBM;
-  return pick_ctas(a, sms) * 2 * tile_rows * (padded_dim(a) + 2) * 4;
+  return pick_ctas(a, sms) * 2 * lay_out_rows(a).per_tile * (padded_dim(a) + 2) * 4;
 }
 
 extern "C" int b200k_paged_attention(const b200k_paged_attention_args* a, b200k_stream stream_) {
@@ -808,8 +1068,10 @@ extern "C" int b200k_paged_attention(const b200k_paged_attention_args* a, b200k_
   p.group = static_cast<int>(a->heads_q / a->heads_kv);
   p.dim = a->head_dim;
   p.rows = p.tokens * p.group;
-  p.row_tiles = static_cast<int>(ceil_div(p.rows, kPaBM));
-  p.tile_rows = p.rows < kPaBM ? p.rows : kPaBM;
+  const Rows rows = lay_out_rows(a);
+  p.tile_height = static_cast<int>(rows.height);
+  p.row_tiles = static_cast<int>(rows.tiles);
+  p.tile_rows = static_cast<int>(rows.per_tile);
   p.page_size = a->page_size;
   p.max_pages = a->max_pages;
   // slots per TMA box: the largest power of two (8 to 128) that divides a page, so that a box
