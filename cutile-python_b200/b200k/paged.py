@@ -169,7 +169,9 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     of a multiple of 8 tokens, qk_scale positive (None: 1 / sqrt(Dim)).  A query that sees no token gives zeros.  Slots that hold none of
     the sequence's tokens are never used.  Rows behind new_lens[b] are padding: they stay as
     they are in a given ``out`` and are zero in one made here."""
-    q = rows_view(q)
+    # the kernel's copies want the queries' rows on 16-byte boundaries
+    if q.stride(-1) != 1 or q.data_ptr() % 16 or any([s % 8 or s == 0 for s in q.stride()[:-1]]):
+        q = empty_rows(q).copy_(q)
     key = (_lib.layout(q, k_cache, v_cache, page_table, cache_lens, new_lens, tree_mask, out), qk_scale,
            torch.is_grad_enabled())
     plan = _ATTENTION.get(key)
@@ -210,6 +212,8 @@ def _attention_args(q, k_cache, v_cache, page_table, cache_lens, new_lens, tree_
     _check_cache(k_cache, v_cache, page_table, cache_lens, new_lens, batch, heads_kv, dim, q.dtype, device)
     if heads_kv == 0 or heads % heads_kv:
         raise ValueError("the number of query heads must be a multiple of the cache's heads.")
+    if heads > 128 * heads_kv:
+        raise ValueError("at most 128 query heads may share a cache head.")
     if dim % 8 or not 0 < dim <= 128:
         raise ValueError("the head dimension must be a multiple of 8 up to 128")
     if k_cache.shape[2] % 8:

@@ -23,6 +23,7 @@
 //   pair   (more rows)          A and B are two row tiles of 128, every key tile serves both
 //
 //   warps 0, 10  TMA producers of K and of V: a box per run of slots inside a page, into rings
+//   warp 11      TMA producer of Q: a box of group heads x tokens is a row tile, token by token
 //   warp 1       MMA issuer: S_x = Q K^T, O_x += P_x V (P from tensor memory)
 //   warps 2..5   softmax group A, warps 6..9 group B: a query row per thread
 //
@@ -43,7 +44,7 @@ namespace {
 
 constexpr int kPaBM = 128;             // query rows of a tile
 constexpr int kPaBN = 128;             // keys of a tile
-constexpr int kPaThreads = 352;        // K warp, MMA warp, two softmax groups of four warps, V warp
+constexpr int kPaThreads = 384;        // K warp, MMA warp, two softmax groups of four warps, V and Q warps
 constexpr int kPaTmemCols = 512;       // S_A, S_B, O_A, O_B; P over S
 constexpr int kPaJoinThreads = 128;
 
@@ -54,7 +55,7 @@ template <int D, bool PAIR> struct Rings {
   static constexpr int kQ = PAIR ? 2 : 1;
   static constexpr int kTiles = 224 * 1024 / kTile - kQ;
   static constexpr int kK = kTiles / 2, kV = kTiles - kK;
-  static constexpr int kSmem = 1024 + (kQ + kTiles) * kTile + 1984;
+  static constexpr int kSmem = (kQ + kTiles) * kTile + 1472 + 8 * 2 * 13 * 4;
 };
 
 struct PagedParams {
@@ -69,15 +70,15 @@ struct PagedParams {
   int64_t q_b, q_h, q_t, o_b, o_h, o_t, kc_p, kc_h, kc_s, vc_p, vc_h, vc_s, mask_b, mask_t, mask_j;
   int64_t page_table_stride, num_pages;
   int batch, tokens, heads_kv, group, dim;
-  int rows, row_tiles;                 // tokens * group; tiles of tile_height of them
-  int tile_height, tile_rows;          // 128 (split) or 256 (pair); rows a tile really has, at most
+  int row_tiles, half_tokens;          // row tiles; tokens of a 128-row half: half_tokens * group <= 128 rows
+  int tile_rows;                       // rows of a tile's partial state
   int page_size, max_pages, box_rows;
   int ctas;
-  int q_vec, o_vec;                    // rows of q / out on 16-byte boundaries
+  int o_vec;                           // rows of out on 16-byte boundaries
   int zero_padding;
   float scale_log2;
   float* ws_ml;                        // (2 ctas, tile_rows, 2): row maximum and sum
-  float* ws_acc;                       // (2 ctas, tile_rows, D)
+  float* ws_acc;                       // (2 ctas, D / 4, tile_rows, 4)
   int* status;
 };
 
@@ -158,7 +159,7 @@ __device__ __forceinline__ bool next_run(const PagedParams& p, Walk& w, Run& r) 
 
 // A softmax warp's walk and run, in shared memory: what a run needs at its two ends only would
 // otherwise be spilled to local memory, whose lines the 20 KB of L1 beside the tiles do not hold.
-constexpr int kRunWords = 16;
+constexpr int kRunWords = 13;
 __device__ __forceinline__ void save_run(volatile int* w, const Walk& k, const Run& r) {
   w[0] = k.left; w[1] = k.b; w[2] = k.item; w[3] = k.tile;
   w[4] = r.seq.have; w[5] = r.seq.fresh; w[6] = r.seq.len; w[7] = r.seq.tiles;
@@ -188,30 +189,44 @@ __device__ __forceinline__ float half_to_float(uint16_t h) {
   else return __half2float(*reinterpret_cast<const __half*>(&h));
 }
 
-// Which of the keys [k0, k0 + 32) a row sees, as bits.  `mask` points at the row's entries.
-__device__ __forceinline__ uint32_t visible_keys(const uint8_t* mask, int64_t mask_j, int have, int fresh, int t, int k0) {
-  const int old = min(32, have - k0);         // tokens from before the step
+// Which of the keys [k0, k0 + 32) a row sees, as bits, warp-collective: lane i fetches key i's entry
+// for one token of the warp's rows after the other (neighbouring bytes, eight tokens on their
+// way at once), and a vote makes the word.  `t` is the lane's own token, [t0, t1] the warp's.
+__device__ __forceinline__ uint32_t visible_keys(const PagedParams& p, const SeqInfo& seq, int b, int t, int t0, int t1,
+                                                 int k0, int lane) {
+  const int old = seq.have - k0;              // tokens from before the step
   if (old >= 32) return 0xffffffffu;
-  uint32_t bits = old > 0 ? (1u << old) - 1u : 0u;
-  const int draft0 = k0 - have;               // of bit 0
-  if (mask == nullptr) {                      // drafts up to t
-    const int n = min(t, fresh - 1) + 1 - draft0;
+  if (k0 >= seq.len) return 0u;
+  if (p.mask == nullptr) {                    // drafts up to t
+    const int n = min(t, seq.fresh - 1) + 1 + old;
     return n >= 32 ? 0xffffffffu : (n > 0 ? (1u << n) - 1u : 0u);
   }
-  const int first = max(0, -draft0), last = min(32, fresh - draft0);
-  mask += draft0 * mask_j;
-#pragma unroll 8
-  for (int i = 0; i < 32; ++i)
-    if (i >= first && i < last && mask[i * mask_j] != 0) bits |= 1u << i;
+  uint32_t bits = old > 0 ? (1u << old) - 1u : 0u;
+  const int draft = lane - old;
+  const bool in = draft >= 0 && draft < seq.fresh && k0 + lane < seq.len;
+  const uint8_t* at = p.mask + b * p.mask_b + t0 * p.mask_t + (in ? draft * p.mask_j : 0);
+#pragma unroll 1
+  for (int tt = t0; tt <= t1; tt += 8) {
+    uint8_t v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = in && tt + u <= t1 ? at[u * p.mask_t] : 0;
+    at += 8 * p.mask_t;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const uint32_t vote = __ballot_sync(0xffffffffu, v[u] != 0);
+      if (t == tt + u) bits |= vote;
+    }
+  }
   return bits;
 }
 
-// A finished row's O in the workspace: adds the share of the step's tokens whose row of V was
+// A finished row's O in the workspace (column k at acc[k / 4][.][k % 4]): adds the share of the step's tokens whose row of V was
 // cleared for being not finite, where the row sees them, and with `whole` writes the output.
 // Such values are a model's failure, but they stay with the rows that see them.
 template <int D, bool BF16>
-__device__ __forceinline__ void add_cleared_drafts(const PagedParams& p, Run run, int hq, int t, float* acc, float m,
-                                                float inv_l, bool whole) {
+__device__ __forceinline__ void add_cleared_drafts(const PagedParams& p, const Run& run, int hq, int t, float* acc,
+                                                   float m, float inv_l, bool whole) {
+  auto at = [&](int k) -> float& { return acc[static_cast<int64_t>(k / 4) * p.tile_rows * 4 + k % 4]; };
   const uint16_t* q_row = p.q + run.b * p.q_b + hq * p.q_h + t * p.q_t;
   const int end = min(run.seq.len, run.last * kPaBN);
   for (int key = max(run.seq.have, run.first * kPaBN); key < end; ++key) {
@@ -230,29 +245,31 @@ __device__ __forceinline__ void add_cleared_drafts(const PagedParams& p, Run run
     for (int k = 0; k < p.dim; ++k) score += half_to_float<BF16>(q_row[k]) * half_to_float<BF16>(k_row[k]);
     const float e = fast_exp2(score * p.scale_log2 - m);
 #pragma unroll 1
-    for (int k = 0; k < p.dim; ++k) acc[k] += e * half_to_float<BF16>(v_row[k]);
+    for (int k = 0; k < p.dim; ++k) at(k) += e * half_to_float<BF16>(v_row[k]);
   }
   if (!whole) return;
   uint16_t* o_row = p.out + run.b * p.o_b + hq * p.o_h + t * p.o_t;
 #pragma unroll 1
   for (int k = 0; k < p.dim; ++k) {
-    if constexpr (BF16) reinterpret_cast<__nv_bfloat16*>(o_row)[k] = __float2bfloat16_rn(acc[k] * inv_l);
-    else reinterpret_cast<__half*>(o_row)[k] = __float2half_rn(acc[k] * inv_l);
+    if constexpr (BF16) reinterpret_cast<__nv_bfloat16*>(o_row)[k] = __float2bfloat16_rn(at(k) * inv_l);
+    else reinterpret_cast<__half*>(o_row)[k] = __float2half_rn(at(k) * inv_l);
   }
 }
 
 template <int D, bool BF16, bool PAIR>
 __global__ void __launch_bounds__(kPaThreads, 1)
-paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
-                       const __grid_constant__ PagedParams p) {
+paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
+                       const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ PagedParams p) {
   using R = Rings<D, PAIR>;
   constexpr int kBoxes = D / 64;            // 64-element (128-byte) slices of the head dim
   constexpr int kBoxBytes = 128 * 128;
-  constexpr int kTileRows = PAIR ? 2 * kPaBM : kPaBM;
-  extern __shared__ uint8_t smem_raw[];
-  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  uint8_t* smem = smem_raw + (base - smem_u32(smem_raw));
-  const uint32_t q_smem = base;
+  // no room for rounding the base up: the swizzle atoms need the declared alignment
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if (smem_u32(smem) & 1023u) {
+    report_status(p.status, 89, 0);
+    return;
+  }
+  const uint32_t q_smem = smem_u32(smem);
   const uint32_t k_smem = q_smem + R::kQ * R::kTile;
   const uint32_t v_smem = k_smem + R::kK * R::kTile;
   uint8_t* tail = smem + (R::kQ + R::kTiles) * R::kTile;
@@ -267,7 +284,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
   volatile int* bad_draft = reinterpret_cast<volatile int*>(tail + 400);   // [2], by run parity
   Walk* walk_start = reinterpret_cast<Walk*>(tail + 408);
   float2* state_b = reinterpret_cast<float2*>(tail + 448);                 // [128] maximum and sum of B's rows
-  volatile int* run_words = reinterpret_cast<volatile int*>(tail + 1472);  // [8 softmax warps][kRunWords]
+  volatile int* run_words = reinterpret_cast<volatile int*>(tail + 1472);  // [8 softmax warps][2][kRunWords]
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -277,7 +294,6 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
     for (int i = 0; i < NUM_BARS; ++i) {
       int count = 1;
       if (i >= P_HALF && i < PV_DONE) count = 4;
-      if (i == Q_FULL) count = PAIR ? 8 : 4;
       if (i == RUN_DONE) count = 8;
       if (i == O_READ) count = 4;
       mbar_init(bar(i), count);
@@ -285,8 +301,15 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
     *abort_flag = 0;
     bad_draft[0] = bad_draft[1] = -1;
     fence_barrier_init();
+    tma_prefetch_desc(&tmap_q);
     tma_prefetch_desc(&tmap_k);
     tma_prefetch_desc(&tmap_v);
+  }
+  if (warp == 0 && lane < 2) {
+    // the page table and the queries are asked for only after the lengths have come: their address
+    // translations start now
+    const void* early = lane == 0 ? static_cast<const void*>(p.page_table) : static_cast<const void*>(p.q);
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<uint64_t>(early)));
   }
   if (warp == 1) {
     tmem_alloc(smem_u32(tmem_slot), kPaTmemCols);
@@ -340,8 +363,44 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
   const uint32_t tmem_base = *tmem_slot;
   constexpr uint32_t kFmt = BF16 ? kFmtBF16 : kFmtF16;
 
-  if (warp == 0 || warp == kPaThreads / 32 - 1) {
-    // the K producer and the V producer
+  if (warp == 11) {
+    // the Q producer: a run's rows once the last S of the run before has read its own, and a
+    // prefetch of the next run's into the L2 (cold, they took 10 us of a full memory system)
+    Walk walk = *walk_start;
+    Run run, next;
+    bool have_run = next_run(p, walk, run), ok = true;
+    const bool elected = elect_one();
+    constexpr int kHalves = PAIR ? 2 : 1;
+    const uint32_t bytes = static_cast<uint32_t>(p.half_tokens * p.group) * 128u * kBoxes * kHalves;
+    int runs = 0;
+    for (; have_run && ok; ++runs) {
+      if (runs > 0 && !mbar_wait(bar(Q_EMPTY), (runs - 1) & 1, abort_flag)) {
+        report_status(p.status, 98, runs);
+        *abort_flag = 1;
+        ok = false;
+        break;
+      }
+      if (elected) mbar_arrive_expect_tx(bar(Q_FULL), bytes);
+      const bool more = next_run(p, walk, next);
+#pragma unroll
+      for (int x = 0; x < kHalves; ++x) {
+#pragma unroll
+        for (int h = 0; h < kBoxes; ++h) {
+          if (elected) {
+            tma_load_4d(q_smem + x * R::kTile + h * kBoxBytes, &tmap_q, bar(Q_FULL), h * 64, run.head * p.group,
+                        (run.row_tile * kHalves + x) * p.half_tokens, run.b);
+            if (more)
+              tma_prefetch_4d(&tmap_q, h * 64, next.head * p.group, (next.row_tile * kHalves + x) * p.half_tokens, next.b);
+          }
+        }
+      }
+      __syncwarp();
+      run = next;
+      have_run = more;
+    }
+    if (runs > 0) mbar_wait(bar(Q_FULL), (runs - 1) & 1, abort_flag);   // nothing in flight when the CTA leaves
+    __syncwarp();
+  } else if (warp == 0 || warp == 10) {
     Walk walk = *walk_start;
     Run run;
     const bool is_v = warp != 0;
@@ -528,69 +587,40 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       *abort_flag = 1;
       ok = false;
     };
-    volatile int* mine = run_words + (warp - 2) * kRunWords;
+    volatile int* words = run_words + (warp - 2) * 2 * kRunWords;   // this run's and the next one's
     // the query row this thread has in a run: token and head, and whether there is one
     struct Place {
       int t, hq;
       bool live;
     };
     auto place_in = [&](const Run& run) {
-      const int r = run.row_tile * kTileRows + (PAIR ? x * kPaBM : 0) + row;   // token * group + head
       Place q;
-      q.t = r / p.group;
-      q.hq = run.head * p.group + (r - q.t * p.group);
-      q.live = r < p.rows && q.t < run.seq.fresh;
+      const int in_half = row / p.group;
+      q.t = (PAIR ? run.row_tile * 2 + x : run.row_tile) * p.half_tokens + in_half;
+      q.hq = run.head * p.group + (row - in_half * p.group);
+      q.live = in_half < p.half_tokens && q.t < run.seq.fresh;
       return q;
     };
-    for (; ok; ++runs) {
+    auto open_run = [&](Walk walk, int number) {
+      Run run;
+      if (!next_run(p, walk, run)) return false;
+      __syncwarp();
+      if (lane == 0) save_run(words + (number & 1) * kRunWords, walk, run);
+      __syncwarp();
+      return true;
+    };
+    bool more = open_run(*walk_start, 0);
+    for (; more && ok; ++runs) {
+      volatile int* mine = words + (runs & 1) * kRunWords;
       int n, first_tile, have;
       bool live, any_live;
       {
-        Walk walk = runs == 0 ? *walk_start : saved_walk(mine);
-        Run run;
-        if (!next_run(p, walk, run)) break;
-        const Place at = place_in(run);
-        live = at.live;
+        const Run run = saved_run(mine);
+        live = place_in(run).live;
         any_live = __any_sync(0xffffffffu, live);
         n = run.last - run.first;
         first_tile = run.first;
         have = run.seq.have;
-        __syncwarp();
-        if (lane == 0) save_run(mine, walk, run);
-        __syncwarp();
-      if (PAIR || x == 1) {
-        // Q: this row in 16-byte pieces, in the 128-byte swizzle of the MMA operand, once the last
-        // S of the run before has read its own.  (Split: B fetches it while A finishes that run.)
-        const uint32_t q_dst = q_smem + (PAIR ? x * R::kTile : 0) + row * 128;
-        const uint16_t* q_row = p.q + run.b * p.q_b + at.hq * p.q_h + at.t * p.q_t;
-        uint4 q4[D / 8];
-#pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
-          q4[c] = make_uint4(0u, 0u, 0u, 0u);
-          if (live && p.q_vec && c * 8 < p.dim) q4[c] = *reinterpret_cast<const uint4*>(q_row + c * 8);
-        }
-        __syncwarp();
-        if (runs > 0 && !mbar_wait(bar(Q_EMPTY), (runs - 1) & 1, abort_flag)) {
-          give_up(98, runs);
-          break;
-        }
-#pragma unroll
-        for (int c = 0; c < D / 8; ++c)
-          st_shared_v4(q_dst + (c / 8) * kBoxBytes + (((c % 8) ^ (row & 7)) * 16), q4[c].x, q4[c].y, q4[c].z, q4[c].w);
-        if (!p.q_vec && live) {
-#pragma unroll 1
-          for (int c = 0; c < p.dim / 8; ++c) {
-            uint32_t w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              w[i] = static_cast<uint32_t>(q_row[c * 8 + 2 * i]) | (static_cast<uint32_t>(q_row[c * 8 + 2 * i + 1]) << 16);
-            st_shared_v4(q_dst + (c / 8) * kBoxBytes + (((c % 8) ^ (row & 7)) * 16), w[0], w[1], w[2], w[3]);
-          }
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(Q_FULL));
-      }
       }
       if (!PAIR && x == 1 && runs > 0 && !mbar_wait(bar(O_READ), (runs - 1) & 1, abort_flag)) {
         give_up(99, runs);                      // A has read this group's O of the run before
@@ -611,19 +641,19 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         const int key0 = j * kPaBN;
         const bool edge = key0 + kPaBN > have;       // the step's tokens, or slots behind the last one
         uint32_t sees[4] = {0u, 0u, 0u, 0u};
-        if (edge && live) {
+        if (edge && any_live) {
           const Run run = saved_run(mine);
           const int t = place_in(run).t;
-          const uint8_t* mask = p.mask == nullptr ? nullptr : p.mask + run.b * p.mask_b + t * p.mask_t;
+          const int t0 = __shfl_sync(0xffffffffu, t, 0);
+          const int t1 = min(__shfl_sync(0xffffffffu, t, 31), run.seq.fresh - 1);
 #pragma unroll 1
           for (int w = 0; w < 4; ++w) {                  // rolled: the words move up
             sees[0] = sees[1];
             sees[1] = sees[2];
             sees[2] = sees[3];
-            sees[3] = visible_keys(mask, p.mask_j, have, run.seq.fresh, t, key0 + 32 * w);
+            sees[3] = visible_keys(p, run.seq, run.b, t, t0, t1, key0 + 32 * w, lane);
           }
         }
-        __syncwarp();
         if (!mbar_wait(bar(S_FULL + x), sp, abort_flag)) {
           give_up(96, j);
           break;
@@ -725,7 +755,10 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
 #pragma unroll
             for (int k = 0; k < 32; ++k) {
               const float2 y = __ffma2_rn(make_float2(s[2 * k], s[2 * k + 1]), scale2, negm2);
-              const float2 e = make_float2(fast_exp2(y.x), fast_exp2(y.y));
+              // pair: every fourth pair on the FMA pipe, as two row tiles keep the special-function
+              // unit busier than the tensor cores (133 -> 130 us); split waits for memory
+              const bool poly = PAIR && k % kFmhaPolyEvery == kFmhaPolyEvery - 1;
+              const float2 e = poly ? exp2_poly_pair(y) : make_float2(fast_exp2(y.x), fast_exp2(y.y));
               sum2[k & 3] = __fadd2_rn(sum2[k & 3], e);
               // P is rounded to the input type: it is the tensor cores' operand
               pk[k] = BF16 ? pack_bf16x2(e.x, e.y) : pack_f16x2(e.x, e.y);
@@ -754,6 +787,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       }
       tile0 += n;
       if (!ok) break;
+      more = open_run(saved_walk(mine), runs + 1);
       if (!PAIR && x == 1) continue;                      // A finishes the run
       const bool edges = (first_tile + n) * kPaBN > have;
       const bool two = !PAIR && n > 1;                    // B has a share of it
@@ -779,17 +813,14 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       const Run run = saved_run(mine);
       const Place at = place_in(run);
       const bool whole = run.first == 0 && run.last == run.seq.tiles;
-      const int64_t slot = (2 * static_cast<int64_t>(blockIdx.x) + (runs == 0 ? 0 : 1)) * p.tile_rows +
-                           (PAIR ? x * kPaBM : 0) + row;
+      const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (runs == 0 ? 0 : 1);
+      const int tile_row = (PAIR ? x * kPaBM : 0) + row;
       const float inv_l = (l > 0.0f) ? __fdividef(1.0f, l) : (l == 0.0f ? 0.0f : l);
       const bool by_hand = edges && bad_draft[runs & 1] == runs;
       const bool to_out = whole && !by_hand;
       uint16_t* o_row = p.out + run.b * p.o_b + at.hq * p.o_h + at.t * p.o_t;
-      float* acc = p.ws_acc + slot * D;
-      if (live && !whole) {
-        p.ws_ml[2 * slot] = m_used;
-        p.ws_ml[2 * slot + 1] = l;
-      }
+      float4* acc = reinterpret_cast<float4*>(p.ws_acc) + slot * (D / 4) * p.tile_rows + tile_row;
+      if (live && !whole) reinterpret_cast<float2*>(p.ws_ml)[slot * p.tile_rows + tile_row] = make_float2(m_used, l);
       if (any_live) {
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
@@ -829,13 +860,14 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
               }
             }
           } else if (live) {
-            float4* dst = reinterpret_cast<float4*>(acc + c * 32);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) dst[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+            for (int k = 0; k < 8; ++k)                   // neighbouring rows side by side
+              acc[static_cast<int64_t>(c * 8 + k) * p.tile_rows] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
           }
           __syncwarp();
         }
-        if (by_hand && live) add_cleared_drafts<D, BF16>(p, run, at.hq, at.t, acc, m_used, inv_l, whole);
+        if (by_hand && live) 
+          add_cleared_drafts<D, BF16>(p, run, at.hq, at.t, reinterpret_cast<float*>(acc), m_used, inv_l, whole);
         __syncwarp();
       }
       tc_fence_before_sync();
@@ -855,88 +887,78 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
   }
 }
 
-// Joins the partial states of items that several CTAs share, and clears padding rows.  A warp
-// owns a row: lanes read the partial maxima and sums side by side, then every lane adds up its
-// columns over the partials.
-template <int D, bool BF16>
-__global__ void __launch_bounds__(kPaJoinThreads)
+// Joins the partial states of items that several CTAs share, and clears padding rows.  A thread owns
+// four columns of a row (neighbouring threads neighbouring rows, as the states are stored) and
+// takes every G-th state in range order; its G partners' results meet in shared memory.
+template <int D, bool BF16, bool PAIR, int G>
+__global__ void __launch_bounds__(kPaJoinThreads * G)
 paged_attention_join_kernel(const __grid_constant__ PagedParams p) {
-  constexpr int kCols = D / 32;              // columns of a lane
   const int lane = threadIdx.x & 31;
   const int per_seq = p.heads_kv * p.row_tiles;
   const int b = blockIdx.y / per_seq, item = blockIdx.y - b * per_seq;
   const int head = item / p.row_tiles, row_tile = item - head * p.row_tiles;
-  const int row = blockIdx.x * (kPaJoinThreads / 32) + (threadIdx.x >> 5);
-  const int r = row_tile * p.tile_height + row;
+  const int element = blockIdx.x * kPaJoinThreads + threadIdx.x % kPaJoinThreads;
+  const int quad = element / p.tile_rows, row = element - quad * p.tile_rows;
   const SeqInfo seq = seq_info(p, b);
   const Ranges ranges(tiles_before(p, p.batch, lane) * per_seq, p.ctas);
   const int first = tiles_before(p, b, lane) * per_seq + item * seq.tiles;
   // the partial states come from the kernel launched just before; every thread waits for it, so
   // that this kernel's end is that one's end too
   pdl_wait();
-  if (row >= p.tile_rows || r >= p.rows) return;
-  const int t = r / p.group;
-  uint16_t* o_row = p.out + b * p.o_b + static_cast<int64_t>(head * p.group + (r - t * p.group)) * p.o_h + t * p.o_t;
-  const int d0 = lane * kCols;
-  float o[kCols];
-#pragma unroll
-  for (int i = 0; i < kCols; ++i) o[i] = 0.f;
-  bool store = false;
-  if (t < seq.fresh && seq.tiles == 0) {
-    store = true;                            // nothing to see: zeros
-  } else if (t < seq.fresh) {
-    const int c0 = ranges.owner(first), c1 = ranges.owner(first + seq.tiles - 1);
-    if (c0 != c1) {
-      store = true;
+  const int half = row / kPaBM, in_half = (row - half * kPaBM) / p.group;
+  const int hq = head * p.group + (row - half * kPaBM) - in_half * p.group;
+  const int t = (PAIR ? row_tile * 2 + half : row_tile) * p.half_tokens + in_half;
+  const bool mine = quad * 4 < p.dim && in_half < p.half_tokens && t < p.tokens;
+  const bool real = mine && t < seq.fresh;
+  const int c0 = seq.tiles > 0 ? ranges.owner(first) : 0, c1 = seq.tiles > 0 ? ranges.owner(first + seq.tiles - 1) : 0;
+  float m = -INFINITY, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto take = [&](float mc, float lc, const float4& a) {
+    if (mc == -INFINITY) return;              // saw nothing
+    const float top = fmaxf(m, mc);
+    const float f = (m == -INFINITY) ? 0.f : exp2f(m - top), g = exp2f(mc - top);
+    l = l * f + lc * g;
+    o.x = o.x * f + a.x * g;
+    o.y = o.y * f + a.y * g;
+    o.z = o.z * f + a.z * g;
+    o.w = o.w * f + a.w * g;
+    m = top;
+  };
+  if (c0 != c1 && real) {
+    const float4* acc = reinterpret_cast<const float4*>(p.ws_acc);
+    const float2* ml = reinterpret_cast<const float2*>(p.ws_ml);
+#pragma unroll 4
+    for (int c = c0 + threadIdx.x / kPaJoinThreads; c <= c1; c += G) {
       // only the first of an item's CTAs may have begun with an earlier item
-      auto slot = [&](int c) {
-        return (2 * static_cast<int64_t>(c) + (ranges.begin(c) >= first ? 0 : 1)) * p.tile_rows + row;
-      };
-      float m = -INFINITY;
-      for (int c = c0 + lane; c <= c1; c += 32)
-        if (ranges.begin(c) < ranges.begin(c + 1)) m = fmaxf(m, p.ws_ml[2 * slot(c)]);
-#pragma unroll
-      for (int s = 16; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
-      float l = 0.f;
-      for (int base = c0; base <= c1; base += 32) {
-        float f = 0.f;
-        int64_t at = 0;
-        const int c = base + lane;
-        // a range may be empty where there are fewer tiles than CTAs
-        if (c <= c1 && ranges.begin(c) < ranges.begin(c + 1)) {
-          at = slot(c);
-          const float mc = p.ws_ml[2 * at];
-          f = (mc == -INFINITY) ? 0.f : exp2f(mc - m);
-          l += f * p.ws_ml[2 * at + 1];
-        }
-        const int n = min(32, c1 - base + 1);
-#pragma unroll 2
-        for (int k = 0; k < n; ++k) {
-          const float fk = __shfl_sync(0xffffffffu, f, k);
-          const int64_t ak = __shfl_sync(0xffffffffu, at, k);
-          if (fk != 0.f) {
-            const float* src = p.ws_acc + ak * D + d0;
-#pragma unroll
-            for (int i = 0; i < kCols; ++i) o[i] = fmaf(fk, src[i], o[i]);
-          }
-        }
-      }
-#pragma unroll
-      for (int s = 16; s > 0; s >>= 1) l += __shfl_xor_sync(0xffffffffu, l, s);
-      const float inv_l = (l > 0.0f) ? __fdividef(1.0f, l) : (l == 0.0f ? 0.0f : l);
-#pragma unroll
-      for (int i = 0; i < kCols; ++i) o[i] *= inv_l;
+      const int64_t slot = 2 * static_cast<int64_t>(c) + (ranges.begin(c) >= first ? 0 : 1);
+      const float2 state = ml[slot * p.tile_rows + row];
+      take(state.x, state.y, acc[(slot * (D / 4) + quad) * p.tile_rows + row]);
     }
-  } else {
-    store = p.zero_padding != 0;
   }
-  if (!store) return;
+  if constexpr (G > 1) {
+    __shared__ float2 sm_ml[G][kPaJoinThreads];
+    __shared__ float4 sm_o[G][kPaJoinThreads];
+    const int g = threadIdx.x / kPaJoinThreads, e = threadIdx.x % kPaJoinThreads;
+    sm_ml[g][e] = make_float2(m, l);
+    sm_o[g][e] = o;
+    __syncthreads();
+    if (g > 0) return;
 #pragma unroll
-  for (int i = 0; i < kCols; ++i) {
-    if (d0 + i < p.dim) {
-      if constexpr (BF16) reinterpret_cast<__nv_bfloat16*>(o_row)[d0 + i] = __float2bfloat16_rn(o[i]);
-      else reinterpret_cast<__half*>(o_row)[d0 + i] = __float2half_rn(o[i]);
-    }
+    for (int k = 1; k < G; ++k) take(sm_ml[k][e].x, sm_ml[k][e].y, sm_o[k][e]);
+  }
+  // a row of an item that one CTA has finished is in place; a padding row is cleared on request
+  if (!mine || (real && c0 == c1 && seq.tiles > 0) || (!real && !p.zero_padding)) return;
+  const float inv_l = (l > 0.0f) ? __fdividef(1.0f, l) : (l == 0.0f ? 0.0f : l);
+  uint16_t* dst = p.out + b * p.o_b + static_cast<int64_t>(hq) * p.o_h + t * p.o_t + quad * 4;
+  const uint32_t lo = BF16 ? pack_bf16x2(o.x * inv_l, o.y * inv_l) : pack_f16x2(o.x * inv_l, o.y * inv_l);
+  const uint32_t hi = BF16 ? pack_bf16x2(o.z * inv_l, o.w * inv_l) : pack_f16x2(o.z * inv_l, o.w * inv_l);
+  if (p.o_vec) {
+    *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
+  } else {
+    dst[0] = static_cast<uint16_t>(lo & 0xffff);
+    dst[1] = static_cast<uint16_t>(lo >> 16);
+    dst[2] = static_cast<uint16_t>(hi & 0xffff);
+    dst[3] = static_cast<uint16_t>(hi >> 16);
   }
 }
 
@@ -944,17 +966,19 @@ paged_attention_join_kernel(const __grid_constant__ PagedParams p) {
 
 int padded_dim(const b200k_paged_attention_args* a) { return a->head_dim <= 64 ? 64 : 128; }
 
-// Rows that share a key/value head, and how they are cut: one 128-row tile ("split"), or tiles of
-// 256 ("pair") where there are more.
+// The rows that share a key/value head, token by token, and how they are cut: one 128-row half
+// ("split"), or tiles of two halves ("pair") where there are more.  A half holds whole tokens.
 struct Rows {
-  int64_t all, height, tiles, per_tile;
+  bool pair;
+  int64_t half_tokens, tiles, per_tile;
 };
 Rows lay_out_rows(const b200k_paged_attention_args* a) {
+  const int64_t group = a->heads_q / a->heads_kv;
   Rows r;
-  r.all = a->tokens * (a->heads_q / a->heads_kv);
-  r.height = r.all <= kPaBM ? kPaBM : 2 * kPaBM;
-  r.tiles = ceil_div(r.all, r.height);
-  r.per_tile = r.all < r.height ? r.all : r.height;
+  r.pair = a->tokens * group > kPaBM;
+  r.half_tokens = r.pair ? kPaBM / group : a->tokens;
+  r.tiles = r.pair ? ceil_div(a->tokens, 2 * r.half_tokens) : 1;
+  r.per_tile = r.pair ? 2 * kPaBM : a->tokens * group;
   return r;
 }
 
@@ -971,6 +995,8 @@ int check_args(const b200k_paged_attention_args* a) {
   if (a->batch < 0 || a->tokens < 0 || a->heads_q < 0 || a->heads_kv <= 0 || a->num_pages < 0 || a->max_pages < 0)
     return fail(B200K_INVALID_ARG, "negative dimension, or no key/value heads");
   if (a->heads_q % a->heads_kv != 0) return fail(B200K_INVALID_ARG, "heads_q must be a multiple of heads_kv");
+  if (a->heads_q > kPaBM * a->heads_kv)
+    return fail(B200K_UNSUPPORTED, "at most %d query heads per key/value head", kPaBM);
   if (a->dtype != B200K_F16 && a->dtype != B200K_BF16) return fail(B200K_INVALID_ARG, "dtype must be f16 or bf16");
   if (a->head_dim <= 0 || a->head_dim > 128 || a->head_dim % 8 != 0)
     return fail(B200K_UNSUPPORTED, "head_dim must be a multiple of 8 up to 128 (got %d)", a->head_dim);
@@ -988,7 +1014,7 @@ int check_args(const b200k_paged_attention_args* a) {
 }
 
 template <int D, bool BF16, bool PAIR>
-int launch_paged_as(const CUtensorMap& tk, const CUtensorMap& tv, const PagedParams& p, int64_t items, cudaStream_t stream) {
+int launch_paged_as(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const PagedParams& p, int64_t items, cudaStream_t stream) {
   constexpr int kSmem = Rings<D, PAIR>::kSmem;
   auto kernel = paged_attention_kernel<D, BF16, PAIR>;
   static bool configured[64] = {};
@@ -1000,19 +1026,25 @@ int launch_paged_as(const CUtensorMap& tk, const CUtensorMap& tv, const PagedPar
       return fail(B200K_CUDA_ERROR, "cudaFuncSetAttribute(%d): %s", kSmem, cudaGetErrorString(e));
     configured[dev] = true;
   }
-  kernel<<<p.ctas, kPaThreads, kSmem, stream>>>(tk, tv, p);
+  kernel<<<p.ctas, kPaThreads, kSmem, stream>>>(tq, tk, tv, p);
   B200K_CHECK_LAUNCH("paged attention launch");
-  const dim3 grid(static_cast<unsigned>(ceil_div(p.tile_rows, kPaJoinThreads / 32)), static_cast<unsigned>(items));
-  const cudaError_t e = launch_after_predecessor(paged_attention_join_kernel<D, BF16>, grid, dim3(kPaJoinThreads), 0,
-                                                 stream, p);
+  const dim3 grid(static_cast<unsigned>(ceil_div(static_cast<int64_t>(p.tile_rows) * (D / 4), kPaJoinThreads)),
+                  static_cast<unsigned>(items));
+  // few blocks mean few items, each shared by many CTAs: eight threads to an output then
+  static_assert(kSmem <= 227 * 1024, "shared memory of one CTA");
+  const cudaError_t e =
+      static_cast<int64_t>(grid.x) * grid.y >= 2 * current_sm_count()
+          ? launch_after_predecessor(paged_attention_join_kernel<D, BF16, PAIR, 1>, grid, dim3(kPaJoinThreads), 0, stream, p)
+          : launch_after_predecessor(paged_attention_join_kernel<D, BF16, PAIR, 8>, grid, dim3(kPaJoinThreads * 8), 0, stream, p);
   if (e != cudaSuccess) return fail(B200K_CUDA_ERROR, "paged attention join launch: %s", cudaGetErrorString(e));
   return B200K_OK;
 }
 
 template <int D, bool BF16>
-int launch_paged(const CUtensorMap& tk, const CUtensorMap& tv, const PagedParams& p, int64_t items, cudaStream_t stream) {
-  return p.tile_height == kPaBM ? launch_paged_as<D, BF16, false>(tk, tv, p, items, stream)
-                                : launch_paged_as<D, BF16, true>(tk, tv, p, items, stream);
+int launch_paged(bool pair, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const PagedParams& p,
+                 int64_t items, cudaStream_t stream) {
+  return pair ? launch_paged_as<D, BF16, true>(tq, tk, tv, p, items, stream)
+              : launch_paged_as<D, BF16, false>(tq, tk, tv, p, items, stream);
 }
 
 }  // namespace
@@ -1035,10 +1067,12 @@ extern "C" int b200k_paged_attention(const b200k_paged_attention_args* a, b200k_
   if (a->batch == 0 || a->tokens == 0 || a->heads_q == 0) return B200K_OK;
   if (!a->q || !a->k_cache || !a->v_cache || !a->out || !a->page_table || !a->cache_lens)
     return fail(B200K_INVALID_ARG, "null pointer");
-  for (int64_t s : {a->kc_stride_p, a->kc_stride_h, a->kc_stride_s, a->vc_stride_p, a->vc_stride_h, a->vc_stride_s})
-    if (s < 0 || s % 8 != 0) return fail(B200K_UNSUPPORTED, "cache strides must be multiples of 16 bytes");
-  if ((reinterpret_cast<uintptr_t>(a->k_cache) | reinterpret_cast<uintptr_t>(a->v_cache)) & 15)
-    return fail(B200K_UNSUPPORTED, "caches must be 16-byte aligned");
+  for (int64_t s : {a->q_stride_b, a->q_stride_h, a->q_stride_t, a->kc_stride_p, a->kc_stride_h, a->kc_stride_s,
+                    a->vc_stride_p, a->vc_stride_h, a->vc_stride_s})
+    if (s < 0 || s % 8 != 0) return fail(B200K_UNSUPPORTED, "query and cache strides must be multiples of 16 bytes");
+  if ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->k_cache) |
+       reinterpret_cast<uintptr_t>(a->v_cache)) & 15)
+    return fail(B200K_UNSUPPORTED, "queries and caches must be 16-byte aligned");
   if (a->num_pages == 0) return fail(B200K_INVALID_ARG, "the cache has no pages");
   const int sms = current_sm_count();
   if (sms <= 0) return fail(B200K_CUDA_ERROR, "no current CUDA device");
@@ -1067,9 +1101,8 @@ extern "C" int b200k_paged_attention(const b200k_paged_attention_args* a, b200k_
   p.heads_kv = static_cast<int>(a->heads_kv);
   p.group = static_cast<int>(a->heads_q / a->heads_kv);
   p.dim = a->head_dim;
-  p.rows = p.tokens * p.group;
   const Rows rows = lay_out_rows(a);
-  p.tile_height = static_cast<int>(rows.height);
+  p.half_tokens = static_cast<int>(rows.half_tokens);
   p.row_tiles = static_cast<int>(rows.tiles);
   p.tile_rows = static_cast<int>(rows.per_tile);
   p.page_size = a->page_size;
@@ -1082,7 +1115,6 @@ extern "C" int b200k_paged_attention(const b200k_paged_attention_args* a, b200k_
   const auto vec = [](const void* base, int64_t sb, int64_t sh, int64_t st) {
     return (reinterpret_cast<uintptr_t>(base) & 15) == 0 && sb % 8 == 0 && sh % 8 == 0 && st % 8 == 0;
   };
-  p.q_vec = vec(a->q, p.q_b, p.q_h, p.q_t);
   p.o_vec = vec(a->out, p.o_b, p.o_h, p.o_t);
   p.zero_padding = a->zero_padding;
   p.scale_log2 = a->qk_scale * 1.4426950408889634f;
@@ -1093,17 +1125,26 @@ extern "C" int b200k_paged_attention(const b200k_paged_attention_args* a, b200k_
 
   const CUtensorMapDataType dt =
       a->dtype == B200K_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  CUtensorMap tk, tv;
-  if (!encode_tmap_4d(&tk, dt, a->k_cache, a->head_dim, a->page_size, a->heads_kv, a->num_pages, p.kc_s * 2, p.kc_h * 2,
-                      p.kc_p * 2, 64, p.box_rows, 1, 1, CU_TENSOR_MAP_SWIZZLE_128B) ||
-      !encode_tmap_4d(&tv, dt, a->v_cache, a->head_dim, a->page_size, a->heads_kv, a->num_pages, p.vc_s * 2, p.vc_h * 2,
-                      p.vc_p * 2, 64, p.box_rows, 1, 1, CU_TENSOR_MAP_SWIZZLE_128B))
+  CUtensorMap tq, tk, tv;
+  // the stride of an axis of one entry is never used, but has to be one that a tensor map takes
+  const auto bytes = [](int64_t entries, int64_t stride) -> uint64_t { return entries == 1 ? 16 : stride * 2; };
+  if (!encode_tmap_4d(&tq, dt, a->q, a->head_dim, a->heads_q, a->tokens, a->batch, bytes(a->heads_q, p.q_h),
+                      bytes(a->tokens, p.q_t), bytes(a->batch, p.q_b), 64, p.group, p.half_tokens, 1,
+                      CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !encode_tmap_4d(&tk, dt, a->k_cache, a->head_dim, a->page_size, a->heads_kv, a->num_pages,
+                      bytes(a->page_size, p.kc_s), bytes(a->heads_kv, p.kc_h), bytes(a->num_pages, p.kc_p), 64,
+                      p.box_rows, 1, 1, CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !encode_tmap_4d(&tv, dt, a->v_cache, a->head_dim, a->page_size, a->heads_kv, a->num_pages,
+                      bytes(a->page_size, p.vc_s), bytes(a->heads_kv, p.vc_h), bytes(a->num_pages, p.vc_p), 64,
+                      p.box_rows, 1, 1, CU_TENSOR_MAP_SWIZZLE_128B))
     return B200K_INVALID_ARG;
   const int64_t items = a->batch * a->heads_kv * p.row_tiles;
   if (items > 65535) return fail(B200K_UNSUPPORTED, "more row tiles than the kernel counts");
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   const bool bf16 = a->dtype == B200K_BF16;
   if (d == 128)
-    return bf16 ? launch_paged<128, true>(tk, tv, p, items, stream) : launch_paged<128, false>(tk, tv, p, items, stream);
-  return bf16 ? launch_paged<64, true>(tk, tv, p, items, stream) : launch_paged<64, false>(tk, tv, p, items, stream);
+    return bf16 ? launch_paged<128, true>(rows.pair, tq, tk, tv, p, items, stream)
+                : launch_paged<128, false>(rows.pair, tq, tk, tv, p, items, stream);
+  return bf16 ? launch_paged<64, true>(rows.pair, tq, tk, tv, p, items, stream)
+              : launch_paged<64, false>(rows.pair, tq, tk, tv, p, items, stream);
 }

@@ -113,7 +113,9 @@ def test_refusals_of_the_entry_point():
         assert call(qk_scale=scale) == _lib.INVALID_ARG
     assert call(q=None) == _lib.INVALID_ARG
     assert call(page_table=None) == _lib.INVALID_ARG
+    assert call(heads_q=258) == _lib.UNSUPPORTED
     assert call(kc_stride_s=60) == _lib.UNSUPPORTED
+    assert call(q_stride_t=60) == _lib.UNSUPPORTED
     assert call(v_cache=(1 << 20) + 8) == _lib.UNSUPPORTED
     assert call(num_pages=0) == _lib.INVALID_ARG
     assert call(tokens=0, q=None) == _lib.OK
@@ -186,6 +188,21 @@ def test_many_tiles_in_a_row(b, hq, hkv, t, d, lens, tree, device_ok):
     c.check(first, mask)
     for _ in range(3):
         assert torch.equal(c.run(tree_mask=mask), first)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("b,hq,hkv,t,d,lens,new", [
+    (2, 6, 2, 60, 64, [500, 37], [60, 50]),      # three heads a token: halves of 126 rows
+    (1, 7, 1, 40, 128, [300], None),             # halves of 18 tokens, 126 rows
+    (2, 128, 1, 2, 64, [200, 0], [1, 2]),        # a token's heads fill a half
+    (1, 100, 1, 3, 128, [130], None),            # 100 of 128 rows a half, the last half empty
+    (1, 10, 5, 64, 96, [1000], None)])
+def test_row_tiles_of_whole_tokens(b, hq, hkv, t, d, lens, new, device_ok):
+    c = Cache(b, hq, hkv, t, d, torch.bfloat16, 16, lens, new)
+    for mask in (None, _tree(b, t, seed=3)):
+        c.check(c.run(tree_mask=mask), mask)
+    c.q = c.q[:1].expand(b, hq, t, d) if b > 1 else c.q
+    c.check(c.run())
 
 
 @pytest.mark.gpu
@@ -353,6 +370,8 @@ def test_refused_inputs(device_ok):
     with pytest.raises(ValueError, match="16-byte"):
         wide = torch.zeros(4, 2, 16, 68, dtype=torch.bfloat16, device="cuda")[..., :64]
         call(kc=wide, vc=wide)
+    with pytest.raises(ValueError, match="at most 128 query heads"):
+        call(q=torch.zeros(2, 258, 3, 64, dtype=torch.bfloat16, device="cuda"))
     with pytest.raises(ValueError, match="multiple of 8 up to 128"):
         big = torch.zeros(4, 2, 16, 136, dtype=torch.bfloat16, device="cuda")
         call(q=torch.zeros(2, 4, 3, 136, dtype=torch.bfloat16, device="cuda"), kc=big, vc=big)
