@@ -157,6 +157,41 @@ __device__ __forceinline__ bool next_run(const PagedParams& p, Walk& w, Run& r) 
   return true;
 }
 
+// Where this CTA's range begins, warp-collective.
+__device__ __forceinline__ Walk walk_start(const PagedParams& p, int lane) {
+  const int per_seq = p.heads_kv * p.row_tiles;
+  const Ranges ranges(tiles_before(p, p.batch, lane) * per_seq, p.ctas);
+  const int begin = ranges.begin(blockIdx.x);
+  Walk w;
+  w.left = ranges.begin(blockIdx.x + 1) - begin;
+  w.b = w.item = w.tile = 0;
+  int before = 0;
+#pragma unroll 1
+  for (int b0 = 0; b0 < p.batch && w.left > 0; b0 += 32) {
+    const int b = b0 + lane;
+    const int tiles = b < p.batch ? seq_info(p, b).tiles : 0;
+    const int mine = tiles * per_seq;
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    const uint32_t here = __ballot_sync(0xffffffffu, begin >= before + upto - mine && begin < before + upto);
+    if (here != 0) {
+      const int from = __ffs(here) - 1;
+      const int in_seq = begin - before - __shfl_sync(0xffffffffu, upto - mine, from);
+      const int its = __shfl_sync(0xffffffffu, tiles, from);
+      w.b = b0 + from;
+      w.item = in_seq / its;
+      w.tile = in_seq - w.item * its;
+      break;
+    }
+    before += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  return w;
+}
+
 // A softmax warp's walk and run, in shared memory: what a run needs at its two ends only would
 // otherwise be spilled to local memory, whose lines the 20 KB of L1 beside the tiles do not hold.
 constexpr int kRunWords = 13;
@@ -282,7 +317,6 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail + 384);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + 392);
   volatile int* bad_draft = reinterpret_cast<volatile int*>(tail + 400);   // [2], by run parity
-  Walk* walk_start = reinterpret_cast<Walk*>(tail + 408);
   float2* state_b = reinterpret_cast<float2*>(tail + 448);                 // [128] maximum and sum of B's rows
   volatile int* run_words = reinterpret_cast<volatile int*>(tail + 1472);  // [8 softmax warps][2][kRunWords]
 
@@ -315,47 +349,28 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     tmem_alloc(smem_u32(tmem_slot), kPaTmemCols);
     tmem_relinquish();
   }
-  if (warp == 2) {
-    // this CTA's range of key tiles and the item it begins in
-    const int per_seq = p.heads_kv * p.row_tiles;
-    const Ranges ranges(tiles_before(p, p.batch, lane) * per_seq, p.ctas);
-    Walk w;
-    const int begin = ranges.begin(blockIdx.x);
-    w.left = ranges.begin(blockIdx.x + 1) - begin;
-    w.b = 0;
-    w.item = 0;
-    w.tile = 0;
-    int before = 0;
-#pragma unroll 1
-    for (int b0 = 0; b0 < p.batch && w.left > 0; b0 += 32) {
-      const int b = b0 + lane;
-      const int tiles = b < p.batch ? seq_info(p, b).tiles : 0;
-      const int mine = tiles * per_seq;
-      int upto = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += v;
-      }
-      const bool here = begin >= before + upto - mine && begin < before + upto;
-      if (__any_sync(0xffffffffu, here)) {
-        if (here) {
-          const int in_seq = begin - (before + upto - mine);
-          w.b = b;
-          w.item = in_seq / tiles;
-          w.tile = in_seq - w.item * tiles;
-          *walk_start = w;
-        }
-        break;
-      }
-      before += __shfl_sync(0xffffffffu, upto, 31);
+  // what the kernel before this one in the stream writes is read from here on
+  pdl_wait();
+  Walk walk = walk_start(p, lane);   // every warp finds its own: no wait for another's
+  Run run;
+  bool have_run = next_run(p, walk, run);
+  // the K and V producers' lane i looks up the i-th run of slots of a tile, all of one page
+  const int boxes_per_tile = kPaBN / p.box_rows;
+  auto find = [&](int j, int& page, int& slot) {
+    const int key = j * kPaBN + lane * p.box_rows;
+    page = slot = 0;
+    if (lane < boxes_per_tile && key < run.seq.len) {
+      const int entry = key / p.page_size;
+      slot = key - entry * p.page_size;
+      page = p.page_table[run.b * p.page_table_stride + entry];
     }
-    if (w.left <= 0 && lane == 0) *walk_start = w;
-    if (blockIdx.x == 0) {
+  };
+  int page = 0, slot = 0;
+  if (have_run && (warp == 0 || warp == 10)) find(run.first, page, slot);
+  if (blockIdx.x == 0 && warp == 2) {
 #pragma unroll 1
-      for (int b = lane; b < p.batch; b += 32)
-        if (!lengths_fit(p, b)) report_bad_index(p.status, kRolePage, b);
-    }
+    for (int b = lane; b < p.batch; b += 32)
+      if (!lengths_fit(p, b)) report_bad_index(p.status, kRolePage, b);
   }
   tc_fence_before_sync();
   __syncthreads();
@@ -366,9 +381,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   if (warp == 11) {
     // the Q producer: a run's rows once the last S of the run before has read its own, and a
     // prefetch of the next run's into the L2 (cold, they took 10 us of a full memory system)
-    Walk walk = *walk_start;
-    Run run, next;
-    bool have_run = next_run(p, walk, run), ok = true;
+    Run next;
+    bool ok = true;
     const bool elected = elect_one();
     constexpr int kHalves = PAIR ? 2 : 1;
     const uint32_t bytes = static_cast<uint32_t>(p.half_tokens * p.group) * 128u * kBoxes * kHalves;
@@ -401,32 +415,17 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     if (runs > 0) mbar_wait(bar(Q_FULL), (runs - 1) & 1, abort_flag);   // nothing in flight when the CTA leaves
     __syncwarp();
   } else if (warp == 0 || warp == 10) {
-    Walk walk = *walk_start;
-    Run run;
     const bool is_v = warp != 0;
     const CUtensorMap* tmap = is_v ? &tmap_v : &tmap_k;
     const int full = is_v ? V_FULL : K_FULL, empty = is_v ? V_EMPTY : K_EMPTY, places = is_v ? R::kV : R::kK;
     const uint32_t ring = is_v ? v_smem : k_smem;
-    const int boxes_per_tile = kPaBN / p.box_rows;
     const uint32_t box_bytes = p.box_rows * 128u;
     const bool elected = elect_one();
     bool ok = true;
     int place = 0, fills = 0;
     uint32_t parity = 1;                       // a fresh ring is empty
-    while (ok && next_run(p, walk, run)) {
-      const int* pages = p.page_table + run.b * p.page_table_stride;
-      // lane i: the i-th run of slots of a tile, all of one page
-      auto find = [&](int j, int& page, int& slot) {
-        const int key = j * kPaBN + lane * p.box_rows;
-        page = slot = 0;
-        if (lane < boxes_per_tile && key < run.seq.len) {
-          const int entry = key / p.page_size;
-          slot = key - entry * p.page_size;
-          page = pages[entry];
-        }
-      };
-      int page, slot;
-      find(run.first, page, slot);
+    for (int runs = 0; have_run && ok; ++runs) {
+      if (runs > 0) find(run.first, page, slot);
       for (int j = run.first; j < run.last; ++j) {
         int next_page = 0, next_slot = 0;
         if (j + 1 < run.last) find(j + 1, next_page, next_slot);   // on its way while this tile is issued
@@ -460,6 +459,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         page = next_page;
         slot = next_slot;
       }
+      have_run = next_run(p, walk, run);
     }
     // no copy of this warp is in flight when the CTA leaves (bounded, also after a failure): the
     // last fill of every ring place
@@ -467,8 +467,6 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       mbar_wait(bar(full + i), ((fills - 1 - i) / places) & 1, abort_flag);
     __syncwarp();
   } else if (warp == 1) {
-    Walk walk = *walk_start;
-    Run run;
     const bool elected = elect_one();
     constexpr uint32_t idesc_qk = make_idesc(kFmt, kFmt, false, false, kPaBM, kPaBN);
     constexpr uint32_t idesc_pv = make_idesc(kFmt, kFmt, false, true, kPaBM, D);
@@ -519,7 +517,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       if (elected) tc_commit(bar(V_EMPTY + vs));
       if (++vs == R::kV) { vs = 0; vp ^= 1; }
     };
-    for (int runs = 0; ok && next_run(p, walk, run); ++runs) {
+    for (int runs = 0; ok && have_run; ++runs, have_run = next_run(p, walk, run)) {
       const int n = run.last - run.first;
       if (!mbar_wait(bar(Q_FULL), runs & 1, abort_flag)) {
         give_up(92, runs);
@@ -601,16 +599,9 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       q.live = in_half < p.half_tokens && q.t < run.seq.fresh;
       return q;
     };
-    auto open_run = [&](Walk walk, int number) {
-      Run run;
-      if (!next_run(p, walk, run)) return false;
-      __syncwarp();
-      if (lane == 0) save_run(words + (number & 1) * kRunWords, walk, run);
-      __syncwarp();
-      return true;
-    };
-    bool more = open_run(*walk_start, 0);
-    for (; more && ok; ++runs) {
+    if (lane == 0) save_run(words, walk, run);
+    __syncwarp();
+    for (; have_run && ok; ++runs) {
       volatile int* mine = words + (runs & 1) * kRunWords;
       int n, first_tile, have;
       bool live, any_live;
@@ -658,14 +649,15 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           give_up(96, j);
           break;
         }
-        if (edge && (!PAIR || x == 0)) {
-          // Row `row` of V is cleared where no token lies, and where a token of the step that some
-          // query may not see is not finite (added by hand in the epilogue).  S_FULL says that
-          // the P V two tiles back is done, so V_FULL's phase is this tile's or the one before.
+        // Row `row` of the tile's V is cleared where no token lies, and where a token of the step that
+        // some query may not see is not finite (added by hand in the epilogue).  After the softmax
+        // of the first half, so that V has had that long to come.  S_FULL said that the P V two
+        // tiles back is done, so V_FULL's phase is this tile's or the one before.
+        auto clear_v = [&]() {
           const int vi = tile0 + i, vs = vi % R::kV;
           if (!mbar_wait(bar(V_FULL + vs), (vi / R::kV) & 1, abort_flag)) {
             give_up(95, j);
-            break;
+            return;
           }
           // (rows lie 128 bytes apart: every lane starts at another 16-byte piece, or all would
           // meet in the same banks)
@@ -688,7 +680,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           }
           fence_proxy_async_smem();
           __syncwarp();
-        }
+        };
         tc_fence_after_sync();
         if (any_live) {                                   // a warp of padding rows only keeps step
           // S in halves of 64 scores, once for the maximum and once for the exponentials: a row of 128
@@ -765,6 +757,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
             }
             tmem_st_32x32b_x32(tmem_s + c * 32, pk);
             if (c == 0) {                                 // the first 64 keys are enough for half of P V
+              if (edge && (!PAIR || x == 0)) clear_v();
               tmem_st_wait();
               tc_fence_before_sync();
               __syncwarp();
@@ -774,9 +767,11 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           l += ((sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y)) + ((sum2[2].x + sum2[2].y) + (sum2[3].x + sum2[3].y));
           tmem_st_wait();
         } else {
+          if (edge && (!PAIR || x == 0)) clear_v();
           __syncwarp();
           if (lane == 0) mbar_arrive(bar(P_HALF + x));
         }
+        if (!ok) break;
         sp ^= 1;
         // before the last P: whoever finds the run's products done finds these arrivals made, so
         // the phases of RUN_DONE cannot lie two apart
@@ -787,7 +782,14 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       }
       tile0 += n;
       if (!ok) break;
-      more = open_run(saved_walk(mine), runs + 1);
+      {
+        Walk on = saved_walk(mine);
+        Run next;
+        have_run = next_run(p, on, next);
+        __syncwarp();
+        if (lane == 0) save_run(words + ((runs + 1) & 1) * kRunWords, on, next);
+        __syncwarp();
+      }
       if (!PAIR && x == 1) continue;                      // A finishes the run
       const bool edges = (first_tile + n) * kPaBN > have;
       const bool two = !PAIR && n > 1;                    // B has a share of it
@@ -894,6 +896,7 @@ template <int D, bool BF16, bool PAIR, int G>
 __global__ void __launch_bounds__(kPaJoinThreads * G)
 paged_attention_join_kernel(const __grid_constant__ PagedParams p) {
   const int lane = threadIdx.x & 31;
+  pdl_launch_dependents();
   const int per_seq = p.heads_kv * p.row_tiles;
   const int b = blockIdx.y / per_seq, item = blockIdx.y - b * per_seq;
   const int head = item / p.row_tiles, row_tile = item - head * p.row_tiles;
@@ -1026,14 +1029,15 @@ int launch_paged_as(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensor
       return fail(B200K_CUDA_ERROR, "cudaFuncSetAttribute(%d): %s", kSmem, cudaGetErrorString(e));
     configured[dev] = true;
   }
-  kernel<<<p.ctas, kPaThreads, kSmem, stream>>>(tq, tk, tv, p);
-  B200K_CHECK_LAUNCH("paged attention launch");
+  // programmatic launches: this kernel's set-up (barriers, tensor memory, descriptors) overlaps the
+  // end of the kernel before it, and its end the set-up of the joining kernel
+  cudaError_t e = launch_after_predecessor(kernel, dim3(p.ctas), dim3(kPaThreads), kSmem, stream, tq, tk, tv, p);
+  if (e != cudaSuccess) return fail(B200K_CUDA_ERROR, "paged attention launch: %s", cudaGetErrorString(e));
   const dim3 grid(static_cast<unsigned>(ceil_div(static_cast<int64_t>(p.tile_rows) * (D / 4), kPaJoinThreads)),
                   static_cast<unsigned>(items));
   // few blocks mean few items, each shared by many CTAs: eight threads to an output then
   static_assert(kSmem <= 227 * 1024, "shared memory of one CTA");
-  const cudaError_t e =
-      static_cast<int64_t>(grid.x) * grid.y >= 2 * current_sm_count()
+  e = static_cast<int64_t>(grid.x) * grid.y >= 2 * current_sm_count()
           ? launch_after_predecessor(paged_attention_join_kernel<D, BF16, PAIR, 1>, grid, dim3(kPaJoinThreads), 0, stream, p)
           : launch_after_predecessor(paged_attention_join_kernel<D, BF16, PAIR, 8>, grid, dim3(kPaJoinThreads * 8), 0, stream, p);
   if (e != cudaSuccess) return fail(B200K_CUDA_ERROR, "paged attention join launch: %s", cudaGetErrorString(e));

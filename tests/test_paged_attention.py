@@ -427,6 +427,37 @@ def test_captured_replayed_and_on_two_streams(device_ok):
 
 
 @pytest.mark.gpu
+def test_captured_behind_other_kinds_of_work(device_ok):
+    # behind a copy, behind a join of two streams, and one call right behind another
+    c = Cache(2, 8, 2, 3, 128, torch.bfloat16, 16, [500, 90])
+    src, side = torch.randn_like(c.q), torch.cuda.Stream()
+    c.run()
+    torch.cuda.synchronize()
+    q = c.q
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.q = q.clone(memory_format=torch.contiguous_format)
+        c.q.copy_(src)
+        one = c.run()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            other = c.kc * 1
+        c.q = c.q + 0
+        torch.cuda.current_stream().wait_stream(side)
+        two = c.run()
+        again = [c.run() for _ in range(4)][-1]
+    for _ in range(2):
+        src.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        c.q = src
+        want = c.run()
+        c.check(want)
+        assert torch.equal(one, want) and torch.equal(two, want) and torch.equal(again, want)
+    assert other.shape == c.kc.shape
+
+
+@pytest.mark.gpu
 def test_a_conversation(device_ok):
     """The operators as they are used: a prompt in two chunks of different lengths per sequence,
     two decode steps, a tree of drafts of which a path is kept, one more step.  Every step's
