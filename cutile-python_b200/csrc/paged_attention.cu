@@ -18,8 +18,10 @@
 //
 // One CTA per SM, two softmax groups A and B whose work interleaves on the tensor cores, so that
 // one's softmax overlaps the other's matrix products:
-//   split  (at most 128 rows)   A and B take the item's key tiles in turn, each with its own
-//                               running maximum, sum and O; A joins the two states at the end
+//   split  (at most 128 rows)   A and B take a run's key tiles in turn, each with its own running
+//                               maximum, sum and O; the group that began (A and B by turns)
+//                               joins the two states at the run's end, while the other already
+//                               works on the next run's first tile
 //   pair   (more rows)          A and B are two row tiles of 128, every key tile serves both
 //
 //   warps 0, 10  TMA producers of K and of V: a box per run of slots inside a page, into rings
@@ -317,7 +319,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail + 384);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + 392);
   volatile int* bad_draft = reinterpret_cast<volatile int*>(tail + 400);   // [2], by run parity
-  float2* state_b = reinterpret_cast<float2*>(tail + 448);                 // [128] maximum and sum of B's rows
+  float2* state_b = reinterpret_cast<float2*>(tail + 448);                 // [128] maximum and sum of the other group's rows
   volatile int* run_words = reinterpret_cast<volatile int*>(tail + 1472);  // [8 softmax warps][2][kRunWords]
 
   const int warp = threadIdx.x >> 5;
@@ -534,7 +536,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           issue_s(0);
           issue_s(1);
         } else {
-          issue_s(i & 1);
+          issue_s((i + runs) & 1);
         }
         free_k();
         if (i == n - 1 && elected) tc_commit(bar(Q_EMPTY));
@@ -562,7 +564,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           if (ok && more && i + 1 == n - 1 && elected) tc_commit(bar(Q_EMPTY));
           if (ok) free_v();
         } else {
-          issue_pv(i & 1, i < 2, i);
+          issue_pv((i + runs) & 1, i < 2, i);
           if (ok) free_v();
           if (ok && i + 2 < n) next_s(i + 2);
         }
@@ -578,7 +580,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     const uint32_t tmem_o = tmem_base + 256 + x * 128 + lane_addr;
     bool ok = true;
     int runs = 0;
-    int tile0 = 0, b_tiles = 0;                 // key tiles of the CTA's earlier runs; B's share of all
+    int tile0 = 0, other_tiles = 0;             // key tiles of the CTA's earlier runs; split: the other group's so far
     uint32_t sp = 0;                            // parity of the group's next S (and P V)
     auto give_up = [&](int role, int detail) {
       report_status(p.status, role, detail);
@@ -613,20 +615,21 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         first_tile = run.first;
         have = run.seq.have;
       }
-      if (!PAIR && x == 1 && runs > 0 && !mbar_wait(bar(O_READ), (runs - 1) & 1, abort_flag)) {
-        give_up(99, runs);                      // A has read this group's O of the run before
-        break;
-      }
-
+      const bool lead = PAIR || ((x + runs) & 1) == 0;   // split: takes the first tile and finishes the run
       float m_used = -INFINITY, l = 0.0f;
       // the run is this warp's no more than to its last P: what others read of it is in place
       auto leave_run = [&]() {
-        if (!PAIR && x == 1) state_b[row] = make_float2(m_used, l);
+        if (!lead) state_b[row] = make_float2(m_used, l);
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(RUN_DONE));
       };
-      const int i0 = PAIR ? 0 : x, di = PAIR ? 1 : 2;
-      if (i0 >= n) leave_run();                 // B of a single tile
+      const int i0 = lead ? 0 : 1, di = PAIR ? 1 : 2;
+      // the group that finished the run before has read this one's O of it: the first P V of this
+      // run may begin to overwrite it
+      auto await_o_read = [&](int i) {
+        if (!PAIR && lead && i == 0 && runs > 0 && !mbar_wait(bar(O_READ), (runs - 1) & 1, abort_flag)) give_up(99, runs);
+      };
+      if (i0 >= n) leave_run();                 // no share of a single tile
       for (int i = i0; i < n; i += di) {
         const int j = first_tile + i;
         const int key0 = j * kPaBN;
@@ -758,6 +761,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
             tmem_st_32x32b_x32(tmem_s + c * 32, pk);
             if (c == 0) {                                 // the first 64 keys are enough for half of P V
               if (edge && (!PAIR || x == 0)) clear_v();
+              await_o_read(i);
               tmem_st_wait();
               tc_fence_before_sync();
               __syncwarp();
@@ -768,6 +772,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           tmem_st_wait();
         } else {
           if (edge && (!PAIR || x == 0)) clear_v();
+          await_o_read(i);
           __syncwarp();
           if (lane == 0) mbar_arrive(bar(P_HALF + x));
         }
@@ -790,12 +795,12 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         if (lane == 0) save_run(words + ((runs + 1) & 1) * kRunWords, on, next);
         __syncwarp();
       }
-      if (!PAIR && x == 1) continue;                      // A finishes the run
+      other_tiles += (lead ? n : n + 1) / 2;
+      if (!lead) continue;                                // the other group finishes the run
       const bool edges = (first_tile + n) * kPaBN > have;
-      const bool two = !PAIR && n > 1;                    // B has a share of it
-      b_tiles += n / 2;
+      const bool two = !PAIR && n > 1;                    // the other group has a share of it
       if (!mbar_wait(bar(PV_DONE + x), sp ^ 1, abort_flag) ||
-          (two && !mbar_wait(bar(PV_DONE + 1), (b_tiles - 1) & 1, abort_flag)) ||
+          (two && !mbar_wait(bar(PV_DONE + (x ^ 1)), (other_tiles - 1) & 1, abort_flag)) ||
           ((!PAIR || edges) && !mbar_wait(bar(RUN_DONE), runs & 1, abort_flag))) {
         give_up(97, runs);
         break;
@@ -833,8 +838,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
             tmem_ld_wait();
 #pragma unroll
             for (int k = 0; k < 32; ++k) o[k] = __uint_as_float(y[k]);
-            if (two) {                                    // B's O lies in the same lanes
-              tmem_ld_32x32b_x32(tmem_o + 128 + c * 32, y);
+            if (two) {                                    // the other group's O lies in the same lanes
+              tmem_ld_32x32b_x32(tmem_base + 256 + (x ^ 1) * 128 + lane_addr + c * 32, y);
               tmem_ld_wait();
 #pragma unroll
               for (int k = 0; k < 32; ++k) o[k] = o[k] * fa + __uint_as_float(y[k]) * fb;
