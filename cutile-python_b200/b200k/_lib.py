@@ -353,48 +353,47 @@ class LaunchCache:
             check(code)
 
 
-def layout(*tensors) -> tuple:
-    """What a wrapper's checks and argument struct depend on: everything about the tensors but
-    their addresses and contents."""
-    return tuple([None if t is None else (t.shape, t.stride(), t.dtype, t.device, t.requires_grad)
-                  for t in tensors])
-
-
 class LayoutPlans:
-    """Checked calls of one entry point, remembered by the layouts (and scalars) that passed:
-    the argument struct with all but its pointers filled in, as bytes, plus what else the
-    wrapper derived.  A call copies the struct and sets its own pointers, so threads and streams
-    share nothing.  Checking and filling in forty fields costs 10 us of a 20 us call, the
-    lookup 3."""
+    """Checked calls of one entry point, remembered by the layouts of their tensors (shapes,
+    strides, types, devices, alignment) and their scalars: csrc/launch_plans.cpp, which a wrapper
+    asks first and whose answer is NotImplemented where it has to check the call itself.  Unlike
+    LaunchCache's, the key holds no address, and threads and streams share nothing of a call."""
 
-    def __init__(self, entry_name: str, struct: type, limit: int = 1024):
-        self.entry_name, self.struct, self.limit = entry_name, struct, limit
-        self.plans: dict = {}
-        self.fn = None
+    def __init__(self, entry_name: str, struct: type):
+        self.entry_name, self.struct = entry_name, struct
+        self.native = None
+        self.call = self._first_call
 
-    def get(self, key):
-        return self.plans.get(key)
+    def _bind(self) -> None:
+        if self.native is None:
+            try:
+                from . import _plans
+            except ImportError as e:
+                raise ImportError("b200k/_plans.so is missing or does not load: build it with "
+                                  f"`python cutile-python_b200/build.py` ({e})") from None
+            entry = ctypes.cast(getattr(lib(), self.entry_name), c_void_p).value
+            self.native = _plans.Plans(entry, check)
+            self.call = self.native.call
 
-    def put(self, key, args, *extra):
-        if len(self.plans) >= self.limit:
-            self.plans.clear()
-        plan = self.plans[key] = (bytes(args), *extra)
-        return plan
+    def _first_call(self, tensors: tuple, scalars: tuple):
+        self._bind()
+        return self.native.call(tensors, scalars)
 
-    def args(self, plan):
-        return self.struct.from_buffer_copy(plan[0])
+    def add(self, tensors: tuple, scalars: tuple, args, inputs, outputs=(), workspace: str | None = None,
+            returns=()) -> None:
+        """``args``: every field but the pointers.  ``inputs``: (field, index into tensors) of those
+        that are not None; ``outputs``: (field, index of the tensor whose shape and type it has);
+        ``workspace``: the pointer field of ``args.workspace_bytes`` of scratch; ``returns``: the
+        number of an output, -1 - i for tensors[i], or None."""
+        self._bind()
 
-    def launch(self, args, device: torch.device) -> None:
-        if self.fn is None:
-            self.fn = getattr(lib(), self.entry_name)
-        index = device.index
-        if torch.cuda.current_device() == index:
-            code = self.fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(index))
-        else:
-            with torch.cuda.device(device):
-                code = self.fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(index))
-        if code < 0:
-            check(code)
+        def offset(field):
+            return getattr(self.struct, field).offset
+
+        self.native.add(tensors, scalars, bytes(args),
+                        tuple((offset(f), i) for f, i in inputs if tensors[i] is not None),
+                        tuple((offset(f), i) for f, i in outputs), -1 if workspace is None else offset(workspace),
+                        0 if workspace is None else args.workspace_bytes, tuple(returns))
 
 
 def device_status() -> tuple[int, int]:

@@ -76,38 +76,31 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
     new_lens[b] are padding: their cache slots stay as they are, as do their rows of a given
     ``q_out``; in a q_out made here they are zero.  A token whose page lies outside the table
     or the cache is not stored, and ``raise_on_device_error()`` names its sequence."""
-    k, v, q = rows_view(k), rows_view(v), rows_view(q)
-    cos, sin = aligned_table(cos, sin)
-    key = (_lib.layout(k, v, q, k_cache, v_cache, page_table, cache_lens, cos, sin, q_weight, k_weight, positions,
-                       new_lens, q_out), eps, interleaved, torch.is_grad_enabled())
-    plan = _APPEND.get(key)
-    if plan is None:
-        plan = _APPEND.put(key, _append_args(k, v, k_cache, v_cache, page_table, cache_lens, cos, sin, q, q_weight,
-                                             k_weight, positions, new_lens, eps, interleaved, q_out))
-    a = _APPEND.args(plan)
-    a.k, a.v, a.k_cache, a.v_cache = k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
-    a.page_table, a.cache_lens = page_table.data_ptr(), cache_lens.data_ptr()
-    if new_lens is not None:
-        a.new_lens = new_lens.data_ptr()
-    if cos is not None:
-        a.cos, a.sin = cos.data_ptr(), sin.data_ptr()
-    if k_weight is not None:
-        a.k_weight = k_weight.data_ptr()
-    if positions is not None:
-        a.positions = positions.data_ptr()
-    if q is not None:
-        if q_out is None:
-            q_out = empty_rows(q)
-        a.q, a.q_out = q.data_ptr(), q_out.data_ptr()
-        if q_weight is not None:
-            a.q_weight = q_weight.data_ptr()
-    _APPEND.launch(a, k.device)
-    return q_out
+    tensors = (k, v, q, k_cache, v_cache, page_table, cache_lens, cos, sin, q_weight, k_weight, positions, new_lens, q_out)
+    scalars = eps, interleaved
+    done = _APPEND.call(tensors, scalars)
+    if done is not NotImplemented:
+        return done
+    a, rows, tables = _append_args(k, v, k_cache, v_cache, page_table, cache_lens, cos, sin, q, q_weight, k_weight,
+                                   positions, new_lens, eps, interleaved, q_out)
+    if any(r is not t for r, t in zip(rows, (k, v, q))) or tables[0] is not cos:      # the call on copies of them
+        return paged_kv_append(rows[0], rows[1], k_cache, v_cache, page_table, cache_lens, *tables, q=rows[2],
+                               q_weight=q_weight, k_weight=k_weight, positions=positions, new_lens=new_lens,
+                               eps=float(eps), interleaved=bool(interleaved), q_out=q_out)
+    scalars = float(eps), bool(interleaved)
+    own_out = q is not None and q_out is None
+    _APPEND.add(tensors, scalars, a,
+                inputs=(("k", 0), ("v", 1), ("q", 2), ("k_cache", 3), ("v_cache", 4), ("page_table", 5),
+                        ("cache_lens", 6), ("cos", 7), ("sin", 8), ("q_weight", 9), ("k_weight", 10),
+                        ("positions", 11), ("new_lens", 12), ("q_out", 13)),
+                outputs=(("q_out", 2),) if own_out else (),
+                returns=(0 if own_out else (None if q is None else -14),))
+    return _APPEND.call(tensors, scalars)
 
 
 def _append_args(k, v, k_cache, v_cache, page_table, cache_lens, cos, sin, q, q_weight, k_weight, positions,
                  new_lens, eps, interleaved, q_out):
-    """Checks a call; every field of it but the pointers."""
+    """Checks a call: every field of it but the pointers, its rows and tables as the kernel takes them."""
     if k.ndim != 4 or k.shape != v.shape:
         raise ValueError("k and v must both be 4D (Batch, KV_Heads, SeqLen, Dim).")
     if not k.is_cuda or v.device != k.device:
@@ -126,9 +119,11 @@ def _append_args(k, v, k_cache, v_cache, page_table, cache_lens, cos, sin, q, q_
         raise ValueError("cos and sin come together")
     if q is None and (q_weight is not None or q_out is not None):
         raise ValueError("q_weight and q_out need q")
+    k, v, q = rows_view(k), rows_view(v), rows_view(q)
     a = _lib.PagedKvAppendArgs()
     if cos is not None:
         a.rotary_dim = check_table(cos, sin, dim, device)
+        cos, sin = aligned_table(cos, sin)
         a.table_rows, a.table_stride = cos.shape[0], cos.stride(0)
     weight_dtype = check_weights(dim, k.dtype, device, q_weight, k_weight)
     a.position_stride_b, a.position_stride_t, a.positions_are_int64 = check_positions(positions, batch, tokens, device)
@@ -151,7 +146,7 @@ def _append_args(k, v, k_cache, v_cache, page_table, cache_lens, cos, sin, q, q_
     a.max_pages, a.page_table_stride = page_table.shape[1], page_table.stride(0)
     a.head_dim, a.interleaved = dim, 1 if interleaved else 0
     a.dtype, a.weight_dtype, a.eps = _lib.dtype_enum(k.dtype), _lib.dtype_enum(weight_dtype), eps
-    return a
+    return a, (k, v, q), (cos, sin)
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -169,32 +164,26 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     of a multiple of 8 tokens, qk_scale positive (None: 1 / sqrt(Dim)).  A query that sees no token gives zeros.  Slots that hold none of
     the sequence's tokens are never used.  Rows behind new_lens[b] are padding: they stay as
     they are in a given ``out`` and are zero in one made here."""
+    tensors, scalars = (q, k_cache, v_cache, page_table, cache_lens, new_lens, tree_mask, out), (qk_scale,)
+    done = _ATTENTION.call(tensors, scalars)
+    if done is not NotImplemented:
+        return done
+    a = _attention_args(q, k_cache, v_cache, page_table, cache_lens, new_lens, tree_mask, qk_scale, out)
+    if qk_scale is not None:
+        qk_scale = float(qk_scale)
     # the kernel's copies want the queries' rows on 16-byte boundaries
     if q.stride(-1) != 1 or q.data_ptr() % 16 or any([s % 8 or s == 0 for s in q.stride()[:-1]]):
-        q = empty_rows(q).copy_(q)
-    key = (_lib.layout(q, k_cache, v_cache, page_table, cache_lens, new_lens, tree_mask, out), qk_scale,
-           torch.is_grad_enabled())
-    plan = _ATTENTION.get(key)
-    if plan is None:
-        a = _attention_args(q, k_cache, v_cache, page_table, cache_lens, new_lens, tree_mask, qk_scale, out)
-        with torch.cuda.device(q.device):
-            a.workspace_bytes = _lib.lib().b200k_paged_attention_workspace_bytes(ctypes.byref(a))
-        plan = _ATTENTION.put(key, a, a.workspace_bytes)
-    if (k_cache.data_ptr() | v_cache.data_ptr()) % 16:
-        raise ValueError("the caches must start on 16-byte boundaries")
-    if out is None:
-        out = empty_rows(q)
-    # made per call: calls on other streams and other captured graphs have their own
-    workspace = torch.empty(plan[1], dtype=torch.uint8, device=q.device)
-    a = _ATTENTION.args(plan)
-    a.q, a.k_cache, a.v_cache, a.out = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr()
-    a.page_table, a.cache_lens, a.workspace = page_table.data_ptr(), cache_lens.data_ptr(), workspace.data_ptr()
-    if new_lens is not None:
-        a.new_lens = new_lens.data_ptr()
-    if tree_mask is not None:
-        a.tree_mask = tree_mask.data_ptr()
-    _ATTENTION.launch(a, q.device)
-    return out
+        return paged_attention(empty_rows(q).copy_(q), k_cache, v_cache, page_table, cache_lens, new_lens=new_lens,
+                               tree_mask=tree_mask, qk_scale=qk_scale, out=out)
+    scalars = (qk_scale,)
+    with torch.cuda.device(q.device):
+        a.workspace_bytes = _lib.lib().b200k_paged_attention_workspace_bytes(ctypes.byref(a))
+    _ATTENTION.add(tensors, scalars, a,
+                   inputs=(("q", 0), ("k_cache", 1), ("v_cache", 2), ("page_table", 3), ("cache_lens", 4),
+                           ("new_lens", 5), ("tree_mask", 6), ("out", 7)),
+                   outputs=(("out", 0),) if out is None else (), workspace="workspace",
+                   returns=(0 if out is None else -8,))
+    return _ATTENTION.call(tensors, scalars)
 
 
 def _attention_args(q, k_cache, v_cache, page_table, cache_lens, new_lens, tree_mask, qk_scale, out):
@@ -222,8 +211,8 @@ def _attention_args(q, k_cache, v_cache, page_table, cache_lens, new_lens, tree_
     if not 0.0 < qk_scale < 3.0e38:
         raise ValueError("qk_scale must be positive and finite")
     for c, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-        if any(s % 8 for s in c.stride()[:3]):
-            raise ValueError(f"{name} must have strides of whole 16-byte units")
+        if c.data_ptr() % 16 or any(s % 8 for s in c.stride()[:3]):
+            raise ValueError(f"{name} must start on a 16-byte boundary with strides of whole 16-byte units")
     a = _lib.PagedAttentionArgs()
     if tree_mask is not None:
         if tree_mask.dtype != torch.bool:

@@ -119,10 +119,13 @@ def empty_rows(like: torch.Tensor) -> torch.Tensor:
 
 def aligned_table(cos, sin):
     """The tables themselves, or 16-byte aligned copies of a common layout."""
-    if cos is None or sin is None or ((cos.data_ptr() | sin.data_ptr()) % 16 == 0 and cos.stride() == sin.stride()
-                                      and cos.stride(-1) == 1 and cos.stride(0) % 4 == 0):
+    if cos is None or sin is None or not cos.numel() or (
+            (cos.data_ptr() | sin.data_ptr()) % 16 == 0 and cos.stride() == sin.stride()
+            and cos.stride(-1) == 1 and cos.stride(0) % 4 == 0):
         return cos, sin
-    return tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t) for t in (cos, sin))
+    width = -(-cos.shape[1] // 4) * 4                # rows of whole 16-byte units
+    return tuple(torch.empty(t.shape[0], width, dtype=t.dtype, device=t.device)[:, :t.shape[1]].copy_(t)
+                 for t in (cos, sin))
 
 
 _FORWARD = _lib.LayoutPlans("b200k_qk_norm_rope", _lib.QkNormRopeArgs)
@@ -130,9 +133,10 @@ _BACKWARD = _lib.LayoutPlans("b200k_qk_norm_rope_backward", _lib.QkNormRopeArgs)
 
 
 def _fill(a, q, k, q_out, k_out, q_weight, k_weight, cos, sin, positions, eps, interleaved):
-    """Every field of a checked call but its pointers."""
+    """Checks the rest of a call and fills in every field but its pointers; the tables to call with."""
     batch, heads, tokens, dim = q.shape
     rotary = check_table(cos, sin, dim, q.device)
+    cos, sin = aligned_table(cos, sin)
     weight_dtype = check_weights(dim, q.dtype, q.device, q_weight, k_weight)
     a.table_rows, a.table_stride = cos.shape[0], cos.stride(0)
     a.position_stride_b, a.position_stride_t, a.positions_are_int64 = check_positions(
@@ -144,17 +148,7 @@ def _fill(a, q, k, q_out, k_out, q_weight, k_weight, cos, sin, positions, eps, i
     a.ko_stride_b, a.ko_stride_h, a.ko_stride_t, _ = k_out.stride()
     a.head_dim, a.rotary_dim, a.interleaved = dim, rotary, 1 if interleaved else 0
     a.dtype, a.weight_dtype, a.eps = _lib.dtype_enum(q.dtype), _lib.dtype_enum(weight_dtype), eps
-
-
-def _point(a, q, k, q_out, k_out, q_weight, k_weight, cos, sin, positions):
-    a.q, a.k, a.q_out, a.k_out = q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr()
-    a.cos, a.sin = cos.data_ptr(), sin.data_ptr()
-    if q_weight is not None:
-        a.q_weight = q_weight.data_ptr()
-    if k_weight is not None:
-        a.k_weight = k_weight.data_ptr()
-    if positions is not None:
-        a.positions = positions.data_ptr()
+    return cos, sin
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor,
@@ -174,28 +168,32 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor,
     Pairs are (i, i + rotary_dim / 2), or neighbours with ``interleaved``.  ``q_out`` / ``k_out``
     may be q / k themselves.  A position outside the table gives NaN rows, and
     ``raise_on_device_error()`` names it."""
-    q, k = rows_view(q), rows_view(k)
-    cos, sin = aligned_table(cos, sin)
-    key = (_lib.layout(q, k, q_weight, k_weight, cos, sin, positions, q_out, k_out), eps, interleaved,
-           torch.is_grad_enabled())
-    plan = _FORWARD.get(key)
-    qo, ko = q_out, k_out
-    if plan is None:
-        _check_rows(q, k)
-        check_no_grad("qk_norm_rope", " and take gradients from qk_norm_rope_backward", q, k, q_weight, k_weight)
-        qo = empty_rows(q) if q_out is None else check_out(q_out, q, "q_out")
-        ko = empty_rows(k) if k_out is None else check_out(k_out, k, "k_out")
-        a = _lib.QkNormRopeArgs()
-        _fill(a, q, k, qo, ko, q_weight, k_weight, cos, sin, positions, eps, interleaved)
-        plan = _FORWARD.put(key, a)
-    if qo is None:
-        qo = empty_rows(q)
-    if ko is None:
-        ko = empty_rows(k)
-    a = _FORWARD.args(plan)
-    _point(a, q, k, qo, ko, q_weight, k_weight, cos, sin, positions)
-    _FORWARD.launch(a, q.device)
-    return qo, ko
+    tensors, scalars = (q, k, q_weight, k_weight, cos, sin, positions, q_out, k_out), (eps, interleaved)
+    done = _FORWARD.call(tensors, scalars)
+    if done is not NotImplemented:
+        return done
+    _check_rows(q, k)
+    check_no_grad("qk_norm_rope", " and take gradients from qk_norm_rope_backward", q, k, q_weight, k_weight)
+    if q_out is not None:
+        check_out(q_out, q, "q_out")
+    if k_out is not None:
+        check_out(k_out, k, "k_out")
+    a = _lib.QkNormRopeArgs()
+    rows = rows_view(q), rows_view(k)
+    tables = _fill(a, *rows, empty_rows(q) if q_out is None else q_out, empty_rows(k) if k_out is None else k_out,
+                   q_weight, k_weight, cos, sin, positions, eps, interleaved)
+    if rows[0] is not q or rows[1] is not k or tables[0] is not cos:      # the call on copies of them
+        return qk_norm_rope(*rows, q_weight, k_weight, *tables, positions, eps=float(eps),
+                            interleaved=bool(interleaved), q_out=q_out, k_out=k_out)
+    scalars = float(eps), bool(interleaved)
+    outputs = [f for f in (("q_out", 0) if q_out is None else None, ("k_out", 1) if k_out is None else None) if f]
+    numbers = iter(range(2))
+    _FORWARD.add(tensors, scalars, a,
+                 inputs=(("q", 0), ("k", 1), ("q_weight", 2), ("k_weight", 3), ("cos", 4), ("sin", 5),
+                         ("positions", 6), ("q_out", 7), ("k_out", 8)),
+                 outputs=outputs,
+                 returns=(next(numbers) if q_out is None else -8, next(numbers) if k_out is None else -9))
+    return _FORWARD.call(tensors, scalars)
 
 
 def qk_norm_rope_backward(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
@@ -207,38 +205,35 @@ def qk_norm_rope_backward(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k
     qk_norm_rope's outputs and its inputs (in-place outputs lose them).  The weights' gradients
     are summed in fp32 over all rows in a fixed order and rounded to the weights' dtype; None
     for a weight of None."""
-    q, k, dq, dk = rows_view(q), rows_view(k), rows_view(dq), rows_view(dk)
-    cos, sin = aligned_table(cos, sin)
-    key = (_lib.layout(dq, dk, q, k, q_weight, k_weight, cos, sin, positions), eps, interleaved,
-           torch.is_grad_enabled())
-    plan = _BACKWARD.get(key)
-    if plan is None:
-        _check_rows(q, k)
-        check_no_grad("qk_norm_rope_backward", "", dq, dk, q, k, q_weight, k_weight)
-        for g, x, name in ((dq, q, "dq"), (dk, k, "dk")):
-            if g.shape != x.shape or g.dtype != x.dtype or g.device != x.device:
-                raise ValueError(f"{name} must have the shape, dtype and device of {name[1]}")
-        a = _lib.QkNormRopeArgs()
-        _fill(a, q, k, empty_rows(q), empty_rows(k), q_weight, k_weight, cos, sin, positions, eps, interleaved)
-        a.dq_stride_b, a.dq_stride_h, a.dq_stride_t, _ = dq.stride()
-        a.dk_stride_b, a.dk_stride_h, a.dk_stride_t, _ = dk.stride()
-        if q_weight is not None or k_weight is not None:
-            with torch.cuda.device(q.device):
-                a.workspace_bytes = _lib.lib().b200k_qk_norm_rope_backward_workspace_bytes(ctypes.byref(a))
-        plan = _BACKWARD.put(key, a, a.workspace_bytes)
-    q_in, k_in = empty_rows(q), empty_rows(k)
-    a = _BACKWARD.args(plan)
-    _point(a, q, k, q_in, k_in, q_weight, k_weight, cos, sin, positions)
-    a.dq_out, a.dk_out = dq.data_ptr(), dk.data_ptr()
-    dqw = dkw = workspace = None
-    if q_weight is not None:
-        dqw = torch.empty_like(q_weight)
-        a.dq_weight = dqw.data_ptr()
-    if k_weight is not None:
-        dkw = torch.empty_like(k_weight)
-        a.dk_weight = dkw.data_ptr()
-    if plan[1]:
-        workspace = torch.empty(plan[1], dtype=torch.uint8, device=q.device)
-        a.workspace = workspace.data_ptr()
-    _BACKWARD.launch(a, q.device)
-    return q_in, k_in, dqw, dkw
+    tensors, scalars = (dq, dk, q, k, q_weight, k_weight, cos, sin, positions), (eps, interleaved)
+    done = _BACKWARD.call(tensors, scalars)
+    if done is not NotImplemented:
+        return done
+    _check_rows(q, k)
+    check_no_grad("qk_norm_rope_backward", "", dq, dk, q, k, q_weight, k_weight)
+    for g, x, name in ((dq, q, "dq"), (dk, k, "dk")):
+        if g.shape != x.shape or g.dtype != x.dtype or g.device != x.device:
+            raise ValueError(f"{name} must have the shape, dtype and device of {name[1]}")
+    a = _lib.QkNormRopeArgs()
+    rows = tuple(rows_view(t) for t in (dq, dk, q, k))
+    tables = _fill(a, rows[2], rows[3], empty_rows(q), empty_rows(k), q_weight, k_weight, cos, sin, positions, eps,
+                   interleaved)
+    if any(r is not t for r, t in zip(rows, tensors)) or tables[0] is not cos:      # the call on copies of them
+        return qk_norm_rope_backward(*rows, q_weight, k_weight, *tables, positions, eps=float(eps),
+                                     interleaved=bool(interleaved))
+    scalars = float(eps), bool(interleaved)
+    a.dq_stride_b, a.dq_stride_h, a.dq_stride_t, _ = dq.stride()
+    a.dk_stride_b, a.dk_stride_h, a.dk_stride_t, _ = dk.stride()
+    if q_weight is not None or k_weight is not None:
+        with torch.cuda.device(q.device):
+            a.workspace_bytes = _lib.lib().b200k_qk_norm_rope_backward_workspace_bytes(ctypes.byref(a))
+    outputs, returns = [("q_out", 2), ("k_out", 3)], [0, 1]
+    for field, i in (("dq_weight", 4), ("dk_weight", 5)):
+        returns.append(None if tensors[i] is None else len(outputs))
+        if tensors[i] is not None:
+            outputs.append((field, i))
+    _BACKWARD.add(tensors, scalars, a,
+                  inputs=(("dq_out", 0), ("dk_out", 1), ("q", 2), ("k", 3), ("q_weight", 4), ("k_weight", 5),
+                          ("cos", 6), ("sin", 7), ("positions", 8)),
+                  outputs=outputs, workspace="workspace", returns=returns)
+    return _BACKWARD.call(tensors, scalars)

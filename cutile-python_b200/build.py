@@ -1,4 +1,5 @@
-"""Builds libb200k.so (sm_100a only) from csrc/*.cu with nvcc, in-tree.
+"""Builds libb200k.so (sm_100a only) from csrc/*.cu with nvcc, and the host module _plans.so from
+csrc/launch_plans.cpp, in-tree.
 
 Usage:  python cutile-python_b200/build.py [--force] [--verbose]
 
@@ -11,15 +12,19 @@ from __future__ import annotations
 
 import argparse
 import concurrent.futures
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ_DIR = os.path.join(HERE, "build")
 LIB_PATH = os.path.join(HERE, "b200k", "libb200k.so")
+PLANS_SRC = os.path.join(CSRC, "launch_plans.cpp")
+PLANS_PATH = os.path.join(HERE, "b200k", "_plans.so")
 
 NVCC_FLAGS = [
     "-std=c++17", "-O3", "-lineinfo",
@@ -53,12 +58,25 @@ def _stale(target: str, deps: list[str]) -> bool:
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def _plans_command(nvcc: str) -> list[str]:
+    """The host module: CPython and torch headers, against the libraries `import torch` loads."""
+    torch = importlib.util.find_spec("torch").submodule_search_locations[0]
+    include = os.path.join(torch, "include")
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(nvcc)))
+    return [shutil.which("g++") or "g++", "-std=c++17", "-O2", "-fPIC", "-shared", PLANS_SRC, "-o", PLANS_PATH,
+            "-I", include, "-I", os.path.join(include, "torch", "csrc", "api", "include"),
+            "-I", os.path.join(cuda, "include"), "-I", sysconfig.get_paths()["include"],
+            "-L", os.path.join(torch, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(OBJ_DIR, exist_ok=True)
     nvcc = _nvcc()
     hdrs = _headers()
     jobs = []
     objs = []
+    if force or _stale(PLANS_PATH, [PLANS_SRC]):
+        jobs.append(_plans_command(nvcc))
     for src in _sources():
         obj = os.path.join(OBJ_DIR, os.path.basename(src)[:-3] + ".o")
         objs.append(obj)
@@ -78,7 +96,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
                 if verbose or r.returncode != 0:
                     sys.stderr.write(" ".join(cmd) + "\n" + r.stdout + r.stderr)
                 if r.returncode != 0:
-                    raise RuntimeError(f"nvcc failed on {cmd[-3]}")
+                    raise RuntimeError(f"compiling failed: {' '.join(cmd)}")
     if jobs or force or _stale(LIB_PATH, objs):
         cmd = [nvcc, "-shared", "-o", LIB_PATH, *objs, "-cudart", "static"]
         r = subprocess.run(cmd, capture_output=True, text=True)

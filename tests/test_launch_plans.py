@@ -1,0 +1,95 @@
+"""The host module that remembers checked calls by the layouts of their tensors: what makes a new
+plan and what does not, and that calls share nothing but plans."""
+import threading
+
+import pytest
+import torch
+
+import b200k
+from b200k import _lib, rope
+
+
+def test_calls_that_cannot_have_a_plan_are_left_to_the_wrapper():
+    plans = _lib.LayoutPlans("b200k_qk_norm_rope", _lib.QkNormRopeArgs)
+    cpu = torch.zeros(2, 2)
+    assert plans.call((cpu,), ()) is NotImplemented            # not on a GPU
+    assert plans.call((None,), ("text",)) is NotImplemented    # a scalar that no kernel takes
+    assert plans.call(([],), ()) is NotImplemented
+    assert plans.native.size() == 0
+    with pytest.raises(TypeError):
+        plans.native.call((cpu,))
+    with pytest.raises(ValueError, match="not a plan"):
+        plans.native.add((cpu,), (), b"x" * 16, (), (), -1, 0, ())
+    with pytest.raises(ValueError, match="not a plan"):        # a pointer behind the struct's end
+        plans.native.add((None,), (), b"x" * 16, (), (), 12, 8, ())
+
+
+def _inputs(b=2, t=5, dtype=torch.bfloat16):
+    q, k = torch.randn(b, 4, t, 64, device="cuda").to(dtype), torch.randn(b, 2, t, 64, device="cuda").to(dtype)
+    w = torch.ones(64, device="cuda", dtype=dtype)
+    return (q, k, w, w, *b200k.rope_table(32, 64, device="cuda"))
+
+
+@pytest.mark.gpu
+def test_one_plan_per_layout(device_ok):
+    args = _inputs()
+    b200k.qk_norm_rope(*args)
+    size = rope._FORWARD.native.size()
+    for _ in range(3):                                          # other addresses and values
+        again = _inputs()
+        want = b200k.qk_norm_rope(*again)
+        got = b200k.qk_norm_rope(*[x.clone() for x in again])
+        assert all(torch.equal(g, w) for g, w in zip(got, want))
+    assert rope._FORWARD.native.size() == size
+    b200k.qk_norm_rope(*_inputs(t=6))                           # another length
+    b200k.qk_norm_rope(*args, eps=1e-3)                         # another scalar
+    b200k.qk_norm_rope(*args, interleaved=True)
+    b200k.qk_norm_rope(*args, q_out=torch.empty_like(args[0]))  # a given output
+    with torch.no_grad():
+        b200k.qk_norm_rope(*args)                               # another grad mode
+    assert rope._FORWARD.native.size() == size + 5
+    wide = torch.randn(2, 4, 5, 65, device="cuda").bfloat16()
+    for q in (wide[..., 1:], wide[..., :64]):                   # the same strides, another alignment
+        got = b200k.qk_norm_rope(q, *args[1:])[0]
+        assert torch.equal(got, b200k.qk_norm_rope(q.contiguous(), *args[1:])[0])
+
+
+@pytest.mark.gpu
+def test_a_remembered_layout_still_refuses_gradients(device_ok):
+    args = _inputs()
+    b200k.qk_norm_rope(*args)
+    with pytest.raises(ValueError, match="autograd"):
+        b200k.qk_norm_rope(args[0].clone().requires_grad_(), *args[1:])
+
+
+@pytest.mark.gpu
+def test_threads_and_streams_share_plans_only(device_ok):
+    cases = [_inputs(t=5 + i % 3) for i in range(6)]
+    want = [b200k.qk_norm_rope(*c) for c in cases]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(number):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for i in range(60):
+                c = (number + i) % len(cases)
+                got = b200k.qk_norm_rope(*cases[c])
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(g, w) for g, w in zip(got, want[c])):
+                    failed.append((number, i))
+
+    threads = [threading.Thread(target=work, args=(n,)) for n in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+
+
+@pytest.mark.gpu
+def test_the_table_is_emptied_when_full(device_ok):
+    args = _inputs(b=1, t=2)
+    for i in range(1030):
+        out = b200k.qk_norm_rope(*args, eps=1e-6 * (i + 1))
+    assert rope._FORWARD.native.size() <= 1024
+    assert torch.equal(out[0], b200k.qk_norm_rope(*args, eps=1e-6 * 1030)[0])
