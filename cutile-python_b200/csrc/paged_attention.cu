@@ -75,6 +75,7 @@ struct PagedParams {
   int row_tiles, half_tokens;          // row tiles; tokens of a 128-row half: half_tokens * group <= 128 rows
   int tile_rows;                       // rows of a tile's partial state
   int page_size, max_pages, box_rows;
+  int page_shift;                      // log2 of the page size, -1 where it is no power of two
   int ctas;
   int o_vec;                           // rows of out on 16-byte boundaries
   int zero_padding;
@@ -139,14 +140,10 @@ struct Run {
   SeqInfo seq;
   int b, head, row_tile, first, last;  // key tiles [first, last)
 };
-__device__ __forceinline__ bool next_run(const PagedParams& p, Walk& w, Run& r) {
-  if (w.left <= 0) return false;
-  do {                                 // sequences without tokens have no tiles
-    if (w.b >= p.batch) return false;
-    r.seq = seq_info(p, w.b);
-  } while (r.seq.tiles == 0 && ++w.b > 0);
+// The run at the walk's place, whose sequence r.seq is, and the walk behind it.
+__device__ __forceinline__ void take_run(const PagedParams& p, Walk& w, Run& r) {
   r.b = w.b;
-  r.head = w.item / p.row_tiles;
+  r.head = p.row_tiles == 1 ? w.item : w.item / p.row_tiles;
   r.row_tile = w.item - r.head * p.row_tiles;
   r.first = w.tile;
   r.last = min(r.seq.tiles, w.tile + w.left);
@@ -156,23 +153,38 @@ __device__ __forceinline__ bool next_run(const PagedParams& p, Walk& w, Run& r) 
     w.item = 0;
     ++w.b;
   }
+}
+__device__ __forceinline__ bool next_run(const PagedParams& p, Walk& w, Run& r) {
+  if (w.left <= 0) return false;
+  do {                                 // sequences without tokens have no tiles
+    if (w.b >= p.batch) return false;
+    r.seq = seq_info(p, w.b);
+  } while (r.seq.tiles == 0 && ++w.b > 0);
+  take_run(p, w, r);
   return true;
 }
 
-// Where this CTA's range begins, warp-collective.
-__device__ __forceinline__ Walk walk_start(const PagedParams& p, int lane) {
+// This CTA's range and its first run, warp-collective; false where it has none.  Up to 32 sequences
+// their lengths are read once (every further trip to the L2 costs 700 cycles before the first copy).
+__device__ __forceinline__ bool first_run(const PagedParams& p, int lane, Walk& w, Run& r) {
   const int per_seq = p.heads_kv * p.row_tiles;
-  const Ranges ranges(tiles_before(p, p.batch, lane) * per_seq, p.ctas);
+  SeqInfo seq = {0, 0, 0, 0};
+  if (lane < p.batch) seq = seq_info(p, lane);
+  int all = seq.tiles;
+#pragma unroll 1
+  for (int b = lane + 32; b < p.batch; b += 32) all += seq_info(p, b).tiles;
+  const Ranges ranges(warp_sum(all) * per_seq, p.ctas);
   const int begin = ranges.begin(blockIdx.x);
-  Walk w;
   w.left = ranges.begin(blockIdx.x + 1) - begin;
-  w.b = w.item = w.tile = 0;
+  if (w.left <= 0) return false;
   int before = 0;
 #pragma unroll 1
-  for (int b0 = 0; b0 < p.batch && w.left > 0; b0 += 32) {
-    const int b = b0 + lane;
-    const int tiles = b < p.batch ? seq_info(p, b).tiles : 0;
-    const int mine = tiles * per_seq;
+  for (int b0 = 0; b0 < p.batch; b0 += 32) {
+    if (b0 > 0) {
+      seq = {0, 0, 0, 0};
+      if (b0 + lane < p.batch) seq = seq_info(p, b0 + lane);
+    }
+    const int mine = seq.tiles * per_seq;
     int upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -182,16 +194,20 @@ __device__ __forceinline__ Walk walk_start(const PagedParams& p, int lane) {
     const uint32_t here = __ballot_sync(0xffffffffu, begin >= before + upto - mine && begin < before + upto);
     if (here != 0) {
       const int from = __ffs(here) - 1;
+      r.seq.have = __shfl_sync(0xffffffffu, seq.have, from);
+      r.seq.fresh = __shfl_sync(0xffffffffu, seq.fresh, from);
+      r.seq.len = __shfl_sync(0xffffffffu, seq.len, from);
+      r.seq.tiles = __shfl_sync(0xffffffffu, seq.tiles, from);
       const int in_seq = begin - before - __shfl_sync(0xffffffffu, upto - mine, from);
-      const int its = __shfl_sync(0xffffffffu, tiles, from);
       w.b = b0 + from;
-      w.item = in_seq / its;
-      w.tile = in_seq - w.item * its;
-      break;
+      w.item = in_seq / r.seq.tiles;
+      w.tile = in_seq - w.item * r.seq.tiles;
+      take_run(p, w, r);
+      return true;
     }
     before += __shfl_sync(0xffffffffu, upto, 31);
   }
-  return w;
+  return false;
 }
 
 // A softmax warp's walk and run, in shared memory: what a run needs at its two ends only would
@@ -355,16 +371,16 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   pdl_wait();
   // where this CTA begins, and its first pages: every warp finds its own, without a wait for
   // another's
-  Walk walk = walk_start(p, lane);
+  Walk walk;
   Run run;
-  bool have_run = next_run(p, walk, run);
+  bool have_run = first_run(p, lane, walk, run);
   // the K and V producers' lane i looks up the i-th run of slots of a tile, all of one page
   const int boxes_per_tile = kPaBN / p.box_rows;
   auto find = [&](int j, int& page, int& slot) {
     const int key = j * kPaBN + lane * p.box_rows;
     page = slot = 0;
     if (lane < boxes_per_tile && key < run.seq.len) {
-      const int entry = key / p.page_size;
+      const int entry = p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size;
       slot = key - entry * p.page_size;
       page = p.page_table[run.b * p.page_table_stride + entry];
     }
@@ -697,16 +713,18 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
             tmem_ld_wait();
 #pragma unroll
             for (int k = 0; k < 64; ++k) s[k] = __uint_as_float(y[k]);
-            if (edge) {
-              const uint32_t lo = half == 0 ? sees[0] : sees[2], hi = half == 0 ? sees[1] : sees[3];
+            const uint32_t lo = half == 0 ? sees[0] : sees[2], hi = half == 0 ? sees[1] : sees[3];
+            if (edge && !__all_sync(0xffffffffu, (lo & hi) == 0xffffffffu)) {
 #pragma unroll
               for (int k = 0; k < 64; ++k)
                 if ((((k < 32 ? lo : hi) >> (k % 32)) & 1u) == 0u) s[k] = -INFINITY;
             }
           };
+          // halves behind the last key that any row of the warp sees are left out
+          const int halves = edge && !__any_sync(0xffffffffu, (sees[2] | sees[3]) != 0u) ? 1 : 2;
           float mx = -INFINITY;
 #pragma unroll 1
-          for (int half = 0; half < 2; ++half) {
+          for (int half = 0; half < halves; ++half) {
             float s[64];
             load_scores(half, s);
             float m4[4];
@@ -746,9 +764,10 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           float2 sum2[4] = {};
 #pragma unroll 1
           for (int c = 0; c < 2; ++c) {
+            uint32_t pk[32];
+            if (c < halves) {
             float s[64];
             load_scores(c, s);                            // P of the first half lies over scores already used
-            uint32_t pk[32];
 #pragma unroll
             for (int k = 0; k < 32; ++k) {
               const float2 y = __ffma2_rn(make_float2(s[2 * k], s[2 * k + 1]), scale2, negm2);
@@ -759,6 +778,10 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
               sum2[k & 3] = __fadd2_rn(sum2[k & 3], e);
               // P is rounded to the input type: it is the tensor cores' operand
               pk[k] = BF16 ? pack_bf16x2(e.x, e.y) : pack_f16x2(e.x, e.y);
+            }
+            } else {
+#pragma unroll
+              for (int k = 0; k < 32; ++k) pk[k] = 0u;
             }
             tmem_st_32x32b_x32(tmem_s + c * 32, pk);
             if (c == 0) {                                 // the first 64 keys are enough for half of P V
@@ -1137,6 +1160,9 @@ extern "C" int b200k_paged_attention(const b200k_paged_attention_args* a, b200k_
   // lies in one page and starts on a whole eight-row swizzle atom of the tile
   p.box_rows = 8;
   while (p.box_rows < kPaBN && a->page_size % (p.box_rows * 2) == 0) p.box_rows *= 2;
+  p.page_shift = -1;
+  for (int i = 3; i < 30; ++i)
+    if (a->page_size == 1 << i) p.page_shift = i;
   p.ctas = static_cast<int>(pick_ctas(a, sms));
   const auto vec = [](const void* base, int64_t sb, int64_t sh, int64_t st) {
     return (reinterpret_cast<uintptr_t>(base) & 15) == 0 && sb % 8 == 0 && sh % 8 == 0 && st % 8 == 0;
