@@ -18,10 +18,10 @@
 //
 // One CTA per SM, two softmax groups A and B whose work interleaves on the tensor cores, so that
 // one's softmax overlaps the other's matrix products:
-//   split  (at most 128 rows)   A and B take a run's key tiles in turn, each with its own running
-//                               maximum, sum and O; the group that began (A and B by turns)
-//                               joins the two states at the run's end, while the other already
-//                               works on the next run's first tile
+//   split  (at most 128 rows)   A and B take the CTA's key tiles in turn, each with its own running
+//                               maximum, sum and O; the group of a run's last tile joins the two
+//                               states at its end, while the other already works on the next
+//                               run's first tile, whose S was issued before (Q has two places)
 //   pair   (more rows)          A and B are two row tiles of 128, every key tile serves both
 //
 //   warps 0, 10  TMA producers of K and of V: a box per run of slots inside a page, into rings
@@ -50,11 +50,11 @@ constexpr int kPaThreads = 384;        // K warp, MMA warp, two softmax groups o
 constexpr int kPaTmemCols = 512;       // S_A, S_B, O_A, O_B; P over S
 constexpr int kPaJoinThreads = 128;
 
-// Rings of K and V tiles in what Q leaves of 224 KB.  V tiles wait for the softmax, so V gets
-// the odd one.
+// Rings of K and V tiles in what Q's two tiles leave of 224 KB.  V tiles wait for the softmax, so V
+// gets the odd one.
 template <int D, bool PAIR> struct Rings {
   static constexpr int kTile = 128 * D * 2;
-  static constexpr int kQ = PAIR ? 2 : 1;
+  static constexpr int kQ = 2;                        // two runs' rows (split), two halves (pair)
   static constexpr int kTiles = 224 * 1024 / kTile - kQ;
   static constexpr int kK = kTiles / 2, kV = kTiles - kK;
   static constexpr int kSmem = (kQ + kTiles) * kTile + 1472 + 8 * 2 * 13 * 4;
@@ -327,7 +327,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   const uint32_t v_smem = k_smem + R::kK * R::kTile;
   uint8_t* tail = smem + (R::kQ + R::kTiles) * R::kTile;
   const uint32_t bar0 = smem_u32(tail);
-  enum { Q_FULL = 0, Q_EMPTY, S_FULL, P_HALF = S_FULL + 2, P_FULL = P_HALF + 2, PV_DONE = P_FULL + 2,
+  enum { Q_FULL = 0, Q_EMPTY = Q_FULL + 2, S_FULL = Q_EMPTY + 2, P_HALF = S_FULL + 2, P_FULL = P_HALF + 2, PV_DONE = P_FULL + 2,
          RUN_DONE = PV_DONE + 2, O_READ, K_FULL, K_EMPTY = K_FULL + R::kK, V_FULL = K_EMPTY + R::kK,
          V_EMPTY = V_FULL + R::kV, NUM_BARS = V_EMPTY + R::kV };
   static_assert(8 * NUM_BARS <= 384, "barriers fit their place");
@@ -399,8 +399,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   constexpr uint32_t kFmt = BF16 ? kFmtBF16 : kFmtF16;
 
   if (warp == 11) {
-    // the Q producer: a run's rows once the last S of the run before has read its own, and a
-    // prefetch of the next run's into the L2 (cold, they took 10 us of a full memory system)
+    // the Q producer: a run's rows once their place's last S is through.  Pair has one place: the
+    // next run's rows are prefetched into the L2 (cold, they took 10 us of a full memory system)
     Run next;
     bool ok = true;
     const bool elected = elect_one();
@@ -408,22 +408,24 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     const uint32_t bytes = static_cast<uint32_t>(p.half_tokens * p.group) * 128u * kBoxes * kHalves;
     int runs = 0;
     for (; have_run && ok; ++runs) {
-      if (runs > 0 && !mbar_wait(bar(Q_EMPTY), (runs - 1) & 1, abort_flag)) {
+      // split: run r in place r % 2, once run r - 2 is through
+      const int place = PAIR ? 0 : runs & 1, fill = PAIR ? runs : runs >> 1;
+      if (fill > 0 && !mbar_wait(bar(Q_EMPTY + place), (fill - 1) & 1, abort_flag)) {
         report_status(p.status, 98, runs);
         *abort_flag = 1;
         ok = false;
         break;
       }
-      if (elected) mbar_arrive_expect_tx(bar(Q_FULL), bytes);
+      if (elected) mbar_arrive_expect_tx(bar(Q_FULL + place), bytes);
       const bool more = next_run(p, walk, next);
 #pragma unroll
       for (int x = 0; x < kHalves; ++x) {
 #pragma unroll
         for (int h = 0; h < kBoxes; ++h) {
           if (elected) {
-            tma_load_4d(q_smem + x * R::kTile + h * kBoxBytes, &tmap_q, bar(Q_FULL), h * 64, run.head * p.group,
-                        (run.row_tile * kHalves + x) * p.half_tokens, run.b);
-            if (more)
+            tma_load_4d(q_smem + (place + x) * R::kTile + h * kBoxBytes, &tmap_q, bar(Q_FULL + place), h * 64,
+                        run.head * p.group, (run.row_tile * kHalves + x) * p.half_tokens, run.b);
+            if (PAIR && more)
               tma_prefetch_4d(&tmap_q, h * 64, next.head * p.group, (next.row_tile * kHalves + x) * p.half_tokens, next.b);
           }
         }
@@ -432,7 +434,9 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       run = next;
       have_run = more;
     }
-    if (runs > 0) mbar_wait(bar(Q_FULL), (runs - 1) & 1, abort_flag);   // nothing in flight when the CTA leaves
+    // nothing in flight when the CTA leaves
+    for (int i = 0; i < (PAIR ? 1 : 2) && i < runs; ++i)
+      mbar_wait(bar(Q_FULL + i), (PAIR ? runs - 1 : (runs - 1 - i) >> 1) & 1, abort_flag);
     __syncwarp();
   } else if (warp == 0 || warp == 10) {
     const bool is_v = warp != 0;
@@ -499,11 +503,11 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       ok = false;
     };
     // S_x = Q_x K^T: both operands K-major, 16 elements (32 bytes) of the head dim per MMA
-    auto issue_s = [&](int x) {
+    auto issue_s = [&](int x, int q_place) {
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
         const uint32_t off = (kk / 4) * kBoxBytes;
-        const uint64_t qd = make_smem_desc(q_smem + (PAIR ? x * R::kTile : 0) + off, 16, 1024, kSwizzle128B) + 2 * (kk % 4);
+        const uint64_t qd = make_smem_desc(q_smem + q_place * R::kTile + off, 16, 1024, kSwizzle128B) + 2 * (kk % 4);
         const uint64_t kd = make_smem_desc(k_smem + ks * R::kTile + off, 16, 1024, kSwizzle128B) + 2 * (kk % 4);
         if (elected) umma<kKindF16>(tmem_base + x * 128, qd, kd, idesc_qk, kk > 0 ? 1u : 0u);
       }
@@ -537,55 +541,75 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       if (elected) tc_commit(bar(V_EMPTY + vs));
       if (++vs == R::kV) { vs = 0; vp ^= 1; }
     };
-    for (int runs = 0; ok && have_run; ++runs, have_run = next_run(p, walk, run)) {
-      const int n = run.last - run.first;
-      if (!mbar_wait(bar(Q_FULL), runs & 1, abort_flag)) {
-        give_up(92, runs);
-        break;
-      }
-      // the next S that fits: `ahead` tiles before its P V
-      auto next_s = [&](int i) {
-        if (!mbar_wait(bar(K_FULL + ks), kp, abort_flag)) {
-          give_up(93, i);
-          return;
-        }
-        tc_fence_after_sync();
-        if (PAIR) {
-          issue_s(0);
-          issue_s(1);
-        } else {
-          issue_s((i + runs) & 1);
-        }
-        free_k();
-        if (i == n - 1 && elected) tc_commit(bar(Q_EMPTY));
-      };
-      next_s(0);
-      if (!PAIR && n > 1 && ok) next_s(1);
-      for (int i = 0; i < n && ok; ++i) {
-        if (!mbar_wait(bar(V_FULL + vs), vp, abort_flag)) {
-          give_up(95, i);
+    if constexpr (PAIR) {
+      for (int runs = 0; ok && have_run; ++runs, have_run = next_run(p, walk, run)) {
+        const int n = run.last - run.first;
+        if (!mbar_wait(bar(Q_FULL), runs & 1, abort_flag) || !mbar_wait(bar(K_FULL + ks), kp, abort_flag)) {
+          give_up(92, runs);
           break;
         }
-        if (PAIR) {
+        tc_fence_after_sync();
+        issue_s(0, 0);
+        issue_s(1, 1);
+        free_k();
+        if (n == 1 && elected) tc_commit(bar(Q_EMPTY));
+        for (int i = 0; i < n && ok; ++i) {
           // P V (A, i)  S (A, i + 1)  P V (B, i)  S (B, i + 1)
           const bool more = i + 1 < n;
-          if (more && !mbar_wait(bar(K_FULL + ks), kp, abort_flag)) {
+          if (!mbar_wait(bar(V_FULL + vs), vp, abort_flag) || (more && !mbar_wait(bar(K_FULL + ks), kp, abort_flag))) {
             give_up(93, i);
             break;
           }
           tc_fence_after_sync();
           issue_pv(0, i == 0, i);
-          if (ok && more) issue_s(0);
+          if (ok && more) issue_s(0, 0);
           if (ok) issue_pv(1, i == 0, i);
-          if (ok && more) issue_s(1);
-          if (ok && more) free_k();
-          if (ok && more && i + 1 == n - 1 && elected) tc_commit(bar(Q_EMPTY));
+          if (ok && more) {
+            issue_s(1, 1);
+            free_k();
+            if (i + 1 == n - 1 && elected) tc_commit(bar(Q_EMPTY));
+          }
           if (ok) free_v();
-        } else {
-          issue_pv((i + runs) & 1, i < 2, i);
-          if (ok) free_v();
-          if (ok && i + 2 < n) next_s(i + 2);
         }
+      }
+    } else {
+      // tiles in the order of the CTA's range, group tile % 2; S two tiles ahead of P V, across runs
+      int i = 0, runs = 0, issued = 0;
+      bool first[2] = {true, true};            // the group's next P V is its first of a run
+      Run next;
+      bool have_next = false;
+      auto next_s = [&]() {
+        if (!have_run) return;
+        const int x = issued & 1, n = run.last - run.first;
+        if ((i == 0 && !mbar_wait(bar(Q_FULL + (runs & 1)), (runs >> 1) & 1, abort_flag)) ||
+            !mbar_wait(bar(K_FULL + ks), kp, abort_flag)) {
+          give_up(93, issued);
+          return;
+        }
+        tc_fence_after_sync();
+        issue_s(x, runs & 1);
+        free_k();
+        first[x] = i < 2;
+        ++issued;
+        if (i == 0) have_next = next_run(p, walk, next);   // found while nothing waits for it
+        if (++i == n) {
+          if (elected) tc_commit(bar(Q_EMPTY + (runs & 1)));
+          run = next;
+          have_run = have_next;
+          i = 0;
+          ++runs;
+        }
+      };
+      next_s();
+      if (ok) next_s();
+      for (int done = 0; ok && done < issued; ++done) {
+        if (!mbar_wait(bar(V_FULL + vs), vp, abort_flag)) {
+          give_up(95, done);
+          break;
+        }
+        issue_pv(done & 1, first[done & 1], done);
+        if (ok) free_v();
+        if (ok) next_s();
       }
     }
     __syncwarp();
@@ -633,19 +657,20 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         first_tile = run.first;
         have = run.seq.have;
       }
-      const bool lead = PAIR || ((x + runs) & 1) == 0;   // split: takes the first tile and finishes the run
+      // split: the first of the run's tiles that is this group's; the group of the last one finishes
+      const int i0 = PAIR ? 0 : (tile0 ^ x) & 1, di = PAIR ? 1 : 2;
+      const bool finish = PAIR || ((tile0 + n - 1 - x) & 1) == 0;
       float m_used = -INFINITY, l = 0.0f;
       // the run is this warp's no more than to its last P: what others read of it is in place
       auto leave_run = [&]() {
-        if (!lead) state_b[row] = make_float2(m_used, l);
+        if (!finish) state_b[row] = make_float2(m_used, l);
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(RUN_DONE));
       };
-      const int i0 = lead ? 0 : 1, di = PAIR ? 1 : 2;
       // the group that finished the run before has read this one's O of it: the first P V of this
       // run may begin to overwrite it
       auto await_o_read = [&](int i) {
-        if (!PAIR && lead && i == 0 && runs > 0 && !mbar_wait(bar(O_READ), (runs - 1) & 1, abort_flag)) give_up(99, runs);
+        if (!PAIR && i == 0 && runs > 0 && !mbar_wait(bar(O_READ), (runs - 1) & 1, abort_flag)) give_up(99, runs);
       };
       if (i0 >= n) leave_run();                 // no share of a single tile
       for (int i = i0; i < n; i += di) {
@@ -820,8 +845,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         if (lane == 0) save_run(words + ((runs + 1) & 1) * kRunWords, on, next);
         __syncwarp();
       }
-      other_tiles += (lead ? n : n + 1) / 2;
-      if (!lead) continue;                                // the other group finishes the run
+      other_tiles += (n + i0) / 2;
+      if (!finish) continue;                              // the other group finishes the run
       const bool edges = (first_tile + n) * kPaBN > have;
       const bool two = !PAIR && n > 1;                    // the other group has a share of it
       if (!mbar_wait(bar(PV_DONE + x), sp ^ 1, abort_flag) ||
