@@ -22,6 +22,11 @@
 //                               maximum, sum and O; the group of a run's last tile joins the two
 //                               states at its end, while the other already works on the next
 //                               run's first tile, whose S was issued before (Q has two places)
+//   quad   (at most 32 rows)    split, with the rows four times in the tile: warp q of a group takes
+//                               keys [32 q, 32 q + 32) of every tile, its P is zero elsewhere, and
+//                               its rows are a partial state of their own.  A warp's 128
+//                               exponentials, 1000 cycles of the special-function unit whether
+//                               one lane has a row or all, become 32, on four schedulers
 //   pair   (more rows)          A and B are two row tiles of 128, every key tile serves both
 //
 //   warps 0, 10  TMA producers of K and of V: a box per run of slots inside a page, into rings
@@ -47,12 +52,14 @@ namespace {
 constexpr int kPaBM = 128;             // query rows of a tile
 constexpr int kPaBN = 128;             // keys of a tile
 constexpr int kPaThreads = 384;        // K warp, MMA warp, two softmax groups of four warps, V and Q warps
+constexpr int kPaQuadRows = 16;        // rows up to which quad is taken
 constexpr int kPaTmemCols = 512;       // S_A, S_B, O_A, O_B; P over S
-constexpr int kPaJoinThreads = 128;
 
 // Rings of K and V tiles in what Q's two tiles leave of 224 KB.  V tiles wait for the softmax, so V
 // gets the odd one.
-template <int D, bool PAIR> struct Rings {
+enum Mode : int { kSplit = 0, kPair = 1, kQuad = 2 };
+
+template <int D> struct Rings {
   static constexpr int kTile = 128 * D * 2;
   static constexpr int kQ = 2;                        // two runs' rows (split), two halves (pair)
   static constexpr int kTiles = 224 * 1024 / kTile - kQ;
@@ -80,8 +87,8 @@ struct PagedParams {
   int o_vec;                           // rows of out on 16-byte boundaries
   int zero_padding;
   float scale_log2;
-  float* ws_ml;                        // (2 ctas, tile_rows, 2): row maximum and sum
-  float* ws_acc;                       // (2 ctas, D / 4, tile_rows, 4)
+  float* ws_ml;                        // (slots, tile_rows, 2): row maximum and sum
+  float* ws_acc;                       // (slots, D / 4, tile_rows, 4): two slots per CTA (quad: and one per item)
   int* status;
 };
 
@@ -278,11 +285,12 @@ __device__ __forceinline__ uint32_t visible_keys(const PagedParams& p, const Seq
 // Such values are a model's failure, but they stay with the rows that see them.
 template <int D, bool BF16>
 __device__ __forceinline__ void add_cleared_drafts(const PagedParams& p, const Run& run, int hq, int t, float* acc,
-                                                   float m, float inv_l, bool whole) {
+                                                   float m, float inv_l, bool whole, int quarter) {
   auto at = [&](int k) -> float& { return acc[static_cast<int64_t>(k / 4) * p.tile_rows * 4 + k % 4]; };
   const uint16_t* q_row = p.q + run.b * p.q_b + hq * p.q_h + t * p.q_t;
   const int end = min(run.seq.len, run.last * kPaBN);
   for (int key = max(run.seq.have, run.first * kPaBN); key < end; ++key) {
+    if (quarter >= 0 && ((key >> 5) & 3) != quarter) continue;   // quad: another warp's key
     const int draft = key - run.seq.have;
     const bool sees = p.mask != nullptr ? p.mask[run.b * p.mask_b + t * p.mask_t + draft * p.mask_j] != 0 : draft <= t;
     const int page = p.page_table[run.b * p.page_table_stride + key / p.page_size];
@@ -309,11 +317,12 @@ __device__ __forceinline__ void add_cleared_drafts(const PagedParams& p, const R
   }
 }
 
-template <int D, bool BF16, bool PAIR>
+template <int D, bool BF16, int MODE>
 __global__ void __launch_bounds__(kPaThreads, 1)
 paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
                        const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ PagedParams p) {
-  using R = Rings<D, PAIR>;
+  constexpr bool PAIR = MODE == kPair, QUAD = MODE == kQuad;
+  using R = Rings<D>;
   constexpr int kBoxes = D / 64;            // 64-element (128-byte) slices of the head dim
   constexpr int kBoxBytes = 128 * 128;
   // no room for rounding the base up: the swizzle atoms need the declared alignment
@@ -404,8 +413,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     Run next;
     bool ok = true;
     const bool elected = elect_one();
-    constexpr int kHalves = PAIR ? 2 : 1;
-    const uint32_t bytes = static_cast<uint32_t>(p.half_tokens * p.group) * 128u * kBoxes * kHalves;
+    constexpr int kHalves = PAIR ? 2 : 1, kCopies = QUAD ? 4 : 1;
+    const uint32_t bytes = static_cast<uint32_t>(p.half_tokens * p.group) * 128u * kBoxes * kHalves * kCopies;
     int runs = 0;
     for (; have_run && ok; ++runs) {
       // split: run r in place r % 2, once run r - 2 is through
@@ -423,8 +432,10 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
 #pragma unroll
         for (int h = 0; h < kBoxes; ++h) {
           if (elected) {
-            tma_load_4d(q_smem + (place + x) * R::kTile + h * kBoxBytes, &tmap_q, bar(Q_FULL + place), h * 64,
-                        run.head * p.group, (run.row_tile * kHalves + x) * p.half_tokens, run.b);
+#pragma unroll
+            for (int copy = 0; copy < kCopies; ++copy)
+              tma_load_4d(q_smem + (place + x) * R::kTile + h * kBoxBytes + copy * 32 * 128, &tmap_q, bar(Q_FULL + place),
+                          h * 64, run.head * p.group, (run.row_tile * kHalves + x) * p.half_tokens, run.b);
             if (PAIR && more)
               tma_prefetch_4d(&tmap_q, h * 64, next.head * p.group, (next.row_tile * kHalves + x) * p.half_tokens, next.b);
           }
@@ -637,9 +648,9 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     };
     auto place_in = [&](const Run& run) {
       Place q;
-      const int in_half = row / p.group;
+      const int in_tile = QUAD ? lane : row, in_half = in_tile / p.group;
       q.t = (PAIR ? run.row_tile * 2 + x : run.row_tile) * p.half_tokens + in_half;
-      q.hq = run.head * p.group + (row - in_half * p.group);
+      q.hq = run.head * p.group + (in_tile - in_half * p.group);
       q.live = in_half < p.half_tokens && q.t < run.seq.fresh;
       return q;
     };
@@ -683,12 +694,16 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           const int t = place_in(run).t;
           const int t0 = __shfl_sync(0xffffffffu, t, 0);
           const int t1 = min(__shfl_sync(0xffffffffu, t, 31), run.seq.fresh - 1);
+          if constexpr (QUAD) {
+            sees[0] = visible_keys(p, run.seq, run.b, t, t0, t1, key0 + 32 * quarter, lane);
+          } else {
 #pragma unroll 1
           for (int w = 0; w < 4; ++w) {                  // rolled: the words move up
             sees[0] = sees[1];
             sees[1] = sees[2];
             sees[2] = sees[3];
             sees[3] = visible_keys(p, run.seq, run.b, t, t0, t1, key0 + 32 * w, lane);
+          }
           }
         }
         if (!mbar_wait(bar(S_FULL + x), sp, abort_flag)) {
@@ -729,6 +744,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         };
         tc_fence_after_sync();
         if (any_live) {                                   // a warp of padding rows only keeps step
+          float sq[32];                                   // quad: the warp's 32 keys
           // S in halves of 64 scores, once for the maximum and once for the exponentials: a row of 128
           // in registers would spill, and local memory is what the L1 beside 224 KB of tiles
           // serves worst
@@ -748,6 +764,25 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           // halves behind the last key that any row of the warp sees are left out
           const int halves = edge && !__any_sync(0xffffffffu, (sees[2] | sees[3]) != 0u) ? 1 : 2;
           float mx = -INFINITY;
+          if constexpr (QUAD) {
+            uint32_t y[32];
+            tmem_ld_32x32b_x32(tmem_s + quarter * 32, y);
+            tmem_ld_wait();
+#pragma unroll
+            for (int k = 0; k < 32; ++k) sq[k] = __uint_as_float(y[k]);
+            if (edge) {
+#pragma unroll
+              for (int k = 0; k < 32; ++k)
+                if (((sees[0] >> k) & 1u) == 0u) sq[k] = -INFINITY;
+            }
+            float m2[2] = {fmax3(sq[0], sq[1], sq[2]), fmax3(sq[16], sq[17], sq[18])};
+#pragma unroll
+            for (int k = 3; k < 15; k += 2) {
+              m2[0] = fmax3(m2[0], sq[k], sq[k + 1]);
+              m2[1] = fmax3(m2[1], sq[16 + k], sq[17 + k]);
+            }
+            mx = fmaxf(fmax3(m2[0], m2[1], sq[15]), sq[31]);
+          } else {
 #pragma unroll 1
           for (int half = 0; half < halves; ++half) {
             float s[64];
@@ -761,6 +796,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
               m4[c] = fmaxf(m4[c], s[16 * c + 15]);
             }
             mx = fmaxf(mx, fmax3(m4[0], m4[1], fmaxf(m4[2], m4[3])));
+          }
           }
           const float m_new = fmaxf(m_used, mx * p.scale_log2);
           const bool grow = (m_new - m_used > kRescaleThreshold) || (m_used == -INFINITY && m_new > -INFINITY);
@@ -787,6 +823,29 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
           const float2 negm2 = make_float2(neg_m, neg_m);
           float2 sum2[4] = {};
+          if constexpr (QUAD) {
+            uint32_t pk[16], none[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              const float2 y = __ffma2_rn(make_float2(sq[2 * k], sq[2 * k + 1]), scale2, negm2);
+              const float2 e = make_float2(fast_exp2(y.x), fast_exp2(y.y));
+              sum2[k & 3] = __fadd2_rn(sum2[k & 3], e);
+              pk[k] = BF16 ? pack_bf16x2(e.x, e.y) : pack_f16x2(e.x, e.y);
+              none[k] = 0u;
+            }
+            // the other warps' keys: zero, where S lay
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              if (w == quarter) tmem_st_32x32b_x16(tmem_s + w * 16, pk);
+              else tmem_st_32x32b_x16(tmem_s + w * 16, none);
+            }
+            if (edge) clear_v();
+            await_o_read(i);
+            tmem_st_wait();
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(P_HALF + x));
+          } else {
 #pragma unroll 1
           for (int c = 0; c < 2; ++c) {
             uint32_t pk[32];
@@ -817,6 +876,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
               __syncwarp();
               if (lane == 0) mbar_arrive(bar(P_HALF + x));
             }
+          }
           }
           l += ((sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y)) + ((sum2[2].x + sum2[2].y) + (sum2[3].x + sum2[3].y));
           tmem_st_wait();
@@ -869,9 +929,12 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       }
       const Run run = saved_run(mine);
       const Place at = place_in(run);
-      const bool whole = run.first == 0 && run.last == run.seq.tiles;
-      const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (runs == 0 ? 0 : 1);
-      const int tile_row = (PAIR ? x * kPaBM : 0) + row;
+      // quad always leaves its four states, a whole item's in a slot of the item's
+      const bool all = run.first == 0 && run.last == run.seq.tiles, whole = !QUAD && all;
+      const int64_t slot = QUAD && all ? 2 * static_cast<int64_t>(p.ctas) + run.b * p.heads_kv + run.head
+                                       : 2 * static_cast<int64_t>(blockIdx.x) + (runs == 0 ? 0 : 1);
+      // quad: every quarter's rows are a state of their own
+      const int tile_row = QUAD ? quarter * (p.tile_rows / 4) + lane : (PAIR ? x * kPaBM : 0) + row;
       const float inv_l = (l > 0.0f) ? __fdividef(1.0f, l) : (l == 0.0f ? 0.0f : l);
       const bool by_hand = edges && bad_draft[runs & 1] == runs;
       const bool to_out = whole && !by_hand;
@@ -924,7 +987,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           __syncwarp();
         }
         if (by_hand && live) 
-          add_cleared_drafts<D, BF16>(p, run, at.hq, at.t, reinterpret_cast<float*>(acc), m_used, inv_l, whole);
+          add_cleared_drafts<D, BF16>(p, run, at.hq, at.t, reinterpret_cast<float*>(acc), m_used, inv_l, whole,
+                                       QUAD ? quarter : -1);
         __syncwarp();
       }
       tc_fence_before_sync();
@@ -947,16 +1011,19 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
 // Joins the partial states of items that several CTAs share, and clears padding rows.  A thread owns
 // four columns of a row (neighbouring threads neighbouring rows, as the states are stored) and
 // takes every G-th state in range order; its G partners' results meet in shared memory.
-template <int D, bool BF16, bool PAIR, int G>
-__global__ void __launch_bounds__(kPaJoinThreads * G)
+template <int D, bool BF16, int MODE, int E, int G>
+__global__ void __launch_bounds__(E * G)
 paged_attention_join_kernel(const __grid_constant__ PagedParams p) {
   const int lane = threadIdx.x & 31;
   pdl_launch_dependents();
   const int per_seq = p.heads_kv * p.row_tiles;
   const int b = blockIdx.y / per_seq, item = blockIdx.y - b * per_seq;
   const int head = item / p.row_tiles, row_tile = item - head * p.row_tiles;
-  const int element = blockIdx.x * kPaJoinThreads + threadIdx.x % kPaJoinThreads;
-  const int quad = element / p.tile_rows, row = element - quad * p.tile_rows;
+  const int element = blockIdx.x * E + threadIdx.x % E;
+  constexpr bool PAIR = MODE == kPair;
+  constexpr int kStates = MODE == kQuad ? 4 : 1;     // partial states of a row that a run leaves
+  const int out_rows = p.tile_rows / kStates;
+  const int quad = element / out_rows, row = element - quad * out_rows;
   const SeqInfo seq = seq_info(p, b);
   const Ranges ranges(tiles_before(p, p.batch, lane) * per_seq, p.ctas);
   const int first = tiles_before(p, b, lane) * per_seq + item * seq.tiles;
@@ -967,11 +1034,11 @@ paged_attention_join_kernel(const __grid_constant__ PagedParams p) {
   const bool real = mine && t < seq.fresh;
   const int c0 = seq.tiles > 0 ? ranges.owner(first) : 0, c1 = seq.tiles > 0 ? ranges.owner(first + seq.tiles - 1) : 0;
   // a row of an item that one CTA has finished is in place; a padding row is cleared on request
-  const bool store = mine && (real ? c0 != c1 || seq.tiles == 0 : p.zero_padding != 0);
+  const bool store = mine && (real ? kStates > 1 || c0 != c1 || seq.tiles == 0 : p.zero_padding != 0);
   uint16_t* dst = p.out + b * p.o_b + static_cast<int64_t>(hq) * p.o_h + t * p.o_t + quad * 4;
-  const int g = threadIdx.x / kPaJoinThreads, e = threadIdx.x % kPaJoinThreads;
-  __shared__ float2 sm_ml[G][kPaJoinThreads];
-  __shared__ float4 sm_o[G][kPaJoinThreads];
+  const int g = threadIdx.x / E, e = threadIdx.x % E;
+  __shared__ float2 sm_ml[G][E];
+  __shared__ float4 sm_o[G][E];
   if (store) asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<uint64_t>(dst)));
   // Everything below runs twice: once on whatever the workspace holds, with nothing stored, while
   // the kernel before still computes - its instructions and address translations are then at
@@ -995,16 +1062,18 @@ paged_attention_join_kernel(const __grid_constant__ PagedParams p) {
       o.w = o.w * f + a.w * h;
       m = top;
     };
-    if (c0 != c1 && real) {
+    if ((kStates > 1 || c0 != c1) && real && seq.tiles > 0) {
       const float4* acc = reinterpret_cast<const float4*>(p.ws_acc);
       const float2* ml = reinterpret_cast<const float2*>(p.ws_ml);
-      const int last = pass == 0 ? min(c1, c0 + G) : c1;
+      const int states = (c1 - c0 + 1) * kStates, last = pass == 0 ? min(states, G) : states;
 #pragma unroll 4
-      for (int c = c0 + g; c <= last; c += G) {
+      for (int k = g; k < last; k += G) {
+        const int c = c0 + k / kStates, at = (k % kStates) * out_rows + row;
         // only the first of an item's CTAs may have begun with an earlier item
-        const int64_t slot = 2 * static_cast<int64_t>(c) + (ranges.begin(c) >= first ? 0 : 1);
-        const float2 state = __ldcg(ml + slot * p.tile_rows + row);
-        take(state.x, state.y, __ldcg(acc + (slot * (D / 4) + quad) * p.tile_rows + row));
+        const int64_t slot = kStates > 1 && c0 == c1 ? 2 * static_cast<int64_t>(p.ctas) + blockIdx.y
+                                                     : 2 * static_cast<int64_t>(c) + (ranges.begin(c) >= first ? 0 : 1);
+        const float2 state = __ldcg(ml + slot * p.tile_rows + at);
+        take(state.x, state.y, __ldcg(acc + (slot * (D / 4) + quad) * p.tile_rows + at));
       }
     }
     if constexpr (G > 1) {
@@ -1038,24 +1107,33 @@ paged_attention_join_kernel(const __grid_constant__ PagedParams p) {
 int padded_dim(const b200k_paged_attention_args* a) { return a->head_dim <= 64 ? 64 : 128; }
 
 // The rows that share a key/value head, token by token, and how they are cut: one 128-row half
-// ("split"), or tiles of two halves ("pair") where there are more.  A half holds whole tokens.
+// ("split", up to 32 of them "quad"), or tiles of two halves ("pair") where there are more.  A half
+// holds whole tokens.
 struct Rows {
-  bool pair;
-  int64_t half_tokens, tiles, per_tile;
+  Mode mode;
+  int64_t half_tokens, tiles, per_tile;      // per_tile: rows of a partial state
+  int64_t slots(const b200k_paged_attention_args* a, int64_t ctas) const {   // partial states
+    return 2 * ctas + (mode == kQuad ? a->batch * a->heads_kv : 0);
+  }
 };
-Rows lay_out_rows(const b200k_paged_attention_args* a) {
+Rows lay_out_rows(const b200k_paged_attention_args* a, int sms) {
   const int64_t group = a->heads_q / a->heads_kv;
   Rows r;
-  r.pair = a->tokens * group > kPaBM;
-  r.half_tokens = r.pair ? kPaBM / group : a->tokens;
-  r.tiles = r.pair ? ceil_div(a->tokens, 2 * r.half_tokens) : 1;
-  r.per_tile = r.pair ? 2 * kPaBM : a->tokens * group;
+  const int64_t rows = a->tokens * group;
+  // quad shortens a tile's softmax and pays with four states per item: it gains where CTAs walk
+  // several short items (64 sequences of up to 500 keys, 8 heads: 49 -> 38 us; of 1000 63 -> 47; 64
+  // items of 2000 keys 17.2 -> 16.5), not where many CTAs share one (32 items 13.7 -> 14.6; 8 items
+  // 17.9 -> 18.5), nor with more rows to write (16 rows 67 -> 61, 32 rows 28.9 -> 32.1)
+  r.mode = rows <= kPaQuadRows && 3 * a->batch * a->heads_kv >= sms ? kQuad : (rows <= kPaBM ? kSplit : kPair);
+  r.half_tokens = r.mode == kPair ? kPaBM / group : a->tokens;
+  r.tiles = r.mode == kPair ? ceil_div(a->tokens, 2 * r.half_tokens) : 1;
+  r.per_tile = r.mode == kPair ? 2 * kPaBM : (r.mode == kQuad ? 4 * rows : rows);
   return r;
 }
 
 // CTAs of a call: one per SM, fewer where there cannot be as many key tiles.
 int64_t pick_ctas(const b200k_paged_attention_args* a, int sms) {
-  const int64_t items = a->batch * a->heads_kv * lay_out_rows(a).tiles;
+  const int64_t items = a->batch * a->heads_kv * lay_out_rows(a, sms).tiles;
   const int64_t most = items * ceil_div(static_cast<int64_t>(a->max_pages) * a->page_size, kPaBN);
   const int64_t n = most < sms ? most : sms;
   return n < 1 ? 1 : n;
@@ -1079,15 +1157,15 @@ int check_args(const b200k_paged_attention_args* a) {
   if (a->tokens * a->heads_q > limit || static_cast<int64_t>(a->max_pages) * a->page_size > limit ||
       a->num_pages >= limit || a->batch > limit || a->heads_kv > limit ||
       a->batch * a->heads_kv > 65535 ||
-      a->batch * a->heads_kv * lay_out_rows(a).tiles * ceil_div(static_cast<int64_t>(a->max_pages) * a->page_size, kPaBN) > limit)
+      a->batch * a->heads_kv * lay_out_rows(a, 1).tiles * ceil_div(static_cast<int64_t>(a->max_pages) * a->page_size, kPaBN) > limit)
     return fail(B200K_UNSUPPORTED, "more rows, pages or sequences than the kernel counts");
   return B200K_OK;
 }
 
-template <int D, bool BF16, bool PAIR>
+template <int D, bool BF16, int MODE>
 int launch_paged_as(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const PagedParams& p, int64_t items, cudaStream_t stream) {
-  constexpr int kSmem = Rings<D, PAIR>::kSmem;
-  auto kernel = paged_attention_kernel<D, BF16, PAIR>;
+  constexpr int kSmem = Rings<D>::kSmem;
+  auto kernel = paged_attention_kernel<D, BF16, MODE>;
   static bool configured[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -1101,24 +1179,33 @@ int launch_paged_as(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensor
   // end of the kernel before it, and its end the set-up of the joining kernel
   cudaError_t e = launch_after_predecessor(kernel, dim3(p.ctas), dim3(kPaThreads), kSmem, stream, tq, tk, tv, p);
   if (e != cudaSuccess) return fail(B200K_CUDA_ERROR, "paged attention launch: %s", cudaGetErrorString(e));
-  const dim3 grid(static_cast<unsigned>(ceil_div(static_cast<int64_t>(p.tile_rows) * (D / 4), kPaJoinThreads)),
-                  static_cast<unsigned>(items));
-  // few blocks mean few items, each shared by many CTAs: four threads to an output then (a token of
-  // 32 heads and 1024 keys 17.1 us with one thread, 15.0 with four, 17.3 with eight; 256 items are
-  // the same with all three)
+  // Many outputs: a thread for each.  Few mean few items, each shared by many CTAs: several threads
+  // to an output, in blocks of a warp of outputs (a token of 32 heads and 1024 keys 13.7 us with
+  // eight, 13.9 with four, 14.4 with sixteen; 8 heads and 8000 keys 17.9, 19.3, 18.4).  Quad has at
+  // least a third as many items as CTAs, so few states each: four threads and larger blocks (32
+  // sequences of 2048 keys, 256 items: 53.2 us against 56.5 with eight and 64.5 with sixteen).
+  constexpr int kFewE = MODE == kQuad ? 128 : 32, kFewG = MODE == kQuad ? 4 : 8;
+  const int64_t outputs = static_cast<int64_t>(p.tile_rows / (MODE == kQuad ? 4 : 1)) * (D / 4);
   static_assert(kSmem <= 227 * 1024, "shared memory of one CTA");
-  e = static_cast<int64_t>(grid.x) * grid.y >= 2 * current_sm_count()
-          ? launch_after_predecessor(paged_attention_join_kernel<D, BF16, PAIR, 1>, grid, dim3(kPaJoinThreads), 0, stream, p)
-          : launch_after_predecessor(paged_attention_join_kernel<D, BF16, PAIR, 4>, grid, dim3(kPaJoinThreads * 4), 0, stream, p);
+  if (outputs * items >= 256 * current_sm_count()) {
+    e = launch_after_predecessor(paged_attention_join_kernel<D, BF16, MODE, 128, 1>,
+                                 dim3(static_cast<unsigned>(ceil_div(outputs, 128)), static_cast<unsigned>(items)),
+                                 dim3(128), 0, stream, p);
+  } else {
+    e = launch_after_predecessor(paged_attention_join_kernel<D, BF16, MODE, kFewE, kFewG>,
+                                 dim3(static_cast<unsigned>(ceil_div(outputs, kFewE)), static_cast<unsigned>(items)),
+                                 dim3(kFewE * kFewG), 0, stream, p);
+  }
   if (e != cudaSuccess) return fail(B200K_CUDA_ERROR, "paged attention join launch: %s", cudaGetErrorString(e));
   return B200K_OK;
 }
 
 template <int D, bool BF16>
-int launch_paged(bool pair, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const PagedParams& p,
+int launch_paged(Mode mode, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const PagedParams& p,
                  int64_t items, cudaStream_t stream) {
-  return pair ? launch_paged_as<D, BF16, true>(tq, tk, tv, p, items, stream)
-              : launch_paged_as<D, BF16, false>(tq, tk, tv, p, items, stream);
+  if (mode == kQuad) return launch_paged_as<D, BF16, kQuad>(tq, tk, tv, p, items, stream);
+  if (mode == kSplit) return launch_paged_as<D, BF16, kSplit>(tq, tk, tv, p, items, stream);
+  return launch_paged_as<D, BF16, kPair>(tq, tk, tv, p, items, stream);
 }
 
 }  // namespace
@@ -1132,7 +1219,8 @@ extern "C" int64_t b200k_paged_attention_workspace_bytes(const b200k_paged_atten
     return 0;
   const int sms = current_sm_count();
   if (sms <= 0) return 0;
-  return pick_ctas(a, sms) * 2 * lay_out_rows(a).per_tile * (padded_dim(a) + 2) * 4;
+  const Rows rows = lay_out_rows(a, sms);
+  return rows.slots(a, pick_ctas(a, sms)) * rows.per_tile * (padded_dim(a) + 2) * 4;
 }
 
 extern "C" int b200k_paged_attention(const b200k_paged_attention_args* a, b200k_stream stream_) {
@@ -1175,7 +1263,7 @@ extern "C" int b200k_paged_attention(const b200k_paged_attention_args* a, b200k_
   p.heads_kv = static_cast<int>(a->heads_kv);
   p.group = static_cast<int>(a->heads_q / a->heads_kv);
   p.dim = a->head_dim;
-  const Rows rows = lay_out_rows(a);
+  const Rows rows = lay_out_rows(a, sms);
   p.half_tokens = static_cast<int>(rows.half_tokens);
   p.row_tiles = static_cast<int>(rows.tiles);
   p.tile_rows = static_cast<int>(rows.per_tile);
@@ -1197,7 +1285,7 @@ extern "C" int b200k_paged_attention(const b200k_paged_attention_args* a, b200k_
   p.scale_log2 = a->qk_scale * 1.4426950408889634f;
   const int d = padded_dim(a);
   p.ws_acc = static_cast<float*>(a->workspace);
-  p.ws_ml = p.ws_acc + static_cast<int64_t>(p.ctas) * 2 * p.tile_rows * d;
+  p.ws_ml = p.ws_acc + rows.slots(a, p.ctas) * p.tile_rows * d;
   p.status = device_status_word();
 
   const CUtensorMapDataType dt =
@@ -1220,8 +1308,8 @@ extern "C" int b200k_paged_attention(const b200k_paged_attention_args* a, b200k_
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   const bool bf16 = a->dtype == B200K_BF16;
   if (d == 128)
-    return bf16 ? launch_paged<128, true>(rows.pair, tq, tk, tv, p, items, stream)
-                : launch_paged<128, false>(rows.pair, tq, tk, tv, p, items, stream);
-  return bf16 ? launch_paged<64, true>(rows.pair, tq, tk, tv, p, items, stream)
-              : launch_paged<64, false>(rows.pair, tq, tk, tv, p, items, stream);
+    return bf16 ? launch_paged<128, true>(rows.mode, tq, tk, tv, p, items, stream)
+                : launch_paged<128, false>(rows.mode, tq, tk, tv, p, items, stream);
+  return bf16 ? launch_paged<64, true>(rows.mode, tq, tk, tv, p, items, stream)
+              : launch_paged<64, false>(rows.mode, tq, tk, tv, p, items, stream);
 }

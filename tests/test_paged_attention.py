@@ -206,6 +206,72 @@ def test_row_tiles_of_whole_tokens(b, hq, hkv, t, d, lens, new, device_ok):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("b,hq,hkv,t,d,page,longest,tree", [
+    (50, 1, 1, 1, 128, 16, 300, False),          # one row an item, several items a CTA
+    (25, 6, 2, 5, 96, 24, 700, True),            # 15 rows
+    (17, 12, 3, 4, 72, 8, 90, True),             # 16 rows, items of one tile
+    (13, 16, 4, 3, 8, 16, 1500, True),
+    (100, 8, 1, 2, 64, 16, 130, False),          # 16 rows, a tile or two
+    (70, 17, 1, 1, 128, 32, 260, False)])        # 17 rows: the tile is not shared by four copies
+def test_many_items_with_few_rows(dtype, b, hq, hkv, t, d, page, longest, tree, device_ok):
+    g = torch.Generator().manual_seed(b)
+    lens = torch.randint(0, longest + 1, (b,), generator=g).tolist()
+    new = torch.randint(0, t + 1, (b,), generator=g).tolist()
+    lens[0], new[0] = longest, t
+    c = Cache(b, hq, hkv, t, d, dtype, page, lens, new, seed=b)
+    mask = _tree(b, t) if tree else None
+    got = c.run(tree_mask=mask)
+    c.check(got, mask)
+    assert torch.equal(got, c.run(tree_mask=mask))
+    assert bool((got.transpose(1, 2)[~c.real] == 0).all())
+    if t > 1:                                     # rows that see nothing, or only what was there
+        none = torch.zeros(t, t, dtype=torch.bool, device="cuda")
+        c.check(c.run(tree_mask=none), none)
+    out = torch.full_like(got, 7.0)
+    c.run(tree_mask=mask, out=out)
+    assert bool((out.transpose(1, 2)[~c.real] == 7).all())
+    real = c.real[:, None, :, None].expand_as(got)
+    assert torch.equal(out[real], got[real])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("value", [math.nan, -math.inf])
+def test_many_items_keep_values_that_are_not_finite_to_their_rows(value, device_ok):
+    # every sequence has a draft with such a value, at every place in a tile; queries that see it not
+    # stay finite, the others have it in that column alone
+    b, t = 60, 4
+    c = Cache(b, 2, 1, t, 64, torch.bfloat16, 16, [3 + 7 * i for i in range(b)], seed=5)
+    mask = torch.tensor([[1, 0, 0, 0], [1, 1, 0, 0], [1, 0, 1, 0], [1, 0, 1, 1]], device="cuda").bool()
+    for i in range(b):
+        at = 3 + 7 * i + 1                       # draft 1: only query 1 sees it
+        c.vc[int(c.table[i, at // 16]), 0, at % 16, 5] = value
+    got = c.run(tree_mask=mask)
+    seen = [0, 2, 3]
+    assert bool(torch.isfinite(got[:, :, seen]).all())
+    assert not bool(torch.isfinite(got[:, :, 1, 5]).any())
+    rest = [i for i in range(64) if i != 5]
+    assert bool(torch.isfinite(got[:, :, 1][..., rest]).all())
+    clean = Cache(b, 2, 1, t, 64, torch.bfloat16, 16, [3 + 7 * i for i in range(b)], seed=5)
+    want = clean.run(tree_mask=mask)
+    assert torch.equal(got[:, :, seen], want[:, :, seen])
+    # the same sums, one weight kept in fp32 instead of bfloat16: 2^-8 of it times |v| < 5
+    assert float((got[:, :, 1][..., rest].double() - want[:, :, 1][..., rest].double()).abs().max()) <= 2 * 5 * 2.0 ** -8
+
+
+@pytest.mark.gpu
+def test_many_items_with_scores_that_grow(device_ok):
+    lens = [900 - 11 * i for i in range(60)]
+    c = Cache(60, 4, 1, 2, 128, torch.bfloat16, 16, lens, spread=4.0)
+    for i, have in enumerate(lens):
+        at = torch.arange(have + 2, device="cuda")
+        where = c.table[i].long()[at // 16]
+        ramp = torch.linspace(0.1, 5.0, have + 2, device="cuda").roll(have // 3)[:, None, None]
+        c.kc[where, :, at % 16] = (c.kc[where, :, at % 16] * ramp).bfloat16()
+    c.check(c.run())
+
+
+@pytest.mark.gpu
 def test_masks_that_leave_rows_empty(device_ok):
     for lens in ([0, 0], [0, 200]):
         c = Cache(2, 4, 2, 6, 64, torch.bfloat16, 16, lens)
