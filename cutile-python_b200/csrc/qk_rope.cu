@@ -40,7 +40,7 @@ struct RopeSide {
   int64_t x_b, x_h, x_t, dy_b, dy_h, dy_t, y_b, y_h, y_t;   // elements; paged output: page, head, slot
   int heads;
   int chunks;            // ceil(heads / heads per group)
-  int log_per;           // backward: log2 of the heads per group
+  int per;               // backward: heads per group, the chunks as even as they come
   int rotate;
   int paged;
   int zero_padding;      // tokens behind new_lens[b] give zero rows (else they are left alone)
@@ -431,43 +431,35 @@ qk_rope_backward_kernel(const __grid_constant__ RopeParams p) {
 #pragma unroll
   for (int k = 0; k < 4; ++k) grad.lo[k] = grad.hi[k] = both(0.f);
 
-  // row number i of a group: head (i mod 2^k) of the chunk that is its task i / 2^k; the same
-  // number of rows for every group of the block (the sums below are warp-collective)
-  const int64_t tasks = p.total_tokens * sd.chunks;
-  const int64_t step = static_cast<int64_t>(sd.blocks) * kGroups;
-  const int64_t first = static_cast<int64_t>(block) * kGroups + group;
-  const int per = 1 << sd.log_per;
-  const int rows = static_cast<int>(((tasks + step - 1) / step) << sd.log_per);
+  // a group's rows: the heads of the chunk that is its task 0, those of task 1, ...; the same number
+  // for every group of the block (the sums below are warp-collective)
+  const int tasks = static_cast<int>(p.total_tokens) * sd.chunks;   // at most 2^30, checked at the launch
+  const int step = sd.blocks * kGroups, first = block * kGroups + group;
+  const int per = sd.per;
+  const int rounds = (tasks + step - 1) / step;
   struct Place {
-    int64_t b, t;
-    int h, heads;                 // first head, heads of this chunk (0: no such task)
+    int b, t, h, heads;           // sequence, token, first head, heads of this chunk (0: no such task)
   };
-  auto place_of = [&](int i) {
-    const int64_t task = static_cast<int64_t>(i >> sd.log_per) * step + first;
+  auto place_of = [&](int round) {
+    const int task = round * step + first;
     Place q = {0, 0, 0, 0};
-    if (task < tasks && i < rows) {
-      int64_t n;
-      if (tasks <= 0x7fffffff) {  // 32-bit divisions where they do
-        const uint32_t n32 = static_cast<uint32_t>(task) / static_cast<uint32_t>(sd.chunks);
-        q.b = n32 / static_cast<uint32_t>(p.tokens);
-        n = n32;
-      } else {
-        n = task / sd.chunks;
-        q.b = n / p.tokens;
-      }
-      q.h = static_cast<int>(task - n * sd.chunks) << sd.log_per;
+    if (task < tasks && round < rounds) {
+      const int n = task / sd.chunks, tokens = static_cast<int>(p.tokens);
+      q.h = (task - n * sd.chunks) * per;
       q.heads = min(sd.heads - q.h, per);
-      q.t = n - q.b * p.tokens;
+      q.b = n / tokens;
+      q.t = n - q.b * tokens;
     }
     return q;
   };
   const T* xs = static_cast<const T*>(sd.x);
   const T* dys = static_cast<const T*>(sd.dy);
   int fetch_heads = 0;            // of the chunk that is being requested
-  auto request = [&](int i, uint4* slot) {
-    const int u = i & (per - 1);
+  int fetch_round = 0, fetch_u = 0;
+  auto request = [&](uint4* slot) {
+    const int u = fetch_u;
     if (u == 0) {
-      const Place q = place_of(i);
+      const Place q = place_of(fetch_round);
       fetch_heads = q.heads;
       xs = static_cast<const T*>(sd.x) + q.b * sd.x_b + q.t * sd.x_t + q.h * sd.x_h;
       dys = static_cast<const T*>(sd.dy) + q.b * sd.dy_b + q.t * sd.dy_t + q.h * sd.dy_h;
@@ -478,9 +470,13 @@ qk_rope_backward_kernel(const __grid_constant__ RopeParams p) {
       xs += sd.x_h;
       dys += sd.dy_h;
     }
+    if (++fetch_u == per) {
+      fetch_u = 0;
+      ++fetch_round;
+    }
     stage_commit();
   };
-  for (int i = 0; i < kStages - 1; ++i) request(i, mine + i * 2 * kSlot);
+  for (int i = 0; i < kStages - 1; ++i) request(mine + i * 2 * kSlot);
   if (norm && threadIdx.x < GS) {
     const Pairs v = load_weights<T, INTER>(sd.w, p.w_is_f32, col);
 #pragma unroll
@@ -491,62 +487,60 @@ qk_rope_backward_kernel(const __grid_constant__ RopeParams p) {
   }
   __syncthreads();
 
-  int heads = 0;                  // of the chunk in hand
-  Angles angles;
-  T* dx = nullptr;
   int use = 0, fill = kStages - 1;
-  for (int i = 0; i < rows; ++i) {
-    const int u = i & (per - 1);
-    request(i + kStages - 1, mine + fill * 2 * kSlot);
-    fill = fill + 1 == kStages ? 0 : fill + 1;
-    if (u == 0) {
-      const Place here = place_of(i);
-      heads = here.heads;
-      if (heads > 0 && rotated) load_angles(p, position_of(p, here.b, here.t), here.t, unit, angles);
-      dx = static_cast<T*>(sd.y) + here.b * sd.y_b + here.t * sd.y_t + here.h * sd.y_h;
-    }
-    stage_wait<kStages - 1>();
-    const uint4* slot = mine + use * 2 * kSlot;
-    use = use + 1 == kStages ? 0 : use + 1;
-    Pairs g = read_staged<T, INTER>(slot + kSlot);
-    if (heads > 0 && rotated) rotate_pairs<true>(g, angles);
-    if (norm) {
-      const Pairs x = read_staged<T, INTER>(slot);
-      Pairs gx, w;
+  for (int round = 0; round < rounds; ++round) {
+    const Place here = place_of(round);
+    const int heads = here.heads;
+    const bool turns = heads > 0 && rotated;
+    Angles angles;
+    if (turns) load_angles(p, position_of(p, here.b, here.t), here.t, unit, angles);
+    T* dx = static_cast<T*>(sd.y) + here.b * sd.y_b + here.t * sd.y_t + here.h * sd.y_h;
+    for (int u = 0; u < per; ++u) {
+      request(mine + fill * 2 * kSlot);
+      fill = fill + 1 == kStages ? 0 : fill + 1;
+      stage_wait<kStages - 1>();
+      const uint4* slot = mine + use * 2 * kSlot;
+      use = use + 1 == kStages ? 0 : use + 1;
+      Pairs g = read_staged<T, INTER>(slot + kSlot);
+      if (turns) rotate_pairs<true>(g, angles);
+      if (norm) {
+        const Pairs x = read_staged<T, INTER>(slot);
+        Pairs gx, w;
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const float4 l = weights[k][unit], h = weights[2 + k][unit];
-        w.lo[2 * k] = make_float2(l.x, l.y);
-        w.lo[2 * k + 1] = make_float2(l.z, l.w);
-        w.hi[2 * k] = make_float2(h.x, h.y);
-        w.hi[2 * k + 1] = make_float2(h.z, h.w);
-      }
-      float2 sq[2] = {both(0.f), both(0.f)}, dot[2] = {both(0.f), both(0.f)};   // sum x^2, sum x g w
+        for (int k = 0; k < 2; ++k) {
+          const float4 l = weights[k][unit], h = weights[2 + k][unit];
+          w.lo[2 * k] = make_float2(l.x, l.y);
+          w.lo[2 * k + 1] = make_float2(l.z, l.w);
+          w.hi[2 * k] = make_float2(h.x, h.y);
+          w.hi[2 * k + 1] = make_float2(h.z, h.w);
+        }
+        float2 sq[2] = {both(0.f), both(0.f)}, dot[2] = {both(0.f), both(0.f)};   // sum x^2, sum x g w
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        gx.lo[k] = __fmul2_rn(g.lo[k], x.lo[k]);
-        gx.hi[k] = __fmul2_rn(g.hi[k], x.hi[k]);
-        sq[0] = __ffma2_rn(x.lo[k], x.lo[k], sq[0]);
-        sq[1] = __ffma2_rn(x.hi[k], x.hi[k], sq[1]);
-        dot[0] = __ffma2_rn(gx.lo[k], w.lo[k], dot[0]);
-        dot[1] = __ffma2_rn(gx.hi[k], w.hi[k], dot[1]);
-      }
-      const float2 sqs = __fadd2_rn(sq[0], sq[1]), dots = __fadd2_rn(dot[0], dot[1]);
-      const float r = rsqrtf(group_sum<GS>(sqs.x + sqs.y) * p.inv_dim + p.eps);
-      const float along = group_sum<GS>(dots.x + dots.y) * p.inv_dim * r * r;   // mean(h u) / (x / u)
-      // rows that are not there are zeros and add nothing
-      const float2 r2 = both(u < heads ? r : 0.f), m2 = both(u < heads ? -r * along : 0.f);
+        for (int k = 0; k < 4; ++k) {
+          gx.lo[k] = __fmul2_rn(g.lo[k], x.lo[k]);
+          gx.hi[k] = __fmul2_rn(g.hi[k], x.hi[k]);
+          sq[0] = __ffma2_rn(x.lo[k], x.lo[k], sq[0]);
+          sq[1] = __ffma2_rn(x.hi[k], x.hi[k], sq[1]);
+          dot[0] = __ffma2_rn(gx.lo[k], w.lo[k], dot[0]);
+          dot[1] = __ffma2_rn(gx.hi[k], w.hi[k], dot[1]);
+        }
+        const float2 sqs = __fadd2_rn(sq[0], sq[1]), dots = __fadd2_rn(dot[0], dot[1]);
+        const float r = rsqrtf(group_sum<GS>(sqs.x + sqs.y) * p.inv_dim + p.eps);
+        const float along = group_sum<GS>(dots.x + dots.y) * p.inv_dim * r * r;   // mean(h u) / (x / u)
+        // rows that are not there are zeros and add nothing
+        const float2 r2 = both(u < heads ? r : 0.f), m2 = both(u < heads ? -r * along : 0.f);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        grad.lo[k] = __ffma2_rn(gx.lo[k], r2, grad.lo[k]);
-        grad.hi[k] = __ffma2_rn(gx.hi[k], r2, grad.hi[k]);
-        g.lo[k] = __ffma2_rn(x.lo[k], m2, __fmul2_rn(__fmul2_rn(g.lo[k], w.lo[k]), r2));
-        g.hi[k] = __ffma2_rn(x.hi[k], m2, __fmul2_rn(__fmul2_rn(g.hi[k], w.hi[k]), r2));
+        for (int k = 0; k < 4; ++k) {
+          grad.lo[k] = __ffma2_rn(gx.lo[k], r2, grad.lo[k]);
+          grad.hi[k] = __ffma2_rn(gx.hi[k], r2, grad.hi[k]);
+          g.lo[k] = __ffma2_rn(x.lo[k], m2, __fmul2_rn(__fmul2_rn(g.lo[k], w.lo[k]), r2));
+          g.hi[k] = __ffma2_rn(x.hi[k], m2, __fmul2_rn(__fmul2_rn(g.hi[k], w.hi[k]), r2));
+        }
       }
-    }
-    if (u < heads) {
-      store_pairs<T, INTER, VEC>(dx, col, g);
-      dx += sd.y_h;
+      if (u < heads) {
+        store_pairs<T, INTER, VEC>(dx, col, g);
+        dx += sd.y_h;
+      }
     }
   }
   stage_wait<0>();
@@ -844,8 +838,10 @@ extern "C" int b200k_qk_norm_rope_backward(const b200k_qk_norm_rope_args* a, b20
     }
     s.heads = static_cast<int>(heads);
     s.rotate = a->rotary_dim > 0;
-    while ((1 << s.log_per) < most && (1 << s.log_per) < heads) ++s.log_per;
-    s.chunks = static_cast<int>(ceil_div(heads, 1 << s.log_per));
+    s.chunks = static_cast<int>(ceil_div(heads, most));
+    s.per = static_cast<int>(ceil_div(heads, s.chunks));
+    if (p.total_tokens > (1 << 30) || p.total_tokens * s.chunks > (1 << 30))
+      return fail(B200K_UNSUPPORTED, "too many rows");
     const int64_t need = ceil_div(p.total_tokens * s.chunks, groups);
     int64_t share = budget * rows / (rows_q + rows_k);
     if (share < 1) share = 1;
