@@ -9,11 +9,19 @@
 //   dw = sum over rows of g * u                  dx = rsqrt(..) * (h - u * mean(h * u))
 //
 // All of it is HBM-bound: about twenty operations per element that is read and written once.
-// A group of 4, 8 or 16 lanes owns one row, a lane 16 of its values as two 16-byte-multiple
-// vectors chosen so that both halves of every rotated pair sit in the same lane (vectors at i
-// and i + R / 2, or two neighbours): no exchange but the sum of squares.  A group keeps one
-// token and walks its heads, so the cosines, sines and weights of its columns stay in
-// registers.  Everything is computed in fp32 and rounded once, at the store.
+// A group of 4, 8 or 16 lanes owns one row, a lane 16 of its values in 16-byte pieces chosen so
+// that both halves of every rotated pair sit in the same lane: no exchange but the sum of squares.
+// A group keeps one token and walks its heads, so the cosines, sines and weights of its columns
+// are fetched once for several rows.  Rows come through shared memory by asynchronous copies,
+// which keep 64 KB (forward) to 160 KB (backward) per SM in flight without holding registers.
+// Everything is computed in fp32 and rounded once, at the store.
+//
+// Measured (4 x 4096 tokens, 32 + 8 heads of 128, bf16; of the 6.55 TB/s a copy reaches): forward 63 us
+// = 5.4 TB/s (registers instead of shared memory 69.5 us; the table's reads and the two passes of a
+// block, fetch and store, are what is left); backward 89 us = 5.7 TB/s (199 us with rows in
+// registers, 101 with scalar fp32 and weights in conflicting banks); append of 8 x 2048 ragged
+// tokens 61 us = 5.0 TB/s; a decode step of 32 sequences 3.0 us, an append step of 64 3.9 us.
+
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -51,7 +59,7 @@ struct RopeParams {
   RopeSide side[3];
   int sides;
   int dim, units, pairs, rotary;    // pairs: units that are rotated
-  int interleaved, w_is_f32;
+  int interleaved, w_is_f32, w_vec;   // w_vec: the weights start on 16-byte boundaries
   int heads_per_group;
   int64_t tokens, total_tokens;     // per sequence, of all sequences
   const float* cos;
@@ -79,102 +87,110 @@ template <> __device__ __forceinline__ float rope_from_f32<float>(float v) { ret
 template <> __device__ __forceinline__ __half rope_from_f32<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 rope_from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// Eight values as they lie in memory: 16 bytes (16-bit types) or 32 bytes (fp32).
-template <typename T> struct Oct {
-  static constexpr int kWords = sizeof(T) / 2;   // uint4s
-  uint4 q[kWords];
+// A lane's values come in pieces of 16 bytes: two of eight 16-bit values or four of four fp32.
+template <typename T> struct Piece {
+  static constexpr int kValues = 16 / sizeof(T), kCount = 16 / kValues;
 };
 
 // A lane's sixteen values as the pairs (lo, hi) that a rotation turns, two pairs to a register
-// pair: fp32 products and sums are issued two at a time.  Half split: lo is the first vector, hi
-// the second.  Interleaved: lo the even, hi the odd elements of both.
+// pair: fp32 products and sums are issued two at a time.  Half split: lo is the first half of the
+// values, hi the second.  Interleaved: lo the even, hi the odd ones.
 struct Pairs {
   float2 lo[4], hi[4];
 };
 template <bool INTER>
-__device__ __forceinline__ Pairs to_pairs(const float (&a)[8], const float (&b)[8]) {
+__device__ __forceinline__ Pairs to_pairs(const float (&v)[16]) {
   Pairs r;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     if constexpr (INTER) {
-      const float* e = k < 2 ? a + 4 * k : b + 4 * (k - 2);
-      r.lo[k] = make_float2(e[0], e[2]);
-      r.hi[k] = make_float2(e[1], e[3]);
+      r.lo[k] = make_float2(v[4 * k], v[4 * k + 2]);
+      r.hi[k] = make_float2(v[4 * k + 1], v[4 * k + 3]);
     } else {
-      r.lo[k] = make_float2(a[2 * k], a[2 * k + 1]);
-      r.hi[k] = make_float2(b[2 * k], b[2 * k + 1]);
+      r.lo[k] = make_float2(v[2 * k], v[2 * k + 1]);
+      r.hi[k] = make_float2(v[8 + 2 * k], v[8 + 2 * k + 1]);
     }
   }
   return r;
 }
 template <bool INTER>
-__device__ __forceinline__ void from_pairs(const Pairs& r, float (&a)[8], float (&b)[8]) {
+__device__ __forceinline__ void from_pairs(const Pairs& r, float (&v)[16]) {
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     if constexpr (INTER) {
-      float* e = k < 2 ? a + 4 * k : b + 4 * (k - 2);
-      e[0] = r.lo[k].x; e[1] = r.hi[k].x; e[2] = r.lo[k].y; e[3] = r.hi[k].y;
+      v[4 * k] = r.lo[k].x; v[4 * k + 1] = r.hi[k].x; v[4 * k + 2] = r.lo[k].y; v[4 * k + 3] = r.hi[k].y;
     } else {
-      a[2 * k] = r.lo[k].x; a[2 * k + 1] = r.lo[k].y;
-      b[2 * k] = r.hi[k].x; b[2 * k + 1] = r.hi[k].y;
+      v[2 * k] = r.lo[k].x; v[2 * k + 1] = r.lo[k].y;
+      v[8 + 2 * k] = r.hi[k].x; v[8 + 2 * k + 1] = r.hi[k].y;
     }
   }
 }
 
+// The values of a piece.
 template <typename T>
-__device__ __forceinline__ void unpack_oct(const Oct<T>& o, float (&f)[8]) {
-  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(&o);
+__device__ __forceinline__ void unpack_piece(const uint4& q, float* f) {
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      f[i] = __uint_as_float(w[i]);
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
       f[2 * i] = __uint_as_float(w[i] << 16);
       f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    } else {
+      const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      f[2 * i] = v.x;
+      f[2 * i + 1] = v.y;
     }
-  } else {
-    const T* e = reinterpret_cast<const T*>(&o);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = rope_to_f32<T>(e[i]);
   }
 }
 
 template <typename T, bool VEC>
-__device__ __forceinline__ void store_oct(T* p, const float (&f)[8]) {
-  Oct<T> o;
-  uint32_t* w = reinterpret_cast<uint32_t*>(&o);
-  if constexpr (sizeof(T) == 4) {
+__device__ __forceinline__ void store_piece(T* p, const float* f) {
+  uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(f[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      w[i] = std::is_same<T, __half>::value ? pack_f16x2(f[2 * i], f[2 * i + 1]) : pack_bf16x2(f[2 * i], f[2 * i + 1]);
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(f[i]);
+    else w[i] = std::is_same<T, __half>::value ? pack_f16x2(f[2 * i], f[2 * i + 1]) : pack_bf16x2(f[2 * i], f[2 * i + 1]);
   }
   if constexpr (VEC) {
-#pragma unroll
-    for (int i = 0; i < Oct<T>::kWords; ++i) reinterpret_cast<uint4*>(p)[i] = o.q[i];
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
   } else {
-    const T* e = reinterpret_cast<const T*>(&o);
+    const T* e = reinterpret_cast<const T*>(w);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) p[i] = e[i];
+    for (int i = 0; i < Piece<T>::kValues; ++i) p[i] = e[i];
   }
 }
 
 // Norm weights of a lane's columns; zeros where it has none.
 template <typename T, bool INTER, typename Columns>
-__device__ __forceinline__ Pairs load_weights(const void* w, int w_is_f32, const Columns& col) {
-  float a[8], b[8];
+__device__ __forceinline__ Pairs load_weights(const RopeParams& p, const void* w, const Columns& col) {
+  constexpr int kValues = Piece<T>::kValues;
+  float v[16];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    a[i] = b[i] = 0.f;
-    if (w_is_f32) {
-      if (col.has_lo) a[i] = static_cast<const float*>(w)[col.lo + i];
-      if (col.has_hi) b[i] = static_cast<const float*>(w)[col.hi + i];
+  for (int q = 0; q < Piece<T>::kCount; ++q) {
+    float* f = v + q * kValues;
+#pragma unroll
+    for (int i = 0; i < kValues; ++i) f[i] = 0.f;
+    if (!col.has[q]) continue;
+    if (p.w_vec && !p.w_is_f32) {
+      unpack_piece<T>(*reinterpret_cast<const uint4*>(static_cast<const T*>(w) + col.at[q]), f);
+    } else if (p.w_vec) {
+#pragma unroll
+      for (int i = 0; i < kValues; i += 4)
+        unpack_piece<float>(*reinterpret_cast<const uint4*>(static_cast<const float*>(w) + col.at[q] + i), f + i);
     } else {
-      if (col.has_lo) a[i] = rope_to_f32<T>(static_cast<const T*>(w)[col.lo + i]);
-      if (col.has_hi) b[i] = rope_to_f32<T>(static_cast<const T*>(w)[col.hi + i]);
+#pragma unroll 1
+      for (int i = 0; i < kValues; ++i) {
+        const int at = col.at[q] + i;
+        const float x = p.w_is_f32 ? static_cast<const float*>(w)[at] : rope_to_f32<T>(static_cast<const T*>(w)[at]);
+#pragma unroll
+        for (int j = 0; j < kValues; ++j)
+          if (j == i) f[j] = x;
+      }
     }
   }
-  return to_pairs<INTER>(a, b);
+  return to_pairs<INTER>(v);
 }
 
 // Cosines and sines of the lane's pairs; with `minus` the negated sines.
@@ -199,28 +215,34 @@ __device__ __forceinline__ float group_sum(float v) {
   return v;
 }
 
-// Which columns a lane holds.
+// Which columns a lane holds: those of its pieces, `unit` the lane's number in the row's group.
+// 16-bit rows: pieces at 8 u and R / 2 + 8 u (half split), or side by side (interleaved).  fp32
+// rows: piece q at q R / 4 + 4 u, so that a group's lanes read and write 16 neighbouring bytes
+// each (32 bytes of a lane side by side cost twice the sectors: 107 us against 79 for 12749 tokens
+// of 36 heads of 128).  Without a piece: column 0, so that addresses stay in the row.
+template <typename T>
 struct LaneColumns {
-  int lo, hi;             // first column of each vector
-  bool has_lo, has_hi;
+  int at[Piece<T>::kCount];
+  bool has[Piece<T>::kCount];
   bool rotated;
 };
 
-template <bool INTER>
-__device__ __forceinline__ LaneColumns lane_columns(const RopeParams& p, int unit) {
-  LaneColumns c;
+template <typename T, bool INTER>
+__device__ __forceinline__ LaneColumns<T> lane_columns(const RopeParams& p, int unit) {
+  constexpr int kCount = Piece<T>::kCount, kValues = Piece<T>::kValues;
+  LaneColumns<T> c;
   c.rotated = unit < p.pairs;
-  if (c.rotated) {
-    c.lo = INTER ? unit * 16 : unit * 8;
-    c.hi = INTER ? unit * 16 + 8 : unit * 8 + p.rotary / 2;
-    c.has_lo = c.has_hi = true;
-  } else {
-    c.lo = p.rotary + (unit - p.pairs) * 16;
-    c.hi = c.lo + 8;
-    c.has_lo = unit < p.units;
-    c.has_hi = c.has_lo && c.hi < p.dim;
-    if (!c.has_lo) c.lo = 0;
-    if (!c.has_hi) c.hi = 0;
+#pragma unroll
+  for (int q = 0; q < kCount; ++q) {
+    if (c.rotated) {
+      c.at[q] = kCount == 4 ? q * 4 * p.pairs + 4 * unit : (INTER ? unit * 16 + 8 * q : unit * 8 + q * (p.rotary / 2));
+      c.has[q] = true;
+    } else {
+      const int rest = p.units - p.pairs, u = unit - p.pairs;   // lanes of the columns that pass through
+      c.at[q] = p.rotary + (kCount == 4 ? q * kValues * rest + kValues * u : u * 16 + 8 * q);
+      c.has[q] = unit < p.units && c.at[q] < p.dim;
+      if (!c.has[q]) c.at[q] = 0;
+    }
   }
   return c;
 }
@@ -235,7 +257,9 @@ __device__ __forceinline__ int64_t position_of(const RopeParams& p, int64_t b, i
 
 // Cosines and sines of a position for the lane's pairs.  A position outside the table is recorded
 // in the status word and gives NaN rows: nothing is read out of range.
-__device__ __forceinline__ void load_angles(const RopeParams& p, int64_t pos, int64_t t, int unit, Angles& g) {
+template <typename T, bool INTER>
+__device__ __forceinline__ void load_angles(const RopeParams& p, int64_t pos, int64_t t, int unit,
+                                            const LaneColumns<T>& col, Angles& g) {
   if (pos < 0 || pos >= p.table_rows) {
     if (unit == 0) report_bad_index(p.status, kRolePosition, static_cast<int>(t));
     const float nan = __int_as_float(0x7fc00000);
@@ -243,49 +267,52 @@ __device__ __forceinline__ void load_angles(const RopeParams& p, int64_t pos, in
     for (int k = 0; k < 4; ++k) g.c[k] = g.s[k] = g.minus[k] = make_float2(nan, nan);
     return;
   }
-  const float4* cr = reinterpret_cast<const float4*>(p.cos + pos * p.table_stride + unit * 8);
-  const float4* sr = reinterpret_cast<const float4*>(p.sin + pos * p.table_stride + unit * 8);
+  const float* cr = p.cos + pos * p.table_stride;
+  const float* sr = p.sin + pos * p.table_stride;
+  if constexpr (Piece<T>::kCount == 4 && INTER) {   // two of the rotation's pairs to a piece
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const float4 c = cr[i], s = sr[i];
-    g.c[2 * i] = make_float2(c.x, c.y);
-    g.c[2 * i + 1] = make_float2(c.z, c.w);
-    g.s[2 * i] = make_float2(s.x, s.y);
-    g.s[2 * i + 1] = make_float2(s.z, s.w);
-    g.minus[2 * i] = make_float2(-s.x, -s.y);
-    g.minus[2 * i + 1] = make_float2(-s.z, -s.w);
+    for (int k = 0; k < 4; ++k) {
+      g.c[k] = *reinterpret_cast<const float2*>(cr + col.at[k] / 2);
+      g.s[k] = *reinterpret_cast<const float2*>(sr + col.at[k] / 2);
+    }
+  } else {                                          // four side by side
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int from = Piece<T>::kCount == 4 ? col.at[i] : unit * 8 + 4 * i;
+      const float4 c = *reinterpret_cast<const float4*>(cr + from), s = *reinterpret_cast<const float4*>(sr + from);
+      g.c[2 * i] = make_float2(c.x, c.y);
+      g.c[2 * i + 1] = make_float2(c.z, c.w);
+      g.s[2 * i] = make_float2(s.x, s.y);
+      g.s[2 * i + 1] = make_float2(s.z, s.w);
+    }
   }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) g.minus[k] = make_float2(-g.s[k].x, -g.s[k].y);
 }
 
-// A lane's two vectors of a row (zeros where it has none), fetched into its own slots of shared
-// memory: [vector][16-byte piece][thread], so neighbouring threads hit neighbouring banks.  With
-// VEC the copies are asynchronous and cost no registers while they are in flight; a thread waits
-// for its own copies only, so no barrier is needed.
+// A lane's pieces of a row (zeros where it has none), fetched into its own slots of shared memory:
+// [piece][thread], so neighbouring threads hit neighbouring banks.  With VEC the copies are
+// asynchronous and cost no registers while they are in flight; a thread waits for its own copies
+// only, so no barrier is needed.
 template <typename T, bool VEC>
-__device__ __forceinline__ void stage_row(uint4* slot, const T* row, const LaneColumns& col, bool on) {
-  constexpr int kWords = Oct<T>::kWords;
+__device__ __forceinline__ void stage_row(uint4* slot, const T* row, const LaneColumns<T>& col, bool on) {
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const bool has = half == 0 ? col.has_lo : col.has_hi;
-    const T* src = row + (half == 0 ? col.lo : col.hi);   // a column of the row also where the lane has none
+  for (int q = 0; q < Piece<T>::kCount; ++q) {
+    const T* src = row + col.at[q];
     if constexpr (VEC) {
-#pragma unroll
-      for (int i = 0; i < kWords; ++i) {
-        const uint32_t dst = smem_u32(slot + (half * kWords + i) * kRopeThreads);
-        // a source size of 0 fills the slot with zeros and reads nothing
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst),
-                     "l"(reinterpret_cast<uint64_t>(reinterpret_cast<const uint4*>(src) + i)), "r"(has && on ? 16 : 0)
-                     : "memory");
-      }
+      const uint32_t dst = smem_u32(slot + q * kRopeThreads);
+      // a source size of 0 fills the slot with zeros and reads nothing
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(src)),
+                   "r"(col.has[q] && on ? 16 : 0)
+                   : "memory");
     } else {
-      Oct<T> o = {};
-      T* e = reinterpret_cast<T*>(&o);
-      if (has && on) {
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      T* e = reinterpret_cast<T*>(&v);
+      if (col.has[q] && on) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = src[i];
+        for (int i = 0; i < Piece<T>::kValues; ++i) e[i] = src[i];
       }
-#pragma unroll
-      for (int i = 0; i < kWords; ++i) slot[(half * kWords + i) * kRopeThreads] = o.q[i];
+      slot[q * kRopeThreads] = v;
     }
   }
 }
@@ -294,23 +321,18 @@ template <int N> __device__ __forceinline__ void stage_wait() { asm volatile("cp
 
 template <typename T, bool INTER>
 __device__ __forceinline__ Pairs read_staged(const uint4* slot) {
-  Oct<T> a, b;
+  float v[16];
 #pragma unroll
-  for (int i = 0; i < Oct<T>::kWords; ++i) {
-    a.q[i] = slot[i * kRopeThreads];
-    b.q[i] = slot[(Oct<T>::kWords + i) * kRopeThreads];
-  }
-  float x[8], y[8];
-  unpack_oct<T>(a, x);
-  unpack_oct<T>(b, y);
-  return to_pairs<INTER>(x, y);
+  for (int q = 0; q < Piece<T>::kCount; ++q) unpack_piece<T>(slot[q * kRopeThreads], v + q * Piece<T>::kValues);
+  return to_pairs<INTER>(v);
 }
 template <typename T, bool INTER, bool VEC>
-__device__ __forceinline__ void store_pairs(T* row, const LaneColumns& col, const Pairs& r) {
-  float a[8], b[8];
-  from_pairs<INTER>(r, a, b);
-  if (col.has_lo) store_oct<T, VEC>(row + col.lo, a);
-  if (col.has_hi) store_oct<T, VEC>(row + col.hi, b);
+__device__ __forceinline__ void store_pairs(T* row, const LaneColumns<T>& col, const Pairs& r) {
+  float v[16];
+  from_pairs<INTER>(r, v);
+#pragma unroll
+  for (int q = 0; q < Piece<T>::kCount; ++q)
+    if (col.has[q]) store_piece<T, VEC>(row + col.at[q], v + q * Piece<T>::kValues);
 }
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
@@ -324,7 +346,7 @@ template <typename T, int GS, bool INTER, bool VEC>
 __global__ void __launch_bounds__(kRopeThreads)
 qk_rope_kernel(const __grid_constant__ RopeParams p) {
   constexpr int kRows = ForwardRows<T>::kMax, kBatch = kRows / 2;
-  constexpr int kSlot = 2 * Oct<T>::kWords * kRopeThreads;
+  constexpr int kSlot = Piece<T>::kCount * kRopeThreads;
   __shared__ uint4 stage[kRows * kSlot];
   uint4* mine = stage + threadIdx.x;
   const int unit = threadIdx.x % GS;
@@ -334,7 +356,7 @@ qk_rope_kernel(const __grid_constant__ RopeParams p) {
   const RopeSide& sd = p.side[which];
   const bool live = n < p.total_tokens;
   const int64_t b = live ? n / p.tokens : 0, t = live ? n - b * p.tokens : 0;
-  const LaneColumns col = lane_columns<INTER>(p, unit);
+  const LaneColumns<T> col = lane_columns<T, INTER>(p, unit);
   const bool padded = live && p.new_lens != nullptr && t >= p.new_lens[b];
 
   const T* x = static_cast<const T*>(sd.x) + b * sd.x_b + t * sd.x_t;
@@ -365,10 +387,10 @@ qk_rope_kernel(const __grid_constant__ RopeParams p) {
   }
   Angles angles;
   const bool rotate = sd.rotate != 0 && col.rotated && store && !padded;
-  if (rotate) load_angles(p, position_of(p, b, t), t, unit, angles);
+  if (rotate) load_angles<T, INTER>(p, position_of(p, b, t), t, unit, col, angles);
   const bool norm = sd.w != nullptr;
   Pairs w;
-  if (norm) w = load_weights<T, INTER>(sd.w, p.w_is_f32, col);
+  if (norm) w = load_weights<T, INTER>(p, sd.w, col);
 
   T* y = static_cast<T*>(sd.y) + out + h_begin * sd.y_h;
 #pragma unroll
@@ -414,7 +436,7 @@ __global__ void __launch_bounds__(kRopeThreads, kBackwardMinBlocks)
 qk_rope_backward_kernel(const __grid_constant__ RopeParams p) {
   constexpr int kStages = sizeof(T) == 4 ? kBackwardStages / 2 : kBackwardStages;
   constexpr int kGroups = kRopeThreads / GS;
-  constexpr int kSlot = 2 * Oct<T>::kWords * kRopeThreads;
+  constexpr int kSlot = Piece<T>::kCount * kRopeThreads;
   __shared__ uint4 stage[kStages * 2 * kSlot];
   __shared__ float4 weights[4][GS];   // [piece][unit]: neighbouring lanes read neighbouring banks
   pdl_launch_dependents();   // the sum of the partial rows may be set up now; it waits for this grid
@@ -424,7 +446,7 @@ qk_rope_backward_kernel(const __grid_constant__ RopeParams p) {
   while (which + 1 < p.sides && static_cast<int>(blockIdx.x) >= p.side[which + 1].first_block) ++which;
   const RopeSide& sd = p.side[which];
   const int block = blockIdx.x - sd.first_block;
-  const LaneColumns col = lane_columns<INTER>(p, unit);
+  const LaneColumns<T> col = lane_columns<T, INTER>(p, unit);
   const bool norm = sd.w != nullptr;
   const bool rotated = col.rotated && sd.rotate != 0;
   Pairs grad;                     // weight gradient of the lane's columns
@@ -478,7 +500,7 @@ qk_rope_backward_kernel(const __grid_constant__ RopeParams p) {
   };
   for (int i = 0; i < kStages - 1; ++i) request(mine + i * 2 * kSlot);
   if (norm && threadIdx.x < GS) {
-    const Pairs v = load_weights<T, INTER>(sd.w, p.w_is_f32, col);
+    const Pairs v = load_weights<T, INTER>(p, sd.w, col);
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       weights[k][unit] = make_float4(v.lo[2 * k].x, v.lo[2 * k].y, v.lo[2 * k + 1].x, v.lo[2 * k + 1].y);
@@ -493,7 +515,7 @@ qk_rope_backward_kernel(const __grid_constant__ RopeParams p) {
     const int heads = here.heads;
     const bool turns = heads > 0 && rotated;
     Angles angles;
-    if (turns) load_angles(p, position_of(p, here.b, here.t), here.t, unit, angles);
+    if (turns) load_angles<T, INTER>(p, position_of(p, here.b, here.t), here.t, unit, col, angles);
     T* dx = static_cast<T*>(sd.y) + here.b * sd.y_b + here.t * sd.y_t + here.h * sd.y_h;
     for (int u = 0; u < per; ++u) {
       request(mine + fill * 2 * kSlot);
@@ -550,23 +572,24 @@ qk_rope_backward_kernel(const __grid_constant__ RopeParams p) {
   static_assert(sizeof(stage) >= kGroups * (GS * 16 + 1) * 4, "the stages are reused for the sums");
   __syncthreads();
   {
-    float a[8], b[8];
-    from_pairs<INTER>(grad, a, b);
+    float v[16];
+    from_pairs<INTER>(grad, v);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      sums[group][unit * 16 + k] = a[k];
-      sums[group][unit * 16 + 8 + k] = b[k];
-    }
+    for (int k = 0; k < 16; ++k) sums[group][unit * 16 + k] = v[k];
   }
   __syncthreads();
   for (int i = threadIdx.x; i < GS * 16; i += kRopeThreads) {
-    const LaneColumns lc = lane_columns<INTER>(p, i / 16);
-    const bool high = (i % 16) >= 8;
-    if (high ? lc.has_hi : lc.has_lo) {
+    const LaneColumns<T> lc = lane_columns<T, INTER>(p, i / 16);
+    constexpr int kValues = Piece<T>::kValues;
+    int column = -1;
+#pragma unroll
+    for (int q = 0; q < Piece<T>::kCount; ++q)
+      if (q == i % 16 / kValues && lc.has[q]) column = lc.at[q] + i % kValues;
+    if (column >= 0) {
       float v = 0.f;
 #pragma unroll 8
       for (int g = 0; g < kGroups; ++g) v += sums[g][i];
-      sd.dw[static_cast<int64_t>(block) * p.dim + (high ? lc.hi : lc.lo) + (i % 8)] = v;
+      sd.dw[static_cast<int64_t>(block) * p.dim + column] = v;
     }
   }
 }
@@ -616,6 +639,12 @@ bool side_vectors(const RopeSide& s, int64_t elem) {
   return multiple_of_16_bytes(s.x, elem, {s.x_b, s.x_h, s.x_t}) &&
          multiple_of_16_bytes(s.y, elem, {s.y_b, s.y_h, s.y_t}) &&
          (s.dy == nullptr || multiple_of_16_bytes(s.dy, elem, {s.dy_b, s.dy_h, s.dy_t}));
+}
+
+int weight_vectors(const RopeParams& p) {
+  uintptr_t bits = 0;
+  for (int i = 0; i < p.sides; ++i) bits |= reinterpret_cast<uintptr_t>(p.side[i].w);
+  return (bits & 15) == 0;
 }
 
 // Lanes per row: the smallest group whose lanes hold 16 values each.
@@ -698,6 +727,7 @@ int launch_forward(RopeParams& p, int dtype, cudaStream_t stream) {
     heads_all += p.side[i].heads;
     vec = vec && side_vectors(p.side[i], dtype == B200K_F32 ? 4 : 2);
   }
+  p.w_vec = weight_vectors(p);
   p.heads_per_group = pick_heads_per_group(p.total_tokens, heads_all, lanes,
                                            dtype == B200K_F32 ? ForwardRows<float>::kMax : ForwardRows<__half>::kMax, sms);
   int64_t chunks = 0;
@@ -857,6 +887,7 @@ extern "C" int b200k_qk_norm_rope_backward(const b200k_qk_norm_rope_args* a, b20
   if (p.sides > 0) {
     bool vec = true;
     for (int i = 0; i < p.sides; ++i) vec = vec && side_vectors(p.side[i], a->dtype == B200K_F32 ? 4 : 2);
+    p.w_vec = weight_vectors(p);
     int e;
     if (a->dtype == B200K_BF16) e = launch_backward_type<__nv_bfloat16>(p, lanes, vec, first, stream);
     else if (a->dtype == B200K_F16) e = launch_backward_type<__half>(p, lanes, vec, first, stream);

@@ -200,6 +200,20 @@ def test_weights_positions_and_eps(w_dtype, device_ok):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,w_dtype", [(torch.bfloat16, torch.bfloat16), (torch.float16, torch.float32),
+                                           (torch.float32, torch.float32)])
+def test_weights_off_their_16_byte_boundaries(dtype, w_dtype, device_ok):
+    for inter in (False, True):
+        q, k, qw, kw, cos, sin, pos = _make(2, 3, 2, 7, 96, dtype, 32, w_dtype=w_dtype)
+        odd = torch.empty(97, dtype=w_dtype, device="cuda")[1:].copy_(qw)
+        _check(q, k, odd, kw, cos, sin, pos, inter)
+        args = (torch.ones_like(q), torch.ones_like(k), q, k)
+        got = b200k.qk_norm_rope_backward(*args, odd, kw, cos, sin, pos, interleaved=inter)
+        want = b200k.qk_norm_rope_backward(*args, qw, kw, cos, sin, pos, interleaved=inter)
+        assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_layouts_and_alignment(dtype, device_ok):
     q, k, qw, kw, cos, sin, pos = _make(2, 4, 2, 11, 64, dtype, 64)
