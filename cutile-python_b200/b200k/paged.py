@@ -75,7 +75,9 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
     places in the cache (drafts of one depth in a tree share a position).  Rows behind
     new_lens[b] are padding: their cache slots stay as they are, as do their rows of a given
     ``q_out``; in a q_out made here they are zero.  A token whose page lies outside the table
-    or the cache is not stored, and ``raise_on_device_error()`` names its sequence."""
+    or the cache is not stored, and ``raise_on_device_error()`` names its sequence.  Sequences may
+    share the pages that they only read: of two tokens that a call stores in one slot, either may
+    stay.  Outputs overlap no input, but for q_out = q."""
     tensors = (k, v, q, k_cache, v_cache, page_table, cache_lens, cos, sin, q_weight, k_weight, positions, new_lens, q_out)
     scalars = eps, interleaved
     done = _APPEND.call(tensors, scalars)
@@ -161,9 +163,12 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     scores a tree of drafts.
 
     float16 or bfloat16, heads a multiple of the cache's, Dim a multiple of 8 up to 128, pages
-    of a multiple of 8 tokens, qk_scale positive (None: 1 / sqrt(Dim)).  A query that sees no token gives zeros.  Slots that hold none of
-    the sequence's tokens are never used.  Rows behind new_lens[b] are padding: they stay as
-    they are in a given ``out`` and are zero in one made here."""
+    of a multiple of 8 tokens, qk_scale positive (None: 1 / sqrt(Dim)).  A query that sees no token
+    gives zeros.  Slots that hold none of the sequence's tokens are never used.  Rows behind
+    new_lens[b] are padding: they stay as they are in a given ``out`` (which overlaps no input) and
+    are zero in one made here.  Sequences may share pages.  A length or page outside the table or
+    the cache is not followed: that sequence's rows mean nothing, and ``raise_on_device_error()``
+    names it."""
     tensors, scalars = (q, k_cache, v_cache, page_table, cache_lens, new_lens, tree_mask, out), (qk_scale,)
     done = _ATTENTION.call(tensors, scalars)
     if done is not NotImplemented:

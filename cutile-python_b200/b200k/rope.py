@@ -166,7 +166,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor,
     A weight of None leaves that norm out (rotation alone).  ``cos`` / ``sin`` are tables by
     position (``rope_table``); ``positions`` is (SeqLen,) or (Batch, SeqLen), None = 0, 1, 2, ...
     Pairs are (i, i + rotary_dim / 2), or neighbours with ``interleaved``.  ``q_out`` / ``k_out``
-    may be q / k themselves.  A position outside the table gives NaN rows, and
+    may be q / k themselves and overlap nothing else.  A position outside the table gives NaN rows, and
     ``raise_on_device_error()`` names it."""
     tensors, scalars = (q, k, q_weight, k_weight, cos, sin, positions, q_out, k_out), (eps, interleaved)
     done = _FORWARD.call(tensors, scalars)

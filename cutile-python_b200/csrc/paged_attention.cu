@@ -22,7 +22,7 @@
 //                               maximum, sum and O; the group of a run's last tile joins the two
 //                               states at its end, while the other already works on the next
 //                               run's first tile, whose S was issued before (Q has two places)
-//   quad   (at most 32 rows)    split, with the rows four times in the tile: warp q of a group takes
+//   quad   (at most 16 rows)    split, with the rows four times in the tile: warp q of a group takes
 //                               keys [32 q, 32 q + 32) of every tile, its P is zero elsewhere, and
 //                               its rows are a partial state of their own.  A warp's 128
 //                               exponentials, 1000 cycles of the special-function unit whether
@@ -84,6 +84,7 @@ struct PagedParams {
   int page_size, max_pages, box_rows;
   int page_shift;                      // log2 of the page size, -1 where it is no power of two
   int ctas;
+  int join_blocks;                     // blocks of the joining kernel for an item
   int o_vec;                           // rows of out on 16-byte boundaries
   int zero_padding;
   float scale_log2;
@@ -280,8 +281,9 @@ __device__ __forceinline__ uint32_t visible_keys(const PagedParams& p, const Seq
   return bits;
 }
 
-// A finished row's O in the workspace (column k at acc[k / 4][.][k % 4]): adds the share of the step's tokens whose row of V was
-// cleared for being not finite, where the row sees them, and with `whole` writes the output.
+// A finished row's O in the workspace (column k at acc[k / 4][.][k % 4]): adds the share of the
+// step's tokens whose row of V was cleared for being not finite, where the row sees them, and with
+// `whole` writes the output.
 // Such values are a model's failure, but they stay with the rows that see them.
 template <int D, bool BF16>
 __device__ __forceinline__ void add_cleared_drafts(const PagedParams& p, const Run& run, int hq, int t, float* acc,
@@ -350,7 +352,6 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
 
-  pdl_launch_dependents();   // the joining kernel may be set up now; it waits for this grid
   if (threadIdx.x == 0) {
     for (int i = 0; i < NUM_BARS; ++i) {
       int count = 1;
@@ -378,6 +379,9 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   }
   // what the kernel before this one in the stream writes is read from here on
   pdl_wait();
+  // The joining kernel may be set up now.  Not earlier: it reads the lengths before it waits for this
+  // grid, and a kernel that writes them may have let its own successor start before its end.
+  pdl_launch_dependents();
   // where this CTA begins, and its first pages: every warp finds its own, without a wait for
   // another's
   Walk walk;
@@ -698,12 +702,12 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
             sees[0] = visible_keys(p, run.seq, run.b, t, t0, t1, key0 + 32 * quarter, lane);
           } else {
 #pragma unroll 1
-          for (int w = 0; w < 4; ++w) {                  // rolled: the words move up
-            sees[0] = sees[1];
-            sees[1] = sees[2];
-            sees[2] = sees[3];
-            sees[3] = visible_keys(p, run.seq, run.b, t, t0, t1, key0 + 32 * w, lane);
-          }
+            for (int w = 0; w < 4; ++w) {                // rolled: the words move up
+              sees[0] = sees[1];
+              sees[1] = sees[2];
+              sees[2] = sees[3];
+              sees[3] = visible_keys(p, run.seq, run.b, t, t0, t1, key0 + 32 * w, lane);
+            }
           }
         }
         if (!mbar_wait(bar(S_FULL + x), sp, abort_flag)) {
@@ -784,19 +788,19 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
             mx = fmaxf(fmax3(m2[0], m2[1], sq[15]), sq[31]);
           } else {
 #pragma unroll 1
-          for (int half = 0; half < halves; ++half) {
-            float s[64];
-            load_scores(half, s);
-            float m4[4];
+            for (int half = 0; half < halves; ++half) {
+              float s[64];
+              load_scores(half, s);
+              float m4[4];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              m4[c] = fmax3(s[16 * c], s[16 * c + 1], s[16 * c + 2]);
+              for (int c = 0; c < 4; ++c) {
+                m4[c] = fmax3(s[16 * c], s[16 * c + 1], s[16 * c + 2]);
 #pragma unroll
-              for (int k = 3; k < 15; k += 2) m4[c] = fmax3(m4[c], s[16 * c + k], s[16 * c + k + 1]);
-              m4[c] = fmaxf(m4[c], s[16 * c + 15]);
+                for (int k = 3; k < 15; k += 2) m4[c] = fmax3(m4[c], s[16 * c + k], s[16 * c + k + 1]);
+                m4[c] = fmaxf(m4[c], s[16 * c + 15]);
+              }
+              mx = fmaxf(mx, fmax3(m4[0], m4[1], fmaxf(m4[2], m4[3])));
             }
-            mx = fmaxf(mx, fmax3(m4[0], m4[1], fmaxf(m4[2], m4[3])));
-          }
           }
           const float m_new = fmaxf(m_used, mx * p.scale_log2);
           const bool grow = (m_new - m_used > kRescaleThreshold) || (m_used == -INFINITY && m_new > -INFINITY);
@@ -847,36 +851,36 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
             if (lane == 0) mbar_arrive(bar(P_HALF + x));
           } else {
 #pragma unroll 1
-          for (int c = 0; c < 2; ++c) {
-            uint32_t pk[32];
-            if (c < halves) {
-            float s[64];
-            load_scores(c, s);                            // P of the first half lies over scores already used
+            for (int c = 0; c < 2; ++c) {
+              uint32_t pk[32];
+              if (c < halves) {
+                float s[64];
+                load_scores(c, s);                            // P of the first half lies over scores already used
 #pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              const float2 y = __ffma2_rn(make_float2(s[2 * k], s[2 * k + 1]), scale2, negm2);
-              // pair: every fourth pair on the FMA pipe, as two row tiles keep the special-function
-              // unit busier than the tensor cores (133 -> 130 us); split waits for memory
-              const bool poly = PAIR && k % kFmhaPolyEvery == kFmhaPolyEvery - 1;
-              const float2 e = poly ? exp2_poly_pair(y) : make_float2(fast_exp2(y.x), fast_exp2(y.y));
-              sum2[k & 3] = __fadd2_rn(sum2[k & 3], e);
-              // P is rounded to the input type: it is the tensor cores' operand
-              pk[k] = BF16 ? pack_bf16x2(e.x, e.y) : pack_f16x2(e.x, e.y);
-            }
-            } else {
+                for (int k = 0; k < 32; ++k) {
+                  const float2 y = __ffma2_rn(make_float2(s[2 * k], s[2 * k + 1]), scale2, negm2);
+                  // pair: every fourth pair on the FMA pipe, as two row tiles keep the special-function
+                  // unit busier than the tensor cores (133 -> 130 us); split waits for memory
+                  const bool poly = PAIR && k % kFmhaPolyEvery == kFmhaPolyEvery - 1;
+                  const float2 e = poly ? exp2_poly_pair(y) : make_float2(fast_exp2(y.x), fast_exp2(y.y));
+                  sum2[k & 3] = __fadd2_rn(sum2[k & 3], e);
+                  // P is rounded to the input type: it is the tensor cores' operand
+                  pk[k] = BF16 ? pack_bf16x2(e.x, e.y) : pack_f16x2(e.x, e.y);
+                }
+              } else {
 #pragma unroll
-              for (int k = 0; k < 32; ++k) pk[k] = 0u;
+                for (int k = 0; k < 32; ++k) pk[k] = 0u;
+              }
+              tmem_st_32x32b_x32(tmem_s + c * 32, pk);
+              if (c == 0) {                                 // the first 64 keys are enough for half of P V
+                if (edge && (!PAIR || x == 0)) clear_v();
+                await_o_read(i);
+                tmem_st_wait();
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(P_HALF + x));
+              }
             }
-            tmem_st_32x32b_x32(tmem_s + c * 32, pk);
-            if (c == 0) {                                 // the first 64 keys are enough for half of P V
-              if (edge && (!PAIR || x == 0)) clear_v();
-              await_o_read(i);
-              tmem_st_wait();
-              tc_fence_before_sync();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(bar(P_HALF + x));
-            }
-          }
           }
           l += ((sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y)) + ((sum2[2].x + sum2[2].y) + (sum2[3].x + sum2[3].y));
           tmem_st_wait();
@@ -986,7 +990,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           }
           __syncwarp();
         }
-        if (by_hand && live) 
+        if (by_hand && live)
           add_cleared_drafts<D, BF16>(p, run, at.hq, at.t, reinterpret_cast<float*>(acc), m_used, inv_l, whole,
                                        QUAD ? quarter : -1);
         __syncwarp();
@@ -1017,9 +1021,10 @@ paged_attention_join_kernel(const __grid_constant__ PagedParams p) {
   const int lane = threadIdx.x & 31;
   pdl_launch_dependents();
   const int per_seq = p.heads_kv * p.row_tiles;
-  const int b = blockIdx.y / per_seq, item = blockIdx.y - b * per_seq;
+  const int any_item = blockIdx.x / p.join_blocks;      // of all sequences
+  const int b = any_item / per_seq, item = any_item - b * per_seq;
   const int head = item / p.row_tiles, row_tile = item - head * p.row_tiles;
-  const int element = blockIdx.x * E + threadIdx.x % E;
+  const int element = (blockIdx.x - any_item * p.join_blocks) * E + threadIdx.x % E;
   constexpr bool PAIR = MODE == kPair;
   constexpr int kStates = MODE == kQuad ? 4 : 1;     // partial states of a row that a run leaves
   const int out_rows = p.tile_rows / kStates;
@@ -1070,7 +1075,7 @@ paged_attention_join_kernel(const __grid_constant__ PagedParams p) {
       for (int k = g; k < last; k += G) {
         const int c = c0 + k / kStates, at = (k % kStates) * out_rows + row;
         // only the first of an item's CTAs may have begun with an earlier item
-        const int64_t slot = kStates > 1 && c0 == c1 ? 2 * static_cast<int64_t>(p.ctas) + blockIdx.y
+        const int64_t slot = kStates > 1 && c0 == c1 ? 2 * static_cast<int64_t>(p.ctas) + any_item
                                                      : 2 * static_cast<int64_t>(c) + (ranges.begin(c) >= first ? 0 : 1);
         const float2 state = __ldcg(ml + slot * p.tile_rows + at);
         take(state.x, state.y, __ldcg(acc + (slot * (D / 4) + quad) * p.tile_rows + at));
@@ -1156,14 +1161,14 @@ int check_args(const b200k_paged_attention_args* a) {
   const int64_t limit = int64_t(1) << 29;   // sums of two such counts fit 32 bits
   if (a->tokens * a->heads_q > limit || static_cast<int64_t>(a->max_pages) * a->page_size > limit ||
       a->num_pages >= limit || a->batch > limit || a->heads_kv > limit ||
-      a->batch * a->heads_kv > 65535 ||
       a->batch * a->heads_kv * lay_out_rows(a, 1).tiles * ceil_div(static_cast<int64_t>(a->max_pages) * a->page_size, kPaBN) > limit)
     return fail(B200K_UNSUPPORTED, "more rows, pages or sequences than the kernel counts");
   return B200K_OK;
 }
 
 template <int D, bool BF16, int MODE>
-int launch_paged_as(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const PagedParams& p, int64_t items, cudaStream_t stream) {
+int launch_paged_as(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, PagedParams p, int64_t items,
+                    cudaStream_t stream) {
   constexpr int kSmem = Rings<D>::kSmem;
   auto kernel = paged_attention_kernel<D, BF16, MODE>;
   static bool configured[64] = {};
@@ -1175,10 +1180,6 @@ int launch_paged_as(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensor
       return fail(B200K_CUDA_ERROR, "cudaFuncSetAttribute(%d): %s", kSmem, cudaGetErrorString(e));
     configured[dev] = true;
   }
-  // programmatic launches: this kernel's set-up (barriers, tensor memory, descriptors) overlaps the
-  // end of the kernel before it, and its end the set-up of the joining kernel
-  cudaError_t e = launch_after_predecessor(kernel, dim3(p.ctas), dim3(kPaThreads), kSmem, stream, tq, tk, tv, p);
-  if (e != cudaSuccess) return fail(B200K_CUDA_ERROR, "paged attention launch: %s", cudaGetErrorString(e));
   // Many outputs: a thread for each.  Few mean few items, each shared by many CTAs: several threads
   // to an output, in blocks of a warp of outputs (a token of 32 heads and 1024 keys 13.7 us with
   // eight, 13.9 with four, 14.4 with sixteen; 8 heads and 8000 keys 17.9, 19.3, 18.4).  Quad has at
@@ -1187,15 +1188,17 @@ int launch_paged_as(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensor
   constexpr int kFewE = MODE == kQuad ? 128 : 32, kFewG = MODE == kQuad ? 4 : 8;
   const int64_t outputs = static_cast<int64_t>(p.tile_rows / (MODE == kQuad ? 4 : 1)) * (D / 4);
   static_assert(kSmem <= 227 * 1024, "shared memory of one CTA");
-  if (outputs * items >= 256 * current_sm_count()) {
-    e = launch_after_predecessor(paged_attention_join_kernel<D, BF16, MODE, 128, 1>,
-                                 dim3(static_cast<unsigned>(ceil_div(outputs, 128)), static_cast<unsigned>(items)),
-                                 dim3(128), 0, stream, p);
-  } else {
-    e = launch_after_predecessor(paged_attention_join_kernel<D, BF16, MODE, kFewE, kFewG>,
-                                 dim3(static_cast<unsigned>(ceil_div(outputs, kFewE)), static_cast<unsigned>(items)),
-                                 dim3(kFewE * kFewG), 0, stream, p);
-  }
+  const bool many = outputs * items >= 256 * current_sm_count();
+  p.join_blocks = static_cast<int>(ceil_div(outputs, many ? 128 : kFewE));
+  if (items * p.join_blocks > INT32_MAX) return fail(B200K_UNSUPPORTED, "more row tiles than a grid has blocks");
+  // programmatic launches: this kernel's set-up (barriers, tensor memory, descriptors) overlaps the
+  // end of the kernel before it, and its end the set-up of the joining kernel
+  cudaError_t e = launch_after_predecessor(kernel, dim3(p.ctas), dim3(kPaThreads), kSmem, stream, tq, tk, tv, p);
+  if (e != cudaSuccess) return fail(B200K_CUDA_ERROR, "paged attention launch: %s", cudaGetErrorString(e));
+  const dim3 grid(static_cast<unsigned>(items * p.join_blocks));
+  e = many ? launch_after_predecessor(paged_attention_join_kernel<D, BF16, MODE, 128, 1>, grid, dim3(128), 0, stream, p)
+           : launch_after_predecessor(paged_attention_join_kernel<D, BF16, MODE, kFewE, kFewG>, grid, dim3(kFewE * kFewG),
+                                      0, stream, p);
   if (e != cudaSuccess) return fail(B200K_CUDA_ERROR, "paged attention join launch: %s", cudaGetErrorString(e));
   return B200K_OK;
 }
@@ -1304,7 +1307,6 @@ extern "C" int b200k_paged_attention(const b200k_paged_attention_args* a, b200k_
                       p.box_rows, 1, 1, CU_TENSOR_MAP_SWIZZLE_128B))
     return B200K_INVALID_ARG;
   const int64_t items = a->batch * a->heads_kv * p.row_tiles;
-  if (items > 65535) return fail(B200K_UNSUPPORTED, "more row tiles than the kernel counts");
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   const bool bf16 = a->dtype == B200K_BF16;
   if (d == 128)

@@ -236,6 +236,18 @@ def test_many_items_with_few_rows(dtype, b, hq, hkv, t, d, page, longest, tree, 
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("t,hq", [(1, 64), (3, 128)])
+def test_more_items_than_a_grid_has_rows(t, hq, device_ok):
+    g = torch.Generator().manual_seed(t)
+    b = 1100
+    lens = torch.randint(0, 31, (b,), generator=g).tolist()
+    c = Cache(b, hq, 64, t, 8, torch.bfloat16, 8, lens, torch.randint(0, t + 1, (b,), generator=g).tolist())
+    got = c.run()
+    c.check(got)
+    assert bool((got.transpose(1, 2)[~c.real] == 0).all())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("value", [math.nan, -math.inf])
 def test_many_items_keep_values_that_are_not_finite_to_their_rows(value, device_ok):
     # every sequence has a draft with such a value, at every place in a tile; queries that see it not
