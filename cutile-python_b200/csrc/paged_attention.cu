@@ -37,6 +37,12 @@
 // What a run does once (masks, Q rows that are not aligned, tokens that are not finite) is kept in
 // rolled loops: unrolled, the kernel was 180 KB of code, more than the instruction cache.
 //
+// Measured (bf16, heads of 128, 32 on 8): 32 sequences of 2048 - 8192 keys, a token each, 115 us = 5.9 TB/s,
+// 0.89 of a copy (quad; a tile of 64 KB every 2230 cycles); 8 x 16 drafts of the same lengths 44 us =
+// 3.9 TB/s, where the first copies, the last softmax and the join are a third; 4 x 64 drafts of 8192 -
+// 32768 keys 124 us: 2.0 - 2.2 us for a tile of 256 rows (pair), bound by the chain S, softmax, P V of a row
+// tile.  One token of 32 heads and 1024 keys (fp16) 13.5 us: launch, lengths -> pages -> K, join.
+//
 // Slots behind a sequence's last token may hold anything: their scores are masked by index and
 // their rows of V are cleared in shared memory, since 0 * NaN is not 0.
 #include <cuda_bf16.h>
