@@ -59,6 +59,7 @@ constexpr int kPaBM = 128;             // query rows of a tile
 constexpr int kPaBN = 128;             // keys of a tile
 constexpr int kPaThreads = 384;        // K warp, MMA warp, two softmax groups of four warps, V and Q warps
 constexpr int kPaQuadRows = 16;        // rows up to which quad is taken
+constexpr int kPaMaxBatch = 65535;     // every warp that looks for its place reads all lengths
 constexpr int kPaTmemCols = 512;       // S_A, S_B, O_A, O_B; P over S
 
 // Rings of K and V tiles in what Q's two tiles leave of 224 KB.  V tiles wait for the softmax, so V
@@ -123,14 +124,6 @@ __device__ __forceinline__ int warp_sum(int v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
-}
-
-// Key tiles of the sequences [0, count), warp-collective.
-__device__ __forceinline__ int tiles_before(const PagedParams& p, int count, int lane) {
-  int sum = 0;
-#pragma unroll 1
-  for (int b = lane; b < count; b += 32) sum += seq_info(p, b).tiles;
-  return warp_sum(sum);
 }
 
 // `total` tiles in `ctas` ranges, the first total % ctas of them one tile longer: first tile of
@@ -1036,8 +1029,15 @@ paged_attention_join_kernel(const __grid_constant__ PagedParams p) {
   const int out_rows = p.tile_rows / kStates;
   const int quad = element / out_rows, row = element - quad * out_rows;
   const SeqInfo seq = seq_info(p, b);
-  const Ranges ranges(tiles_before(p, p.batch, lane) * per_seq, p.ctas);
-  const int first = tiles_before(p, b, lane) * per_seq + item * seq.tiles;
+  int all = 0, before = 0;             // key tiles of all sequences, of those before this one
+#pragma unroll 1
+  for (int i = lane; i < p.batch; i += 32) {
+    const int tiles = seq_info(p, i).tiles;
+    all += tiles;
+    before += i < b ? tiles : 0;
+  }
+  const Ranges ranges(warp_sum(all) * per_seq, p.ctas);
+  const int first = warp_sum(before) * per_seq + item * seq.tiles;
   const int half = row / kPaBM, in_half = (row - half * kPaBM) / p.group;
   const int hq = head * p.group + (row - half * kPaBM) - in_half * p.group;
   const int t = (PAIR ? row_tile * 2 + half : row_tile) * p.half_tokens + in_half;
@@ -1171,7 +1171,7 @@ int check_args(const b200k_paged_attention_args* a) {
     return fail(B200K_UNSUPPORTED, "page_size must be a positive multiple of 8 (got %d)", a->page_size);
   const int64_t limit = int64_t(1) << 29;   // sums of two such counts fit 32 bits
   if (a->tokens * a->heads_q > limit || static_cast<int64_t>(a->max_pages) * a->page_size > limit ||
-      a->num_pages >= limit || a->batch > limit || a->heads_kv > limit ||
+      a->num_pages >= limit || a->batch > kPaMaxBatch || a->heads_kv > limit ||
       a->batch * a->heads_kv * lay_out_rows(a, 1).tiles * ceil_div(static_cast<int64_t>(a->max_pages) * a->page_size, kPaBN) > limit)
     return fail(B200K_UNSUPPORTED, "more rows, pages or sequences than the kernel counts");
   return B200K_OK;

@@ -697,8 +697,8 @@ int b200k_paged_kv_append(const b200k_paged_kv_append_args* args, b200k_stream s
  * table as its end; both are recorded in the status word.
  * Query head h reads key/value head h / (heads_q / heads_kv).  D a multiple of 8 up to 128;
  * page_size a multiple of 8; bases and strides of q and of the caches multiples of 16 bytes; at
- * most 128 query heads per key/value head.  Padding rows of
- * out are left as they are, or become zero with `zero_padding`. */
+ * most 128 query heads per key/value head and 65535 sequences.  Padding rows of out are left as
+ * they are, or become zero with `zero_padding`. */
 typedef struct {
   const void* q;                /* (batch, heads_q, tokens, D) */
   const void* k_cache;
