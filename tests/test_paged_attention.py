@@ -383,6 +383,18 @@ def test_agrees_with_contiguous_attention(device_ok):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("t", [1, 5])
+def test_sequences_share_the_pages_of_a_prefix(t, device_ok):
+    c = Cache(6, 8, 2, t, 128, torch.bfloat16, 16, [640, 647, 655, 900, 640, 1300])
+    c.table[1:, :40] = c.table[0, :40]            # 640 tokens, whole pages
+    c.check(c.run())
+    c.table[4] = c.table[0]                       # a whole sequence twice, its step's tokens too
+    got = c.run()
+    c.check(got)
+    assert torch.equal(got, c.run())
+
+
+@pytest.mark.gpu
 def test_pages_and_lengths_out_of_range_are_reported():
     c = Cache(3, 4, 2, 2, 64, torch.bfloat16, 16, [100, 50, 200])
     good = c.run()
