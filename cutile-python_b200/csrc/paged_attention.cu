@@ -861,7 +861,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                   // pair: every fourth pair on the FMA pipe, as two row tiles keep the special-function
                   // unit busier than the tensor cores (133 -> 130 us); split waits for memory
                   const bool poly = PAIR && k % kFmhaPolyEvery == kFmhaPolyEvery - 1;
-                  const float2 e = poly ? exp2_poly_pair(y) : make_float2(fast_exp2(y.x), fast_exp2(y.y));
+                  const float2 e = poly ? exp2_poly_pair<true>(y) : make_float2(fast_exp2(y.x), fast_exp2(y.y));
                   sum2[k & 3] = __fadd2_rn(sum2[k & 3], e);
                   // P is rounded to the input type: it is the tensor cores' operand
                   pk[k] = BF16 ? pack_bf16x2(e.x, e.y) : pack_f16x2(e.x, e.y);

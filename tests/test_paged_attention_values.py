@@ -1,0 +1,66 @@
+"""Attention over a paged cache where rows see nothing, and where queries, keys or values are not
+finite, in every form that the kernel takes: rows four times in a tile (many items of up to 16
+rows), one row tile, pairs of row tiles (more than 128 rows), items of one CTA and shared ones.
+The formulas, the cache and the tolerances are those of test_paged_attention."""
+import math
+
+import pytest
+import torch
+
+import oracle
+from test_paged_attention import Cache, _tree
+
+# (sequences, query heads, key/value heads, tokens, head dim, lengths): what the rows and items give
+FORMS = {
+    "quad": (60, 4, 1, 2, 64, [5 + 7 * i for i in range(60)]),              # eight rows, items of one CTA and shared ones
+    "split": (2, 8, 2, 5, 64, [90, 40]),                                    # 20 rows, items of one tile
+    "split shared": (1, 8, 2, 5, 128, [3000]),
+    "pair": (2, 8, 2, 40, 64, [70, 0]),                                     # 160 rows, items of one tile
+    "pair shared": (1, 8, 2, 70, 128, [1500]),
+}
+
+
+def _cache(form, dtype, seed=0):
+    b, hq, hkv, t, d, lens = FORMS[form]
+    return Cache(b, hq, hkv, t, d, dtype, 16, lens, seed=seed)
+
+
+def _slot(c, b, at):
+    """Index of token `at` of sequence b in a cache, all heads."""
+    return int(c.table[b, at // 16]), slice(None), at % 16
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("b,hq,hkv,t,lens", [
+    (2, 8, 2, 40, [0, 200]),            # 160 rows over an empty cache: an item of one tile, one CTA's
+    (90, 8, 2, 40, [0] * 90),           # more items than CTAs
+    (1, 2, 1, 300, [0]),                # items of three tiles that CTAs share
+    (2, 256, 2, 2, [0, 50])])           # a token's 128 heads fill a row tile
+def test_rows_that_see_nothing_among_more_than_128(dtype, b, hq, hkv, t, lens, device_ok):
+    c = Cache(b, hq, hkv, t, 64, dtype, 16, lens, seed=t)
+    mask = torch.rand(t, t, generator=torch.Generator().manual_seed(1)).cuda() < 0.2
+    mask[0] = mask[t // 2] = False
+    got = c.run(tree_mask=mask)
+    c.check(got, mask)
+    assert bool((got[0, :, [0, t // 2]] == 0).all())
+    none = torch.zeros_like(mask)
+    got = c.run(tree_mask=none)
+    c.check(got, none)
+    assert bool((got[0] == 0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMS)
+def test_large_values_stay_with_the_rows_that_see_them(form, device_ok):
+    # 2^118 times 2^-125 would be a 2^-7: a masked draft's weight is zero
+    c, clean = _cache(form, torch.bfloat16), _cache(form, torch.bfloat16)
+    t = c.q.shape[2]
+    mask = torch.eye(t, dtype=torch.bool, device="cuda")
+    mask[:, 0] = True
+    for b in range(c.q.shape[0]):
+        for j in range(1, t):
+            c.vc[_slot(c, b, int(c.lens[b]) + j)] = 2.0 ** 118
+    got = c.run(tree_mask=mask)
+    c.check(got, mask)
+    assert torch.equal(got[:, :, 0], clean.run(tree_mask=mask)[:, :, 0])
