@@ -14,28 +14,39 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
   return r;
 }
 
+// The larger one, NaN where either is NaN.
+__device__ __forceinline__ float fmax_or_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // Every kFmhaPolyEvery-th pair of scores takes its exp2 on the FMA pipe (a degree-3
 // polynomial after splitting off the integer part) instead of the special-function unit,
 // which is the busiest pipe of the softmax.  Relative error 7.5e-5, far below the rounding
 // of P to 16 bits.  0 disables the polynomial path.
 //
-// Arguments far below zero: without EXACT_ZERO they give 2^-125, which a row that sees something
-// does not notice.  With it the power of two is a factor of its own, so that arguments from -127
-// down (a masked score's -inf) give the bits of 2^-127, a zero: rows that see nothing keep a sum
-// of zero, and a masked value no weight.  One more product per pair (4 x 64 drafts over 8192 - 32768 keys
+// Arguments far below zero: without EXACT_ENDS they give 2^-125, which a row that sees something
+// does not notice, and so does NaN.  With it the power of two is a factor of its own, so that
+// arguments from -127 down (a masked score's -inf) give the bits of 2^-127, a zero: rows that see
+// nothing keep a sum of zero, and a masked value no weight.  NaN stays NaN.  One more product per pair (4 x 64 drafts over 8192 - 32768 keys
 // 127 us as before); the contiguous attention, whose rows all see something, keeps the shorter form.
 #ifndef B200K_FMHA_POLY
 #define B200K_FMHA_POLY 4
 #endif
 constexpr int kFmhaPolyEvery = B200K_FMHA_POLY;
 
-template <bool EXACT_ZERO = false>
+template <bool EXACT_ENDS = false>
 __device__ __forceinline__ float2 exp2_poly_pair(float2 x) {
   const float2 magic = make_float2(12582912.0f, 12582912.0f);       // 1.5 * 2^23
   const float2 neg_magic = make_float2(-12582912.0f, -12582912.0f);
-  constexpr float kLeast = EXACT_ZERO ? -127.0f : -125.0f;
-  x.x = fmaxf(x.x, kLeast);
-  x.y = fmaxf(x.y, kLeast);
+  if constexpr (EXACT_ENDS) {
+    x.x = fmax_or_nan(x.x, -127.0f);
+    x.y = fmax_or_nan(x.y, -127.0f);
+  } else {
+    x.x = fmaxf(x.x, -125.0f);
+    x.y = fmaxf(x.y, -125.0f);
+  }
   const float2 t = __fadd2_rn(x, magic);            // integer part lands in the low mantissa bits
   const float2 i = __fadd2_rn(t, neg_magic);
   const float2 f = __fadd2_rn(x, make_float2(-i.x, -i.y));   // in [-0.5, 0.5]
@@ -43,7 +54,7 @@ __device__ __forceinline__ float2 exp2_poly_pair(float2 x) {
                         make_float2(0.2426111251115799f, 0.2426111251115799f));
   p = __ffma2_rn(p, f, make_float2(0.6932609677314758f, 0.6932609677314758f));
   p = __ffma2_rn(p, f, make_float2(0.9999280571937561f, 0.9999280571937561f));
-  if constexpr (EXACT_ZERO) {
+  if constexpr (EXACT_ENDS) {
     const int one = 127 << 23;
     return __fmul2_rn(p, make_float2(__int_as_float((__float_as_int(t.x) << 23) + one),
                                      __int_as_float((__float_as_int(t.y) << 23) + one)));

@@ -64,3 +64,23 @@ def test_large_values_stay_with_the_rows_that_see_them(form, device_ok):
     got = c.run(tree_mask=mask)
     c.check(got, mask)
     assert torch.equal(got[:, :, 0], clean.run(tree_mask=mask)[:, :, 0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", ["pair"])
+@pytest.mark.parametrize("draft", [False, True])
+@pytest.mark.parametrize("residue", range(8))
+def test_a_key_of_nan_reaches_every_row_that_sees_it(form, draft, residue, device_ok):
+    # at every place of the eight scores that one round of exponentials takes
+    c = _cache(form, torch.bfloat16)
+    b, t = c.q.shape[0], c.q.shape[2]
+    mask = _tree(b, t, seed=residue)
+    for i in range(b):
+        have = int(c.lens[i])
+        first, end = (have, have + t) if draft else (0, have)
+        places = [at for at in range(first, end) if at % 8 == residue]
+        if places:
+            c.kc[_slot(c, i, places[len(places) // 2])][..., 3] = math.nan
+    got = c.run(tree_mask=mask)
+    want, _ = oracle.paged_attention_ref(c.q, c.kc, c.vc, c.table, c.lens, None, mask)
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
