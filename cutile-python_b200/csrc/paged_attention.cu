@@ -1067,10 +1067,12 @@ paged_attention_join_kernel(const __grid_constant__ PagedParams p) {
     if (pass == 1) pdl_wait();
     float m = -INFINITY, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    // A state that saw nothing has a maximum of -inf and a sum of 0.  One that saw NaN alone has that
+    // maximum too (maxima ignore NaN) and a sum of NaN, which no factor of 0 removes.  Without a
+    // branch, so that the loads of several states are under way at once.
     auto take = [&](float mc, float lc, const float4& a) {
-      if (mc == -INFINITY) return;              // saw nothing
       const float top = fmaxf(m, mc);
-      const float f = (m == -INFINITY) ? 0.f : fast_exp2(m - top), h = fast_exp2(mc - top);
+      const float f = (m == -INFINITY) ? 0.f : fast_exp2(m - top), h = (mc == -INFINITY) ? 0.f : fast_exp2(mc - top);
       l = l * f + lc * h;
       o.x = o.x * f + a.x * h;
       o.y = o.y * f + a.y * h;

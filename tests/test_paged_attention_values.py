@@ -67,7 +67,7 @@ def test_large_values_stay_with_the_rows_that_see_them(form, device_ok):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("form", ["pair"])
+@pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("draft", [False, True])
 @pytest.mark.parametrize("residue", range(8))
 def test_a_key_of_nan_reaches_every_row_that_sees_it(form, draft, residue, device_ok):
@@ -84,3 +84,28 @@ def test_a_key_of_nan_reaches_every_row_that_sees_it(form, draft, residue, devic
     got = c.run(tree_mask=mask)
     want, _ = oracle.paged_attention_ref(c.q, c.kc, c.vc, c.table, c.lens, None, mask)
     assert torch.equal(torch.isnan(got), torch.isnan(want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("form", FORMS)
+def test_a_query_of_nan_gives_a_row_of_nan(dtype, form, device_ok):
+    c, clean = _cache(form, dtype), _cache(form, dtype)
+    t = c.q.shape[2]
+    c.q[:, 1, t - 1, 5] = math.nan
+    got = c.run()
+    bad = torch.zeros_like(got, dtype=torch.bool)
+    bad[:, 1, t - 1] = True
+    assert bool(torch.isnan(got[bad]).all()) and torch.equal(got[~bad], clean.run()[~bad])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("first,end", [(0, 5), (0, 32), (32, 64), (0, 128), (128, 1400)])
+def test_ranges_of_nan_keys_are_not_dropped(form, first, end, device_ok):
+    # a quarter of a tile, a tile, a CTA's whole range: states whose scores are all NaN
+    c = _cache(form, torch.bfloat16)
+    for i in range(c.q.shape[0]):
+        for at in range(first, min(end, int(c.lens[i]))):
+            c.kc[_slot(c, i, at)] = math.nan
+    c.check(c.run())
