@@ -48,6 +48,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <cfloat>
+
 #include "common.cuh"
 #include "host.h"
 #include "softmax.cuh"
@@ -235,6 +237,13 @@ __device__ __forceinline__ Run saved_run(volatile int* w) {
   r.seq.have = w[4]; r.seq.fresh = w[5]; r.seq.len = w[6]; r.seq.tiles = w[7];
   r.b = w[8]; r.head = w[9]; r.row_tile = w[10]; r.first = w[11]; r.last = w[12];
   return r;
+}
+
+// 1 / l of a row: 0 where it saw no key (the maximum is -inf).  A sum of 0 over keys that it saw, whose
+// scores are all -inf, is the softmax's 0 / 0; a sum that is NaN stays NaN.
+__device__ __forceinline__ float softmax_factor(float m, float l) {
+  if (l > 0.0f) return __fdividef(1.0f, l);
+  return m == -INFINITY ? l : __int_as_float(0x7fc00000);
 }
 
 // Whether a 16-bit float is an infinity or NaN, for the two halves of a word.
@@ -801,7 +810,9 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
               mx = fmaxf(mx, fmax3(m4[0], m4[1], fmaxf(m4[2], m4[3])));
             }
           }
-          const float m_new = fmaxf(m_used, mx * p.scale_log2);
+          // a row that sees a key has a maximum above -inf, also where its scores are -inf or NaN
+          const bool some = !edge || (sees[0] | sees[1] | sees[2] | sees[3]) != 0u;
+          const float m_new = fmax3(m_used, mx * p.scale_log2, some ? -FLT_MAX : -INFINITY);
           const bool grow = (m_new - m_used > kRescaleThreshold) || (m_used == -INFINITY && m_new > -INFINITY);
           const bool any_grow = __any_sync(0xffffffffu, grow);
           float alpha = 1.0f;
@@ -938,7 +949,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                                        : 2 * static_cast<int64_t>(blockIdx.x) + (runs == 0 ? 0 : 1);
       // quad: every quarter's rows are a state of their own
       const int tile_row = QUAD ? quarter * (p.tile_rows / 4) + lane : (PAIR ? x * kPaBM : 0) + row;
-      const float inv_l = (l > 0.0f) ? __fdividef(1.0f, l) : (l == 0.0f ? 0.0f : l);
+      const float inv_l = softmax_factor(m_used, l);
       const bool by_hand = edges && bad_draft[runs & 1] == runs;
       const bool to_out = whole && !by_hand;
       uint16_t* o_row = p.out + run.b * p.o_b + at.hq * p.o_h + at.t * p.o_t;
@@ -1067,9 +1078,9 @@ paged_attention_join_kernel(const __grid_constant__ PagedParams p) {
     if (pass == 1) pdl_wait();
     float m = -INFINITY, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    // A state that saw nothing has a maximum of -inf and a sum of 0.  One that saw NaN alone has that
-    // maximum too (maxima ignore NaN) and a sum of NaN, which no factor of 0 removes.  Without a
-    // branch, so that the loads of several states are under way at once.
+    // A state that saw nothing has a maximum of -inf and a sum of 0; the sum of one that saw NaN is
+    // NaN, which no factor of 0 removes.  Without a branch, so that the loads of several states are
+    // under way at once.
     auto take = [&](float mc, float lc, const float4& a) {
       const float top = fmaxf(m, mc);
       const float f = (m == -INFINITY) ? 0.f : fast_exp2(m - top), h = (mc == -INFINITY) ? 0.f : fast_exp2(mc - top);
@@ -1104,7 +1115,7 @@ paged_attention_join_kernel(const __grid_constant__ PagedParams p) {
         for (int k = 1; k < G; ++k) take(sm_ml[k][e].x, sm_ml[k][e].y, sm_o[k][e]);
       }
     }
-    const float inv_l = (l > 0.0f) ? __fdividef(1.0f, l) : (l == 0.0f ? 0.0f : l);
+    const float inv_l = softmax_factor(m, l);
     const uint32_t lo = BF16 ? pack_bf16x2(o.x * inv_l, o.y * inv_l) : pack_f16x2(o.x * inv_l, o.y * inv_l);
     const uint32_t hi = BF16 ? pack_bf16x2(o.z * inv_l, o.w * inv_l) : pack_f16x2(o.z * inv_l, o.w * inv_l);
     if (pass == 1 && store && g == 0) {

@@ -109,3 +109,43 @@ def test_ranges_of_nan_keys_are_not_dropped(form, first, end, device_ok):
         for at in range(first, min(end, int(c.lens[i]))):
             c.kc[_slot(c, i, at)] = math.nan
     c.check(c.run())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMS)
+def test_scores_of_minus_infinity(form, device_ok):
+    # a key of -inf has no weight; where a row sees no other, its softmax is 0 / 0.  A row that sees
+    # no key at all stays zero.
+    c = _cache(form, torch.bfloat16)
+    b, t = c.q.shape[0], c.q.shape[2]
+    c.q[..., 0] = 1.0
+    mask = _tree(b, t, seed=2)
+    for i in range(b):
+        for at in range(int(c.lens[i])):
+            if i % 2 == 0 or at % 3 == 0:
+                c.kc[_slot(c, i, at)][..., 0] = -math.inf
+        c.kc[_slot(c, i, int(c.lens[i]) + t - 1)][..., 0] = -math.inf
+    c.check(c.run(tree_mask=mask), mask)
+    mask[:, t - 1] = False
+    mask[:, t - 2] = False
+    mask[:, t - 2, t - 1] = True                 # sees the draft of -inf alone, besides the cache
+    got = c.run(tree_mask=mask)
+    c.check(got, mask)
+    for i in range(b):
+        if int(c.lens[i]) == 0:
+            assert bool((got[i, :, t - 1] == 0).all()) and bool(torch.isnan(got[i, :, t - 2]).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMS)
+def test_a_query_of_infinity(form, device_ok):
+    # scores of inf make the row NaN, scores of -inf drop the key
+    c, clean = _cache(form, torch.bfloat16), _cache(form, torch.bfloat16)
+    t = c.q.shape[2]
+    c.q[:, 1, t - 1, 5] = math.inf
+    got = c.run()
+    want, _ = oracle.paged_attention_ref(c.q, c.kc, c.vc, c.table, c.lens)
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    rest = torch.ones_like(got, dtype=torch.bool)
+    rest[:, 1, t - 1] = False
+    assert torch.equal(got[rest], clean.run()[rest])
