@@ -78,14 +78,13 @@ template <int D> struct Rings {
 
 struct PagedParams {
   const uint16_t* q;
-  const uint16_t* k;                   // caches as plain memory: the rare path of non-finite drafts
-  const uint16_t* v;
+  const uint16_t* v;                   // as plain memory: the rare path of values that are not finite
   uint16_t* out;
   const int* page_table;
   const int* cache_lens;
   const int* new_lens;
   const uint8_t* mask;
-  int64_t q_b, q_h, q_t, o_b, o_h, o_t, kc_p, kc_h, kc_s, vc_p, vc_h, vc_s, mask_b, mask_t, mask_j;
+  int64_t o_b, o_h, o_t, vc_p, vc_h, vc_s, mask_b, mask_t, mask_j;
   int64_t page_table_stride, num_pages;
   int batch, tokens, heads_kv, group, dim;
   int row_tiles, half_tokens;          // row tiles; tokens of a 128-row half: half_tokens * group <= 128 rows
@@ -246,11 +245,11 @@ __device__ __forceinline__ float softmax_factor(float m, float l) {
   return m == -INFINITY ? l : __int_as_float(0x7fc00000);
 }
 
-// Whether a 16-bit float is an infinity or NaN, for the two halves of a word.
+// Ones in the halves of a word whose 16-bit floats are finite.
 template <bool BF16>
-__device__ __forceinline__ bool word_not_finite(uint32_t w) {
+__device__ __forceinline__ uint32_t finite_halves(uint32_t w) {
   const uint32_t e = BF16 ? 0x7f80u : 0x7c00u;
-  return (w & e) == e || ((w >> 16) & e) == e;
+  return ((w & e) == e ? 0u : 0xffffu) | (((w >> 16) & e) == e ? 0u : 0xffff0000u);
 }
 template <bool BF16>
 __device__ __forceinline__ float half_to_float(uint16_t h) {
@@ -289,41 +288,64 @@ __device__ __forceinline__ uint32_t visible_keys(const PagedParams& p, const Seq
   return bits;
 }
 
-// A finished row's O in the workspace (column k at acc[k / 4][.][k % 4]): adds the share of the
-// step's tokens whose row of V was cleared for being not finite, where the row sees them, and with
-// `whole` writes the output.
-// Such values are a model's failure, but they stay with the rows that see them.
-template <int D, bool BF16>
-__device__ __forceinline__ void add_cleared_drafts(const PagedParams& p, const Run& run, int hq, int t, float* acc,
-                                                   float m, float inv_l, bool whole, int quarter) {
-  auto at = [&](int k) -> float& { return acc[static_cast<int64_t>(k / 4) * p.tile_rows * 4 + k % 4]; };
-  const uint16_t* q_row = p.q + run.b * p.q_b + hq * p.q_h + t * p.q_t;
-  const int end = min(run.seq.len, run.last * kPaBN);
-  for (int key = max(run.seq.have, run.first * kPaBN); key < end; ++key) {
-    if (quarter >= 0 && ((key >> 5) & 3) != quarter) continue;   // quad: another warp's key
-    const int draft = key - run.seq.have;
-    const bool sees = p.mask != nullptr ? p.mask[run.b * p.mask_b + t * p.mask_t + draft * p.mask_j] != 0 : draft <= t;
-    const int page = p.page_table[run.b * p.page_table_stride + key / p.page_size];
-    if (!sees || page < 0 || page >= p.num_pages) continue;
-    const uint16_t* v_row = p.v + page * p.vc_p + run.head * p.vc_h + (key % p.page_size) * p.vc_s;
-    bool bad = false;
+// Adds to a row that has been written, to out (`whole`) or as a partial state (column k at
+// acc[k / 4][.][k % 4]), the values that are not finite in the V of the step's tokens that token t
+// sees, among keys [from, to): they were taken out of the tile, and any weight leaves them what they
+// are.  `quarter` (quad): only the keys of that quarter of a tile, -1: all.
+template <bool BF16>
+__device__ __forceinline__ void add_not_finite(const PagedParams& p, const Run& run, int t, int quarter, bool whole,
+                                               uint16_t* o_row, float* acc) {
+  const int from = max(run.seq.have, run.first * kPaBN);
+  int to = min(run.seq.len, run.last * kPaBN);
+  if (p.mask == nullptr) to = min(to, run.seq.have + t + 1);
+  const uint8_t* mask = p.mask + run.b * p.mask_b + t * p.mask_t;
+  const int* pages = p.page_table + run.b * p.page_table_stride;
 #pragma unroll 1
-    for (int k = 0; k < p.dim; ++k) bad = bad || word_not_finite<BF16>(v_row[k]);
-    if (!bad) continue;
-    const uint16_t* k_row = p.k + page * p.kc_p + run.head * p.kc_h + (key % p.page_size) * p.kc_s;
-    float score = 0.f;
+  for (int c0 = 0; c0 < p.dim; c0 += 8) {
+    const uint16_t* v = p.v + run.head * p.vc_h + c0;
+    float sum[8] = {};
+    bool all_nan = false;
+    // four slots of a page on their way at once
 #pragma unroll 1
-    for (int k = 0; k < p.dim; ++k) score += half_to_float<BF16>(q_row[k]) * half_to_float<BF16>(k_row[k]);
-    const float e = fast_exp2(score * p.scale_log2 - m);
-#pragma unroll 1
-    for (int k = 0; k < p.dim; ++k) at(k) += e * half_to_float<BF16>(v_row[k]);
-  }
-  if (!whole) return;
-  uint16_t* o_row = p.out + run.b * p.o_b + hq * p.o_h + t * p.o_t;
-#pragma unroll 1
-  for (int k = 0; k < p.dim; ++k) {
-    if constexpr (BF16) reinterpret_cast<__nv_bfloat16*>(o_row)[k] = __float2bfloat16_rn(at(k) * inv_l);
-    else reinterpret_cast<__half*>(o_row)[k] = __float2half_rn(at(k) * inv_l);
+    for (int k0 = from & ~3; k0 < to && !all_nan; k0 += 4) {
+      if (quarter >= 0 && ((k0 >> 5) & 3) != quarter) continue;
+      const int entry = k0 / p.page_size, page = pages[entry];
+      if (page < 0 || page >= p.num_pages) continue;
+      const uint16_t* at = v + page * p.vc_p + (k0 - entry * p.page_size) * p.vc_s;
+      uint4 rows[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int key = k0 + u;
+        const bool sees = key >= from && key < to && (p.mask == nullptr || mask[(key - run.seq.have) * p.mask_j] != 0);
+        rows[u] = sees ? *reinterpret_cast<const uint4*>(at + u * p.vc_s) : make_uint4(0u, 0u, 0u, 0u);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const uint32_t w[4] = {rows[u].x, rows[u].y, rows[u].z, rows[u].w};
+        uint32_t bad[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bad[i] = w[i] & ~finite_halves<BF16>(w[i]);
+        if ((bad[0] | bad[1] | bad[2] | bad[3]) == 0u) continue;
+        all_nan = true;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          sum[2 * i] += half_to_float<BF16>(static_cast<uint16_t>(bad[i] & 0xffffu));
+          sum[2 * i + 1] += half_to_float<BF16>(static_cast<uint16_t>(bad[i] >> 16));
+          all_nan = all_nan && sum[2 * i] != sum[2 * i] && sum[2 * i + 1] != sum[2 * i + 1];
+        }
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (sum[e] == 0.f) continue;
+      if (whole) {
+        const float y = half_to_float<BF16>(o_row[c0 + e]) + sum[e];
+        if constexpr (BF16) reinterpret_cast<__nv_bfloat16*>(o_row)[c0 + e] = __float2bfloat16_rn(y);
+        else reinterpret_cast<__half*>(o_row)[c0 + e] = __float2half_rn(y);
+      } else {
+        acc[static_cast<int64_t>((c0 + e) / 4) * p.tile_rows * 4 + (c0 + e) % 4] += sum[e];
+      }
+    }
   }
 }
 
@@ -722,9 +744,9 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           give_up(96, j);
           break;
         }
-        // Row `row` of the tile's V is cleared where no token lies, and where a token of the step that
-        // some query may not see is not finite (added by hand in the epilogue).  After the softmax
-        // of the first half, so that V has had that long to come.  S_FULL said that the P V two
+        // Row `row` of the tile's V is cleared where no token lies; in a token of the step that some query
+        // may not see, the values that are not finite are (the epilogue adds them to the rows that see
+        // them).  After the softmax of the first half, so that V has had that long to come.  S_FULL said that the P V two
         // tiles back is done, so V_FULL's phase is this tile's or the one before.
         auto clear_v = [&]() {
           const int vi = tile0 + i, vs = vi % R::kV;
@@ -736,20 +758,24 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           // meet in the same banks)
           const uint32_t v_row = v_smem + vs * R::kTile + row * 128;
           const int key = key0 + row;
-          bool clear = key >= mine[6];                    // the sequence's length
-          if (!clear && key >= have && (p.mask != nullptr || p.tokens > 1)) {
-#pragma unroll 2
-            for (int c = 0; c < D / 8; ++c) {
-              uint32_t y[4];
-              ld_shared_v4(v_row + (c / 8) * kBoxBytes + ((c ^ row) & 7) * 16, y);
-              clear = clear || word_not_finite<BF16>(y[0]) || word_not_finite<BF16>(y[1]) ||
-                      word_not_finite<BF16>(y[2]) || word_not_finite<BF16>(y[3]);
-            }
-            if (clear) bad_draft[runs & 1] = runs;
-          }
-          if (clear) {
+          if (key >= mine[6]) {                           // the sequence's length
 #pragma unroll 2
             for (int c = 0; c < D / 8; ++c) st_shared_v4(v_row + (c / 8) * kBoxBytes + ((c ^ row) & 7) * 16, 0u, 0u, 0u, 0u);
+          } else if (key >= have && (p.mask != nullptr || p.tokens > 1)) {
+            bool bad = false;
+#pragma unroll 2
+            for (int c = 0; c < D / 8; ++c) {
+              const uint32_t at = v_row + (c / 8) * kBoxBytes + ((c ^ row) & 7) * 16;
+              uint32_t y[4], keep[4];
+              ld_shared_v4(at, y);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) keep[i] = finite_halves<BF16>(y[i]);
+              if ((keep[0] & keep[1] & keep[2] & keep[3]) != 0xffffffffu) {
+                st_shared_v4(at, y[0] & keep[0], y[1] & keep[1], y[2] & keep[2], y[3] & keep[3]);
+                bad = true;
+              }
+            }
+            if (bad) bad_draft[runs & 1] = runs;
           }
           fence_proxy_async_smem();
           __syncwarp();
@@ -951,7 +977,6 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
       const int tile_row = QUAD ? quarter * (p.tile_rows / 4) + lane : (PAIR ? x * kPaBM : 0) + row;
       const float inv_l = softmax_factor(m_used, l);
       const bool by_hand = edges && bad_draft[runs & 1] == runs;
-      const bool to_out = whole && !by_hand;
       uint16_t* o_row = p.out + run.b * p.o_b + at.hq * p.o_h + at.t * p.o_t;
       float4* acc = reinterpret_cast<float4*>(p.ws_acc) + slot * (D / 4) * p.tile_rows + tile_row;
       if (live && !whole) reinterpret_cast<float2*>(p.ws_ml)[slot * p.tile_rows + tile_row] = make_float2(m_used, l);
@@ -972,7 +997,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
               for (int k = 0; k < 32; ++k) o[k] = o[k] * fa + __uint_as_float(y[k]) * fb;
             }
           }
-          if (live && to_out) {
+          if (live && whole) {
             uint32_t pk[16];
 #pragma unroll
             for (int k = 0; k < 16; ++k)
@@ -1000,9 +1025,9 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
           }
           __syncwarp();
         }
-        if (by_hand && live)
-          add_cleared_drafts<D, BF16>(p, run, at.hq, at.t, reinterpret_cast<float*>(acc), m_used, inv_l, whole,
-                                       QUAD ? quarter : -1);
+        // (a sum of NaN makes the row NaN anyway)
+        if (by_hand && live && l == l)
+          add_not_finite<BF16>(p, run, at.t, QUAD ? quarter : -1, whole, o_row, reinterpret_cast<float*>(acc));
         __syncwarp();
       }
       tc_fence_before_sync();
@@ -1271,16 +1296,13 @@ extern "C" int b200k_paged_attention(const b200k_paged_attention_args* a, b200k_
 
   PagedParams p = {};
   p.q = static_cast<const uint16_t*>(a->q);
-  p.k = static_cast<const uint16_t*>(a->k_cache);
   p.v = static_cast<const uint16_t*>(a->v_cache);
   p.out = static_cast<uint16_t*>(a->out);
   p.page_table = a->page_table;
   p.cache_lens = a->cache_lens;
   p.new_lens = a->new_lens;
   p.mask = a->tree_mask;
-  p.q_b = a->q_stride_b; p.q_h = a->q_stride_h; p.q_t = a->q_stride_t;
   p.o_b = a->o_stride_b; p.o_h = a->o_stride_h; p.o_t = a->o_stride_t;
-  p.kc_p = a->kc_stride_p; p.kc_h = a->kc_stride_h; p.kc_s = a->kc_stride_s;
   p.vc_p = a->vc_stride_p; p.vc_h = a->vc_stride_h; p.vc_s = a->vc_stride_s;
   p.mask_b = a->mask_stride_b; p.mask_t = a->mask_stride_t; p.mask_j = a->mask_stride_j;
   p.page_table_stride = a->page_table_stride;
@@ -1320,11 +1342,11 @@ extern "C" int b200k_paged_attention(const b200k_paged_attention_args* a, b200k_
   CUtensorMap tq, tk, tv;
   // the stride of an axis of one entry is never used, but has to be one that a tensor map takes
   const auto bytes = [](int64_t entries, int64_t stride) -> uint64_t { return entries == 1 ? 16 : stride * 2; };
-  if (!encode_tmap_4d(&tq, dt, a->q, a->head_dim, a->heads_q, a->tokens, a->batch, bytes(a->heads_q, p.q_h),
-                      bytes(a->tokens, p.q_t), bytes(a->batch, p.q_b), 64, p.group, p.half_tokens, 1,
+  if (!encode_tmap_4d(&tq, dt, a->q, a->head_dim, a->heads_q, a->tokens, a->batch, bytes(a->heads_q, a->q_stride_h),
+                      bytes(a->tokens, a->q_stride_t), bytes(a->batch, a->q_stride_b), 64, p.group, p.half_tokens, 1,
                       CU_TENSOR_MAP_SWIZZLE_128B) ||
       !encode_tmap_4d(&tk, dt, a->k_cache, a->head_dim, a->page_size, a->heads_kv, a->num_pages,
-                      bytes(a->page_size, p.kc_s), bytes(a->heads_kv, p.kc_h), bytes(a->num_pages, p.kc_p), 64,
+                      bytes(a->page_size, a->kc_stride_s), bytes(a->heads_kv, a->kc_stride_h), bytes(a->num_pages, a->kc_stride_p), 64,
                       p.box_rows, 1, 1, CU_TENSOR_MAP_SWIZZLE_128B) ||
       !encode_tmap_4d(&tv, dt, a->v_cache, a->head_dim, a->page_size, a->heads_kv, a->num_pages,
                       bytes(a->page_size, p.vc_s), bytes(a->heads_kv, p.vc_h), bytes(a->num_pages, p.vc_p), 64,

@@ -149,3 +149,44 @@ def test_a_query_of_infinity(form, device_ok):
     rest = torch.ones_like(got, dtype=torch.bool)
     rest[:, 1, t - 1] = False
     assert torch.equal(got[rest], clean.run()[rest])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_draft_values_that_are_not_finite_change_their_columns_alone(dtype, form, value, device_ok):
+    c, clean = _cache(form, dtype), _cache(form, dtype)
+    b, t = c.q.shape[0], c.q.shape[2]
+    bad = ((1, 5), (t // 2, 33), (t - 1, 5))
+    for i in range(b):
+        for j, column in bad:
+            c.vc[_slot(c, i, int(c.lens[i]) + j)][..., column] = value
+    causal = torch.ones(b, t, t, dtype=torch.bool, device="cuda").tril()
+    for mask in (_tree(b, t, seed=3), None):
+        sees = causal if mask is None else mask
+        where = torch.zeros_like(c.q, dtype=torch.bool)
+        for j, column in bad:
+            where[..., column] |= sees[:, None, :, j]
+        got, want = c.run(tree_mask=mask), clean.run(tree_mask=mask)
+        clean.check(want, mask)
+        assert torch.equal(got[~where], want[~where])
+        assert bool((torch.isnan(got[where]) if math.isnan(value) else got[where] == value).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("columns", [[7], list(range(64))])
+def test_a_chunk_whose_values_are_all_nan(columns, device_ok):
+    # as after a failure in the layer before: the call ends in good time and says NaN
+    b, t, have = 2, 1500, [0, 333]
+    c, clean = (Cache(b, 4, 2, t, 64, torch.bfloat16, 16, have) for _ in range(2))
+    for i in range(b):
+        at = torch.arange(have[i] + 20, have[i] + t, device="cuda")
+        rows = c.vc[c.table[i].long()[at // 16], :, at % 16]
+        rows[..., columns] = math.nan
+        c.vc[c.table[i].long()[at // 16], :, at % 16] = rows
+    got, want = c.run(), clean.run()
+    where = torch.zeros_like(got, dtype=torch.bool)
+    where[:, :, 20:, columns] = True
+    assert torch.equal(torch.isnan(got), where)
+    assert torch.equal(got[~where], want[~where])
