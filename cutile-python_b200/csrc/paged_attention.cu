@@ -1047,6 +1047,44 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
   }
 }
 
+// Four columns of a row, from column c0, with those that are NaN taken from V itself: the sum of the
+// values there that are not finite, over the keys that token t sees.  With a weight above zero each is
+// what it is, and beside them the finite ones do not matter.  Where there is no such value, the
+// NaN stays.
+template <bool BF16>
+__device__ __forceinline__ float4 infinite_values(const PagedParams& p, const SeqInfo& seq, int b, int head, int t, int c0,
+                                               float4 o) {
+  const uint8_t* mask = p.mask + b * p.mask_b + t * p.mask_t;
+  const int* pages = p.page_table + b * p.page_table_stride;
+  const uint16_t* v = p.v + head * p.vc_h + c0;
+  const int to = p.mask == nullptr ? min(seq.len, seq.have + t + 1) : seq.len;
+  float sum[4] = {};
+  bool all_nan = false;
+#pragma unroll 1
+  for (int k0 = 0; k0 < to && !all_nan; k0 += 4) {            // four slots of a page
+    const int entry = k0 / p.page_size, page = pages[entry];
+    if (page < 0 || page >= p.num_pages) continue;
+    const uint16_t* at = v + page * p.vc_p + (k0 - entry * p.page_size) * p.vc_s;
+    uint2 rows[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int key = k0 + u;
+      const bool sees = key < to && (p.mask == nullptr || key < seq.have || mask[(key - seq.have) * p.mask_j] != 0);
+      rows[u] = sees ? *reinterpret_cast<const uint2*>(at + u * p.vc_s) : make_uint2(0u, 0u);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const uint32_t bad[2] = {rows[u].x & ~finite_halves<BF16>(rows[u].x), rows[u].y & ~finite_halves<BF16>(rows[u].y)};
+      if ((bad[0] | bad[1]) == 0u) continue;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum[i] += half_to_float<BF16>(static_cast<uint16_t>(bad[i / 2] >> (16 * (i & 1))));
+      all_nan = sum[0] != sum[0] && sum[1] != sum[1] && sum[2] != sum[2] && sum[3] != sum[3];
+    }
+  }
+  const auto chosen = [](float old, float found) { return old != old && found != 0.f ? found : old; };
+  return make_float4(chosen(o.x, sum[0]), chosen(o.y, sum[1]), chosen(o.z, sum[2]), chosen(o.w, sum[3]));
+}
+
 // Joins the partial states of items that several CTAs share, and clears padding rows.  A thread owns
 // four columns of a row (neighbouring threads neighbouring rows, as the states are stored) and
 // takes every G-th state in range order; its G partners' results meet in shared memory.
@@ -1140,6 +1178,9 @@ paged_attention_join_kernel(const __grid_constant__ PagedParams p) {
         for (int k = 1; k < G; ++k) take(sm_ml[k][e].x, sm_ml[k][e].y, sm_o[k][e]);
       }
     }
+    // quad: the three quarters that have no share of a key multiply its V by zeros, and 0 * inf is NaN
+    if (kStates > 1 && pass == 1 && store && g == 0 && real && l == l && !(o.x + o.y + o.z + o.w == o.x + o.y + o.z + o.w))
+      o = infinite_values<BF16>(p, seq, b, head, t, quad * 4, o);
     const float inv_l = softmax_factor(m, l);
     const uint32_t lo = BF16 ? pack_bf16x2(o.x * inv_l, o.y * inv_l) : pack_f16x2(o.x * inv_l, o.y * inv_l);
     const uint32_t hi = BF16 ? pack_bf16x2(o.z * inv_l, o.w * inv_l) : pack_f16x2(o.z * inv_l, o.w * inv_l);

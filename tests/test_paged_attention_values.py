@@ -190,3 +190,28 @@ def test_a_chunk_whose_values_are_all_nan(columns, device_ok):
     where[:, :, 20:, columns] = True
     assert torch.equal(torch.isnan(got), where)
     assert torch.equal(got[~where], want[~where])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("form", FORMS)
+def test_values_of_earlier_tokens_that_are_not_finite(dtype, form, device_ok):
+    # column 3: inf, 4: -inf, 5: both, 6: NaN and inf, 40: NaN; the last at the last earlier token
+    c = _cache(form, dtype)
+    for i in range(c.q.shape[0]):
+        have = int(c.lens[i])
+        for column, at, value in ((3, 0, math.inf), (4, have // 2, -math.inf), (5, 1, math.inf), (5, have - 2, -math.inf),
+                                  (6, 2, math.nan), (6, 3, math.inf), (40, have - 1, math.nan)):
+            if have > 4:
+                c.vc[_slot(c, i, at)][..., column] = value
+    c.check(c.run())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("b", [2, 60])
+def test_a_decode_step_whose_own_value_is_not_finite(b, value, device_ok):
+    c = Cache(b, 4, 1, 1, 64, torch.bfloat16, 16, [3 * i for i in range(b)])
+    for i in range(b):
+        c.vc[_slot(c, i, 3 * i)][..., i % 64] = value
+    c.check(c.run())
