@@ -380,20 +380,21 @@ class LayoutPlans:
         return self.native.call(tensors, scalars)
 
     def add(self, tensors: tuple, scalars: tuple, args, inputs, outputs=(), workspace: str | None = None,
-            returns=()) -> None:
-        """``args``: every field but the pointers.  ``inputs``: (field, index into tensors) of those
-        that are not None; ``outputs``: (field, index of the tensor whose shape and type it has);
-        ``workspace``: the pointer field of ``args.workspace_bytes`` of scratch; ``returns``: the
-        number of an output, -1 - i for tensors[i], or None."""
+            returns=()):
+        """Remembers a checked call, makes it and gives its results.  ``args``: every field but the
+        pointers.  ``inputs``: (field, index into tensors) of those that are not None; ``outputs``:
+        (field, index of the tensor whose shape and type it has); ``workspace``: the pointer field of
+        ``args.workspace_bytes`` of scratch; ``returns``: the number of an output, -1 - i for
+        tensors[i], or None."""
         self._bind()
 
         def offset(field):
             return getattr(self.struct, field).offset
 
-        self.native.add(tensors, scalars, bytes(args),
-                        tuple((offset(f), i) for f, i in inputs if tensors[i] is not None),
-                        tuple((offset(f), i) for f, i in outputs), -1 if workspace is None else offset(workspace),
-                        0 if workspace is None else args.workspace_bytes, tuple(returns))
+        return self.native.add(
+            tensors, scalars, bytes(args), tuple((offset(f), i) for f, i in inputs if tensors[i] is not None),
+            tuple((offset(f), i) for f, i in outputs), -1 if workspace is None else offset(workspace),
+            0 if workspace is None else args.workspace_bytes, tuple(returns))
 
 
 def device_status() -> tuple[int, int]:

@@ -91,13 +91,12 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
                                eps=float(eps), interleaved=bool(interleaved), q_out=q_out)
     scalars = float(eps), bool(interleaved)
     own_out = q is not None and q_out is None
-    _APPEND.add(tensors, scalars, a,
-                inputs=(("k", 0), ("v", 1), ("q", 2), ("k_cache", 3), ("v_cache", 4), ("page_table", 5),
-                        ("cache_lens", 6), ("cos", 7), ("sin", 8), ("q_weight", 9), ("k_weight", 10),
-                        ("positions", 11), ("new_lens", 12), ("q_out", 13)),
-                outputs=(("q_out", 2),) if own_out else (),
-                returns=(0 if own_out else (None if q is None else -14),))
-    return _APPEND.call(tensors, scalars)
+    return _APPEND.add(tensors, scalars, a,
+                       inputs=(("k", 0), ("v", 1), ("q", 2), ("k_cache", 3), ("v_cache", 4), ("page_table", 5),
+                               ("cache_lens", 6), ("cos", 7), ("sin", 8), ("q_weight", 9), ("k_weight", 10),
+                               ("positions", 11), ("new_lens", 12), ("q_out", 13)),
+                       outputs=(("q_out", 2),) if own_out else (),
+                       returns=(0 if own_out else (None if q is None else -14),))
 
 
 def _append_args(k, v, k_cache, v_cache, page_table, cache_lens, cos, sin, q, q_weight, k_weight, positions,
@@ -183,12 +182,11 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     scalars = (qk_scale,)
     with torch.cuda.device(q.device):
         a.workspace_bytes = _lib.lib().b200k_paged_attention_workspace_bytes(ctypes.byref(a))
-    _ATTENTION.add(tensors, scalars, a,
-                   inputs=(("q", 0), ("k_cache", 1), ("v_cache", 2), ("page_table", 3), ("cache_lens", 4),
-                           ("new_lens", 5), ("tree_mask", 6), ("out", 7)),
-                   outputs=(("out", 0),) if out is None else (), workspace="workspace",
-                   returns=(0 if out is None else -8,))
-    return _ATTENTION.call(tensors, scalars)
+    return _ATTENTION.add(tensors, scalars, a,
+                          inputs=(("q", 0), ("k_cache", 1), ("v_cache", 2), ("page_table", 3), ("cache_lens", 4),
+                                  ("new_lens", 5), ("tree_mask", 6), ("out", 7)),
+                          outputs=(("out", 0),) if out is None else (), workspace="workspace",
+                          returns=(0 if out is None else -8,))
 
 
 def _attention_args(q, k_cache, v_cache, page_table, cache_lens, new_lens, tree_mask, qk_scale, out):

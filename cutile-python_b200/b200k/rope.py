@@ -188,12 +188,11 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor,
     scalars = float(eps), bool(interleaved)
     outputs = [f for f in (("q_out", 0) if q_out is None else None, ("k_out", 1) if k_out is None else None) if f]
     numbers = iter(range(2))
-    _FORWARD.add(tensors, scalars, a,
-                 inputs=(("q", 0), ("k", 1), ("q_weight", 2), ("k_weight", 3), ("cos", 4), ("sin", 5),
-                         ("positions", 6), ("q_out", 7), ("k_out", 8)),
-                 outputs=outputs,
-                 returns=(next(numbers) if q_out is None else -8, next(numbers) if k_out is None else -9))
-    return _FORWARD.call(tensors, scalars)
+    return _FORWARD.add(tensors, scalars, a,
+                        inputs=(("q", 0), ("k", 1), ("q_weight", 2), ("k_weight", 3), ("cos", 4), ("sin", 5),
+                                ("positions", 6), ("q_out", 7), ("k_out", 8)),
+                        outputs=outputs,
+                        returns=(next(numbers) if q_out is None else -8, next(numbers) if k_out is None else -9))
 
 
 def qk_norm_rope_backward(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
@@ -232,8 +231,7 @@ def qk_norm_rope_backward(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k
         returns.append(None if tensors[i] is None else len(outputs))
         if tensors[i] is not None:
             outputs.append((field, i))
-    _BACKWARD.add(tensors, scalars, a,
-                  inputs=(("dq_out", 0), ("dk_out", 1), ("q", 2), ("k", 3), ("q_weight", 4), ("k_weight", 5),
-                          ("cos", 6), ("sin", 7), ("positions", 8)),
-                  outputs=outputs, workspace="workspace", returns=returns)
-    return _BACKWARD.call(tensors, scalars)
+    return _BACKWARD.add(tensors, scalars, a,
+                         inputs=(("dq_out", 0), ("dk_out", 1), ("q", 2), ("k", 3), ("q_weight", 4), ("k_weight", 5),
+                                 ("cos", 6), ("sin", 7), ("positions", 8)),
+                         outputs=outputs, workspace="workspace", returns=returns)

@@ -21,6 +21,7 @@
 #include <c10/cuda/CUDAStream.h>
 
 #include <cstring>
+#include <deque>
 #include <memory>
 #include <string>
 #include <unordered_map>
@@ -29,7 +30,7 @@
 
 namespace {
 
-constexpr size_t kMaxPlans = 1024;        // the table is emptied when full
+constexpr size_t kMaxPlans = 1024;        // beyond, a new one takes the oldest's place
 constexpr Py_ssize_t kMaxTensors = 24;
 constexpr size_t kMaxArgBytes = 1024;
 
@@ -45,11 +46,26 @@ struct Plan {
   static constexpr int kNone = -1000;
 };
 
+// Plans by key, and the keys in the order they came; a full table drops its oldest.
+struct Table {
+  std::unordered_map<std::string, std::shared_ptr<const Plan>> plans;
+  std::deque<const std::string*> order;               // (a map's keys stay where they are)
+
+  void put(const std::string& key, std::shared_ptr<const Plan> plan) {
+    const auto [at, added] = plans.insert_or_assign(key, std::move(plan));
+    if (!added) return;
+    order.push_back(&at->first);
+    if (plans.size() <= kMaxPlans) return;
+    plans.erase(plans.find(*order.front()));
+    order.pop_front();
+  }
+};
+
 struct Plans {
   PyObject_HEAD
   EntryPoint entry;
   PyObject* check;                                    // raises the error of a negative status
-  std::unordered_map<std::string, std::shared_ptr<const Plan>>* table;
+  Table* table;
 };
 
 struct Call {
@@ -111,7 +127,7 @@ int plans_init(PyObject* self_, PyObject* args, PyObject*) {
   self->entry = reinterpret_cast<EntryPoint>(static_cast<uintptr_t>(address));
   Py_INCREF(check);
   Py_XSETREF(self->check, check);
-  if (self->table == nullptr) self->table = new std::unordered_map<std::string, std::shared_ptr<const Plan>>();
+  if (self->table == nullptr) self->table = new Table();
   return 0;
 }
 
@@ -135,7 +151,84 @@ bool read_pairs(PyObject* seq, Py_ssize_t tensors, size_t arg_bytes, std::vector
   return true;
 }
 
-// add(tensors, scalars, args, inputs, outputs, workspace_offset, workspace_bytes, returns)
+// Runs a plan: makes its outputs and workspace, sets the pointers in a copy of the struct, calls the
+// entry point.  The caller holds `plan`: another thread may drop it from the table meanwhile.
+PyObject* launch(const Plans* self, const Plan& plan, const Call& call, PyObject* tensors) {
+  alignas(16) char args[kMaxArgBytes];
+  std::memcpy(args, plan.args.data(), plan.args.size());
+  const auto set = [&args](int offset, const void* pointer) { std::memcpy(args + offset, &pointer, sizeof(pointer)); };
+  for (const auto& [offset, index] : plan.inputs) set(offset, call.tensor[index]->data_ptr());
+  const at::Device device = call.tensor[0]->device();
+  int code;
+  std::vector<at::Tensor> outputs;
+  {
+    const c10::cuda::CUDAGuard guard(device);
+    outputs.reserve(plan.outputs.size());
+    for (const auto& [offset, index] : plan.outputs) {
+      const at::Tensor& like = *call.tensor[index];
+      outputs.push_back(at::empty(like.sizes(), at::TensorOptions().dtype(like.scalar_type()).device(device)));
+      set(offset, outputs.back().data_ptr());
+    }
+    // made per call: calls on other streams and other captured graphs have their own
+    at::Tensor workspace;
+    if (plan.workspace_offset >= 0 && plan.workspace_bytes > 0) {
+      workspace = at::empty({plan.workspace_bytes}, at::TensorOptions().dtype(at::kByte).device(device));
+      set(plan.workspace_offset, workspace.data_ptr());
+    }
+    void* stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
+    Py_BEGIN_ALLOW_THREADS
+    code = self->entry(args, stream);
+    Py_END_ALLOW_THREADS
+  }
+  if (code < 0) {
+    PyObject* raised = PyObject_CallFunction(self->check, "i", code);
+    if (raised != nullptr) {
+      Py_DECREF(raised);
+      PyErr_Format(PyExc_RuntimeError, "entry point returned %d", code);
+    }
+    return nullptr;
+  }
+  const auto result = [&](int v) -> PyObject* {
+    if (v == Plan::kNone) Py_RETURN_NONE;
+    if (v >= 0) return THPVariable_Wrap(outputs[v]);
+    return Py_NewRef(PyTuple_GET_ITEM(tensors, -1 - v));
+  };
+  if (plan.returns.size() == 1) return result(plan.returns[0]);
+  PyObject* tuple = PyTuple_New(static_cast<Py_ssize_t>(plan.returns.size()));
+  if (tuple == nullptr) return nullptr;
+  for (size_t i = 0; i < plan.returns.size(); ++i) {
+    PyObject* o = result(plan.returns[i]);
+    if (o == nullptr) {
+      Py_DECREF(tuple);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(tuple, static_cast<Py_ssize_t>(i), o);
+  }
+  return tuple;
+}
+
+// The error that the C++ exception being handled becomes.
+PyObject* raise_current() {
+  try {
+    throw;
+  } catch (const c10::OutOfMemoryError& e) {
+    PyObject* torch = PyImport_ImportModule("torch");
+    PyObject* type = torch == nullptr ? nullptr : PyObject_GetAttrString(torch, "OutOfMemoryError");
+    Py_XDECREF(torch);
+    if (type != nullptr) {
+      PyErr_SetString(type, e.what());
+      Py_DECREF(type);
+    }
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+  } catch (...) {
+    PyErr_SetString(PyExc_RuntimeError, "unknown C++ exception");
+  }
+  return nullptr;
+}
+
+// add(tensors, scalars, args, inputs, outputs, workspace_offset, workspace_bytes, returns): remembers the
+// call and makes it.  One step, so that no other thread's plans come between.
 PyObject* plans_add(PyObject* self_, PyObject* args) try {
   auto* self = reinterpret_cast<Plans*>(self_);
   if (self->table == nullptr) {
@@ -151,8 +244,8 @@ PyObject* plans_add(PyObject* self_, PyObject* args) try {
                         &workspace, &returns))
     return nullptr;
   Call call;
-  bool ok = read_call(tensors, scalars, call) && size > 0 && static_cast<size_t>(size) <= kMaxArgBytes &&
-            read_pairs(inputs, call.count, size, plan.inputs) && read_pairs(outputs, call.count, size, plan.outputs) &&
+  bool ok = read_call(tensors, scalars, call) && call.count > 0 && call.tensor[0] != nullptr && size > 0 &&
+            static_cast<size_t>(size) <= kMaxArgBytes && read_pairs(inputs, call.count, size, plan.inputs) && read_pairs(outputs, call.count, size, plan.outputs) &&
             workspace >= 0 && (plan.workspace_offset < 0 || plan.workspace_offset + static_cast<Py_ssize_t>(sizeof(void*)) <= size) &&
             PyTuple_Check(returns);
   for (const auto& [offset, index] : plan.inputs) ok = ok && call.tensor[index] != nullptr;
@@ -173,102 +266,38 @@ PyObject* plans_add(PyObject* self_, PyObject* args) try {
   }
   plan.args.assign(bytes, size);
   plan.workspace_bytes = workspace;
-  if (self->table->size() >= kMaxPlans) self->table->clear();
-  (*self->table)[call.key] = std::make_shared<const Plan>(std::move(plan));
-  Py_RETURN_NONE;
-} catch (const std::exception& e) {
-  PyErr_SetString(PyExc_RuntimeError, e.what());
-  return nullptr;
+  const auto kept = std::make_shared<const Plan>(std::move(plan));
+  self->table->put(call.key, kept);
+  return launch(self, *kept, call, tensors);
+} catch (...) {
+  return raise_current();
 }
 
 // call(tensors, scalars): the outputs, or NotImplemented where these layouts have no plan
-PyObject* plans_call(PyObject* self_, PyObject* const* argv, Py_ssize_t argc) {
+PyObject* plans_call(PyObject* self_, PyObject* const* argv, Py_ssize_t argc) try {
   auto* self = reinterpret_cast<Plans*>(self_);
   if (argc != 2 || self->table == nullptr) {
     PyErr_SetString(PyExc_TypeError, "call(tensors, scalars) of a Plans with an entry point");
     return nullptr;
   }
-  try {
-    Call call;
-    if (!read_call(argv[0], argv[1], call)) Py_RETURN_NOTIMPLEMENTED;
-    const auto found = self->table->find(call.key);
-    if (found == self->table->end()) Py_RETURN_NOTIMPLEMENTED;
-    // held: another thread may empty the table while this one launches
-    const std::shared_ptr<const Plan> held = found->second;
-    const Plan& plan = *held;
-    alignas(16) char args[kMaxArgBytes];
-    std::memcpy(args, plan.args.data(), plan.args.size());
-    const auto set = [&args](int offset, const void* pointer) { std::memcpy(args + offset, &pointer, sizeof(pointer)); };
-    for (const auto& [offset, index] : plan.inputs) set(offset, call.tensor[index]->data_ptr());
-    const at::Device device = call.tensor[0]->device();
-    int code;
-    std::vector<at::Tensor> outputs;
-    {
-      const c10::cuda::CUDAGuard guard(device);
-      outputs.reserve(plan.outputs.size());
-      for (const auto& [offset, index] : plan.outputs) {
-        const at::Tensor& like = *call.tensor[index];
-        outputs.push_back(at::empty(like.sizes(), at::TensorOptions().dtype(like.scalar_type()).device(device)));
-        set(offset, outputs.back().data_ptr());
-      }
-      // made per call: calls on other streams and other captured graphs have their own
-      at::Tensor workspace;
-      if (plan.workspace_offset >= 0 && plan.workspace_bytes > 0) {
-        workspace = at::empty({plan.workspace_bytes}, at::TensorOptions().dtype(at::kByte).device(device));
-        set(plan.workspace_offset, workspace.data_ptr());
-      }
-      void* stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
-      Py_BEGIN_ALLOW_THREADS
-      code = self->entry(args, stream);
-      Py_END_ALLOW_THREADS
-    }
-    if (code < 0) {
-      PyObject* raised = PyObject_CallFunction(self->check, "i", code);
-      if (raised != nullptr) {
-        Py_DECREF(raised);
-        PyErr_Format(PyExc_RuntimeError, "entry point returned %d", code);
-      }
-      return nullptr;
-    }
-    const auto result = [&](int v) -> PyObject* {
-      if (v == Plan::kNone) Py_RETURN_NONE;
-      if (v >= 0) return THPVariable_Wrap(outputs[v]);
-      return Py_NewRef(PyTuple_GET_ITEM(argv[0], -1 - v));
-    };
-    if (plan.returns.size() == 1) return result(plan.returns[0]);
-    PyObject* tuple = PyTuple_New(static_cast<Py_ssize_t>(plan.returns.size()));
-    if (tuple == nullptr) return nullptr;
-    for (size_t i = 0; i < plan.returns.size(); ++i) {
-      PyObject* o = result(plan.returns[i]);
-      if (o == nullptr) {
-        Py_DECREF(tuple);
-        return nullptr;
-      }
-      PyTuple_SET_ITEM(tuple, static_cast<Py_ssize_t>(i), o);
-    }
-    return tuple;
-  } catch (const c10::OutOfMemoryError& e) {
-    PyObject* torch = PyImport_ImportModule("torch");
-    PyObject* type = torch == nullptr ? nullptr : PyObject_GetAttrString(torch, "OutOfMemoryError");
-    Py_XDECREF(torch);
-    if (type != nullptr) {
-      PyErr_SetString(type, e.what());
-      Py_DECREF(type);
-    }
-    return nullptr;
-  } catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
-    return nullptr;
-  }
+  Call call;
+  if (!read_call(argv[0], argv[1], call)) Py_RETURN_NOTIMPLEMENTED;
+  const auto found = self->table->plans.find(call.key);
+  if (found == self->table->plans.end()) Py_RETURN_NOTIMPLEMENTED;
+  const std::shared_ptr<const Plan> plan = found->second;
+  return launch(self, *plan, call, argv[0]);
+} catch (...) {
+  return raise_current();
 }
 
 PyObject* plans_size(PyObject* self_, PyObject*) {
   const auto* table = reinterpret_cast<Plans*>(self_)->table;
-  return PyLong_FromSize_t(table == nullptr ? 0 : table->size());
+  return PyLong_FromSize_t(table == nullptr ? 0 : table->plans.size());
 }
 
 PyMethodDef plans_methods[] = {
-    {"add", plans_add, METH_VARARGS, "add(tensors, scalars, args, inputs, outputs, workspace_offset, workspace_bytes, returns)"},
+    {"add", plans_add, METH_VARARGS, "add(tensors, scalars, args, inputs, outputs, workspace_offset, workspace_bytes, returns): "
+     "remembers the call and makes it"},
     {"call", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(plans_call)), METH_FASTCALL,
      "call(tensors, scalars): the call's results, NotImplemented for layouts without a plan"},
     {"size", plans_size, METH_NOARGS, "remembered plans"},

@@ -93,3 +93,38 @@ def test_the_table_is_emptied_when_full(device_ok):
         out = b200k.qk_norm_rope(*args, eps=1e-6 * (i + 1))
     assert rope._FORWARD.native.size() <= 1024
     assert torch.equal(out[0], b200k.qk_norm_rope(*args, eps=1e-6 * 1030)[0])
+
+
+@pytest.mark.gpu
+def test_a_new_layout_is_called_although_others_fill_the_table(device_ok, monkeypatch):
+    # what another thread may do between a call's checks and the call
+    add, args = _lib.LayoutPlans.add, _inputs(t=9)
+    want = b200k.qk_norm_rope(*args, eps=1e-6)
+
+    def add_and_fill(self, tensors, scalars, *rest, **kw):
+        out = add(self, tensors, scalars, *rest, **kw)
+        for i in range(1100):
+            add(self, tensors, (2.0 + i, False), *rest, **kw)
+        return out
+
+    monkeypatch.setattr(_lib.LayoutPlans, "add", add_and_fill)
+    args = [x.clone() for x in args]
+    got = b200k.qk_norm_rope(args[0][:, :, :8], args[1][:, :, :8], *args[2:])
+    assert all(torch.equal(g, w[:, :, :8]) for g, w in zip(got, want))
+    assert rope._FORWARD.native.size() == 1024
+
+
+@pytest.mark.gpu
+def test_a_full_table_loses_one_plan_for_a_new_one(device_ok, monkeypatch):
+    args, checked = _inputs(b=1, t=4), []
+    check = rope._check_rows
+    monkeypatch.setattr(rope, "_check_rows", lambda *a: (checked.append(1), check(*a)))
+    for i in range(1100):                         # more than the table holds
+        b200k.qk_norm_rope(*args, eps=1e-5 * (i + 1))
+    b200k.qk_norm_rope(*args, eps=3.0)
+    checked.clear()
+    for i in range(100, 1100):
+        b200k.qk_norm_rope(*args, eps=1e-5 * (i + 1))
+    assert not checked and rope._FORWARD.native.size() == 1024
+    b200k.qk_norm_rope(*args, eps=1e-5)           # the oldest has gone
+    assert checked
