@@ -4,6 +4,7 @@
 #include <stdio.h>
 #include <string.h>
 #include <mutex>
+#include <new>
 #include <unordered_map>
 
 #include "host.h"
@@ -128,9 +129,12 @@ static bool encode_tmap(CUtensorMap* out, CUtensorMapDataType dtype, int rank, c
   }
   if (!encode_tmap_uncached(out, dtype, rank, base, dims, strides_bytes, box, swizzle)) return false;
   std::lock_guard<std::mutex> lock(g_tmap_mutex);
-  if (g_tmap_cache.size() >= kTmapCacheEntries) g_tmap_cache.clear();
-  g_tmap_cache.emplace(key, *out);
   ++g_tmap_misses;
+  if (g_tmap_cache.size() >= kTmapCacheEntries) g_tmap_cache.clear();
+  try {
+    g_tmap_cache.emplace(key, *out);
+  } catch (const std::bad_alloc&) {   // the map serves this call; no exception leaves a C entry point
+  }
   return true;
 }
 

@@ -151,6 +151,12 @@ bool read_pairs(PyObject* seq, Py_ssize_t tensors, size_t arg_bytes, std::vector
   return true;
 }
 
+// The interpreter's lock, released while this lives: taken back also where an exception leaves.
+struct ReleasedLock {
+  PyThreadState* const state = PyEval_SaveThread();
+  ~ReleasedLock() { PyEval_RestoreThread(state); }
+};
+
 // Runs a plan: makes its outputs and workspace, sets the pointers in a copy of the struct, calls the
 // entry point.  The caller holds `plan`: another thread may drop it from the table meanwhile.
 PyObject* launch(const Plans* self, const Plan& plan, const Call& call, PyObject* tensors) {
@@ -176,9 +182,8 @@ PyObject* launch(const Plans* self, const Plan& plan, const Call& call, PyObject
       set(plan.workspace_offset, workspace.data_ptr());
     }
     void* stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
-    Py_BEGIN_ALLOW_THREADS
+    const ReleasedLock released;
     code = self->entry(args, stream);
-    Py_END_ALLOW_THREADS
   }
   if (code < 0) {
     PyObject* raised = PyObject_CallFunction(self->check, "i", code);

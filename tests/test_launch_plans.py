@@ -1,5 +1,8 @@
 """The host module that remembers checked calls by the layouts of their tensors: what makes a new
 plan and what does not, and that calls share nothing but plans."""
+import ctypes
+import shutil
+import subprocess
 import threading
 
 import pytest
@@ -128,3 +131,24 @@ def test_a_full_table_loses_one_plan_for_a_new_one(device_ok, monkeypatch):
     assert not checked and rope._FORWARD.native.size() == 1024
     b200k.qk_norm_rope(*args, eps=1e-5)           # the oldest has gone
     assert checked
+
+
+@pytest.mark.gpu
+def test_an_exception_in_an_entry_point_becomes_an_error(device_ok, tmp_path):
+    # the interpreter's lock is not held in there, and is again where the error is raised
+    cxx = shutil.which("g++")
+    if cxx is None:
+        pytest.skip("no C++ compiler")
+    (tmp_path / "throws.cpp").write_text(
+        '#include <stdexcept>\nextern "C" int throws(const void*, void*) { throw std::runtime_error("no room"); }\n')
+    subprocess.run([cxx, "-shared", "-fPIC", "-o", tmp_path / "throws.so", tmp_path / "throws.cpp"], check=True)
+    entry = ctypes.cast(ctypes.CDLL(tmp_path / "throws.so").throws, ctypes.c_void_p).value
+    x = torch.ones(4, device="cuda")
+    rope._FORWARD._bind()
+    plans = type(rope._FORWARD.native)(entry, _lib.check)
+    with pytest.raises(RuntimeError, match="no room"):
+        plans.add((x,), (), b"x" * 16, ((0, 0),), ((8, 0),), -1, 0, (0,))
+    for _ in range(3):
+        with pytest.raises(RuntimeError, match="no room"):
+            plans.call((x,), ())
+    assert plans.size() == 1
