@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -35,6 +36,10 @@ def check_no_grad(name: str, instead: str, *tensors) -> None:
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise ValueError(f"{name} is not recorded by autograd: call it under torch.no_grad(){instead}")
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError(f"{name} is not recorded by autograd: it passes no tangents on")
 
 
 def check_out(t: torch.Tensor, like: torch.Tensor, name: str) -> torch.Tensor:

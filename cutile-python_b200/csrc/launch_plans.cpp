@@ -76,7 +76,8 @@ struct Call {
 
 template <typename T> void put(std::string& key, T v) { key.append(reinterpret_cast<const char*>(&v), sizeof(v)); }
 
-// False where a call can have no plan (an argument that is no strided CUDA tensor, an odd scalar):
+// False where a call can have no plan (an argument that is no strided CUDA tensor or has a tangent, an
+// odd scalar):
 // the wrapper's checks say what is wrong with it.
 bool read_call(PyObject* tensors, PyObject* scalars, Call& c) {
   if (!PyTuple_Check(tensors) || !PyTuple_Check(scalars) || PyTuple_GET_SIZE(tensors) > kMaxTensors) return false;
@@ -91,7 +92,7 @@ bool read_call(PyObject* tensors, PyObject* scalars, Call& c) {
     }
     if (!THPVariable_Check(o)) return false;
     const at::Tensor& t = THPVariable_Unpack(o);
-    if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided) return false;
+    if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || t._fw_grad(0).defined()) return false;
     c.tensor[i] = &t;
     put<int8_t>(c.key, static_cast<int8_t>(t.dim()));
     put<int8_t>(c.key, static_cast<int8_t>(t.scalar_type()));

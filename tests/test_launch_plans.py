@@ -65,6 +65,37 @@ def test_a_remembered_layout_still_refuses_gradients(device_ok):
         b200k.qk_norm_rope(args[0].clone().requires_grad_(), *args[1:])
 
 
+def test_tangents_are_refused():
+    x = torch.ones(3)
+    rope.check_no_grad("f", "", x, None)
+    with torch.autograd.forward_ad.dual_level():
+        rope.check_no_grad("f", "", x, None)
+        with pytest.raises(ValueError, match="autograd"):
+            rope.check_no_grad("f", "", x, torch.autograd.forward_ad.make_dual(x, x))
+
+
+@pytest.mark.gpu
+def test_a_remembered_layout_still_refuses_tangents(device_ok):
+    args = _inputs()
+    want = b200k.qk_norm_rope(*args)
+    grads = b200k.qk_norm_rope_backward(*want, *args)
+    cache = torch.zeros(3, 2, 16, 64, device="cuda").bfloat16()
+    table, lens = (torch.zeros(shape, dtype=torch.int32, device="cuda") for shape in ((2, 1), (2,)))
+    b200k.paged_kv_append(args[1], args[1], cache, cache.clone(), table, lens)
+    b200k.paged_attention(args[0], cache, cache, table, lens)
+    with torch.autograd.forward_ad.dual_level():
+        dual = [torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)) for x in args[:2]]
+        assert all(torch.equal(g, w) for g, w in zip(b200k.qk_norm_rope(*args), want))
+        for call in (lambda: b200k.qk_norm_rope(args[0], dual[1], *args[2:]),
+                     lambda: b200k.qk_norm_rope_backward(want[0], want[1], dual[0], *args[1:]),
+                     lambda: b200k.paged_kv_append(dual[1], args[1], cache, cache.clone(), table, lens),
+                     lambda: b200k.paged_attention(dual[0], cache, cache, table, lens)):
+            with pytest.raises(ValueError, match="autograd"):
+                call()
+    again = b200k.qk_norm_rope_backward(*want, *args)
+    assert all(torch.equal(g, w) for g, w in zip(again, grads))
+
+
 @pytest.mark.gpu
 def test_threads_and_streams_share_plans_only(device_ok):
     cases = [_inputs(t=5 + i % 3) for i in range(6)]
