@@ -114,7 +114,7 @@ def _append_args(k, v, k_cache, v_cache, page_table, cache_lens, cos, sin, q, q_
     device = k.device
     if dim % 8 or not 0 < dim <= 256:
         raise ValueError("the head dimension must be a multiple of 8 up to 256")
-    check_no_grad("paged_kv_append", "", k, v, q, q_weight, k_weight, k_cache, v_cache)
+    check_no_grad("paged_kv_append", "", k, v, q, q_weight, k_weight, cos, sin, k_cache, v_cache, q_out)
     _check_cache(k_cache, v_cache, page_table, cache_lens, new_lens, batch, heads, dim, k.dtype, device)
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin come together")
@@ -199,7 +199,7 @@ def _attention_args(q, k_cache, v_cache, page_table, cache_lens, new_lens, tree_
         raise TypeError("paged_attention supports float16 and bfloat16")
     batch, heads, tokens, dim = q.shape
     device = q.device
-    check_no_grad("paged_attention", "", q, k_cache, v_cache)
+    check_no_grad("paged_attention", "", q, k_cache, v_cache, out)
     heads_kv = k_cache.shape[1] if k_cache.ndim == 4 else 0
     _check_cache(k_cache, v_cache, page_table, cache_lens, new_lens, batch, heads_kv, dim, q.dtype, device)
     if heads_kv == 0 or heads % heads_kv:

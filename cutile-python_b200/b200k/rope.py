@@ -178,7 +178,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor,
     if done is not NotImplemented:
         return done
     _check_rows(q, k)
-    check_no_grad("qk_norm_rope", " and take gradients from qk_norm_rope_backward", q, k, q_weight, k_weight)
+    check_no_grad("qk_norm_rope", " and take gradients from qk_norm_rope_backward", q, k, q_weight, k_weight,
+                  cos, sin, q_out, k_out)
     if q_out is not None:
         check_out(q_out, q, "q_out")
     if k_out is not None:
@@ -214,7 +215,7 @@ def qk_norm_rope_backward(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k
     if done is not NotImplemented:
         return done
     _check_rows(q, k)
-    check_no_grad("qk_norm_rope_backward", "", dq, dk, q, k, q_weight, k_weight)
+    check_no_grad("qk_norm_rope_backward", "", dq, dk, q, k, q_weight, k_weight, cos, sin)
     for g, x, name in ((dq, q, "dq"), (dk, k, "dk")):
         if g.shape != x.shape or g.dtype != x.dtype or g.device != x.device:
             raise ValueError(f"{name} must have the shape, dtype and device of {name[1]}")

@@ -97,6 +97,28 @@ def test_a_remembered_layout_still_refuses_tangents(device_ok):
 
 
 @pytest.mark.gpu
+def test_gradients_of_tables_and_outputs_are_refused(device_ok):
+    q, k, w, _, cos, sin = args = _inputs()
+    cache = torch.zeros(3, 2, 16, 64, device="cuda").bfloat16()
+    table, lens = (torch.zeros(shape, dtype=torch.int32, device="cuda") for shape in ((2, 1), (2,)))
+
+    def learned(x):
+        return x.clone().requires_grad_()
+
+    for call in (lambda: b200k.qk_norm_rope(q, k, w, w, learned(cos), sin),
+                 lambda: b200k.qk_norm_rope(*args, q_out=learned(q)),
+                 lambda: b200k.qk_norm_rope(*args, k_out=learned(k)),
+                 lambda: b200k.qk_norm_rope_backward(q, k, q, k, w, w, cos, learned(sin)),
+                 lambda: b200k.paged_kv_append(k, k, cache, cache.clone(), table, lens, learned(cos), sin),
+                 lambda: b200k.paged_kv_append(k, k, cache, cache.clone(), table, lens, q=q, q_out=learned(q)),
+                 lambda: b200k.paged_attention(q, cache, cache, table, lens, out=learned(q))):
+        with pytest.raises(ValueError, match="autograd"):
+            call()
+        with torch.no_grad():
+            call()
+
+
+@pytest.mark.gpu
 def test_threads_and_streams_share_plans_only(device_ok):
     cases = [_inputs(t=5 + i % 3) for i in range(6)]
     want = [b200k.qk_norm_rope(*c) for c in cases]
