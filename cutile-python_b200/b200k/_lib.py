@@ -417,7 +417,8 @@ def raise_on_device_error() -> None:
         what = {80: "a position outside the rotation table (token {})",
                 81: "a page of sequence {} outside the page table or the cache"}
         role, detail = (info >> 8) & 0xff, (info >> 16) & 0xffff
-        raise B200KError(code, what.get(role, f"index of kind {role} out of range ({{}})").format(detail))
+        where = f"{detail} or a later one" if detail == 0xffff else detail
+        raise B200KError(code, what.get(role, f"index of kind {role} out of range ({{}})").format(where))
     if code != 0:
         raise B200KError(code, f"device-side wait gave up (role {(info >> 8) & 0xff}, "
                                f"detail {(info >> 16) & 0xffff})")

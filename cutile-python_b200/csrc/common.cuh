@@ -45,11 +45,12 @@ __device__ __forceinline__ void report_status(int* status, int role, int detail)
 }
 
 // An index in device memory that lies outside what it points into: the access is skipped and
-// the status word tells which kind of index (role) and where (detail).  Code 2 instead of a
-// wait's 1, so that the host can tell the two apart.
+// the status word tells which kind of index (role) and where (detail, 65535 for that and all
+// behind it).  Code 2 instead of a wait's 1, so that the host can tell the two apart.
 enum : int { kRolePosition = 80, kRolePage = 81 };
-__device__ __forceinline__ void report_bad_index(int* status, int role, int detail) {
-  if (status != nullptr) atomicCAS(status, 0, 2 | ((role & 0xff) << 8) | ((detail & 0xffff) << 16));
+__device__ __forceinline__ void report_bad_index(int* status, int role, int64_t detail) {
+  const int place = detail < 0xffff ? static_cast<int>(detail) : 0xffff;
+  if (status != nullptr) atomicCAS(status, 0, 2 | ((role & 0xff) << 8) | (place << 16));
 }
 
 // ---------------------------------------------------------------------------

@@ -261,7 +261,7 @@ template <typename T, bool INTER>
 __device__ __forceinline__ void load_angles(const RopeParams& p, int64_t pos, int64_t t, int unit,
                                             const LaneColumns<T>& col, Angles& g) {
   if (pos < 0 || pos >= p.table_rows) {
-    if (unit == 0) report_bad_index(p.status, kRolePosition, static_cast<int>(t));
+    if (unit == 0) report_bad_index(p.status, kRolePosition, t);
     const float nan = __int_as_float(0x7fc00000);
 #pragma unroll
     for (int k = 0; k < 4; ++k) g.c[k] = g.s[k] = g.minus[k] = make_float2(nan, nan);
@@ -379,7 +379,7 @@ qk_rope_kernel(const __grid_constant__ RopeParams p) {
     int64_t page = -1;
     if (entry >= 0 && entry < p.max_pages) page = p.page_table[b * p.page_table_stride + entry];
     if (page < 0 || page >= p.num_pages) {
-      if (unit == 0) report_bad_index(p.status, kRolePage, static_cast<int>(b));
+      if (unit == 0) report_bad_index(p.status, kRolePage, b);
       store = false;
     } else {
       out = page * sd.y_b + (at - entry * p.page_size) * sd.y_t;

@@ -60,7 +60,8 @@ int b200k_sm_count(void);                       /* SMs of the current device, <0
  * in device memory that lies outside what it points into: a position, a page)
  * B200K_INVALID_ARG; *info packs (role << 8 | detail << 16) of the wait that gave up or of
  * the index: role 80 = a position outside the rotation table (detail: token), 81 = a page
- * outside the page table or the cache (detail: sequence). */
+ * outside the page table or the cache (detail: sequence); a detail of 65535 is that or any later
+ * one. */
 int b200k_device_status(int* code, int* info);
 /* The one piece of state the library owns: a mutex-guarded cache of encoded TMA tensor maps
  * keyed by (base pointer, data type, dims, strides, box, swizzle), at most 8192 entries of

@@ -386,3 +386,15 @@ def test_captured_and_on_another_stream(device_ok):
     torch.cuda.synchronize()
     for outs in got:
         assert all(torch.equal(a, w) for a, w in zip(outs, want))
+
+
+@pytest.mark.gpu
+def test_positions_outside_the_table_name_late_tokens_as_such():
+    q = torch.zeros(1, 1, 70001, 16, dtype=torch.float16, device="cuda")
+    cos, sin = b200k.rope_table(70000, 16, device="cuda")
+    b200k.qk_norm_rope(q, q, None, None, cos, sin)                 # token 70000: beyond the 16 bits of its place
+    with pytest.raises(b200k.B200KError, match=r"token 65535 or a later one"):
+        b200k.raise_on_device_error()
+    b200k.qk_norm_rope(q[:, :, :65536], q[:, :, :65536], None, None, cos[:65534], sin[:65534])
+    with pytest.raises(b200k.B200KError, match=r"token (65534\)|65535 or a later one)"):
+        b200k.raise_on_device_error()
