@@ -919,8 +919,8 @@ extern "C" int b200k_paged_kv_append(const b200k_paged_kv_append_args* a, b200k_
   if (rc != B200K_OK) return rc;
   if (a->page_size <= 0 || a->num_pages < 0 || a->max_pages < 0)
     return fail(B200K_INVALID_ARG, "page_size must be positive, page counts not negative");
-  if (p.total_tokens == 0 || a->heads_kv == 0) return B200K_OK;
-  if (!a->k || !a->v || !a->k_cache || !a->v_cache || !a->page_table || !a->cache_lens)
+  if (p.total_tokens == 0) return B200K_OK;
+  if (!a->cache_lens || (a->heads_kv > 0 && (!a->k || !a->v || !a->k_cache || !a->v_cache || !a->page_table)))
     return fail(B200K_INVALID_ARG, "null pointer");
   p.positions = a->positions;
   p.pos_b = a->position_stride_b;
@@ -943,7 +943,7 @@ extern "C" int b200k_paged_kv_append(const b200k_paged_kv_append_args* a, b200k_
     s.rotate = a->rotary_dim > 0;
     s.zero_padding = a->zero_padding;
   }
-  for (int which = 0; which < 2; ++which) {
+  for (int which = 0; which < 2 && a->heads_kv > 0; ++which) {
     RopeSide& s = p.side[p.sides++];
     s.heads = static_cast<int>(a->heads_kv);
     s.paged = 1;
@@ -958,5 +958,6 @@ extern "C" int b200k_paged_kv_append(const b200k_paged_kv_append_args* a, b200k_
       s.y_b = a->vc_stride_p; s.y_h = a->vc_stride_h; s.y_t = a->vc_stride_s;
     }
   }
+  if (p.sides == 0) return B200K_OK;
   return launch_forward(p, a->dtype, static_cast<cudaStream_t>(stream));
 }

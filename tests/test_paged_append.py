@@ -256,3 +256,16 @@ def test_captured_steps_advance(device_ok):
     assert torch.equal(s.lens, lens0 + 2) and torch.equal(s.vc.cpu(), want_v)
     # k: at most one rounding and 32 * 2^-24 of a sum of two magnitudes, values below 16
     assert float((s.kc.cpu().double() - want_k).abs().max()) <= 2.0 ** -11 * 16 + 32 * EPS32 * 32
+
+
+@pytest.mark.gpu
+def test_queries_without_key_value_heads(device_ok):
+    s = Step(2, 4, 2, 6, 64, torch.bfloat16, 16, [12, 90], [6, 2])
+    want = s.append()
+    s.k, s.v, s.kc, s.vc = s.k[:, :0], s.v[:, :0], s.kc[:, :0], s.vc[:, :0]
+    q_out = torch.full_like(want, 7.0)
+    assert s.append(q_out=q_out) is q_out
+    real = s.real[:, None, :, None].expand_as(want)
+    assert torch.equal(q_out[real], want[real]) and bool((q_out[~real] == 7).all())
+    assert torch.equal(s.append(), want)
+    assert s.append(q=None, q_weight=None) is None
