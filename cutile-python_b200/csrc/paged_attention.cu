@@ -1249,9 +1249,11 @@ int check_args(const b200k_paged_attention_args* a) {
   if (a->page_size <= 0 || a->page_size % 8 != 0)
     return fail(B200K_UNSUPPORTED, "page_size must be a positive multiple of 8 (got %d)", a->page_size);
   const int64_t limit = int64_t(1) << 29;   // sums of two such counts fit 32 bits
-  if (a->tokens * a->heads_q > limit || static_cast<int64_t>(a->max_pages) * a->page_size > limit ||
+  const int64_t width = static_cast<int64_t>(a->max_pages) * a->page_size;   // tokens that a sequence's table can name
+  if (a->tokens > limit || a->heads_q > limit || a->tokens * a->heads_q > limit || width > limit ||
       a->num_pages >= limit || a->batch > kPaMaxBatch || a->heads_kv > limit ||
-      a->batch * a->heads_kv * lay_out_rows(a, 1).tiles * ceil_div(static_cast<int64_t>(a->max_pages) * a->page_size, kPaBN) > limit)
+      // key tiles of all items, were every table full: never summed with another such count
+      a->batch * a->heads_kv * lay_out_rows(a, 1).tiles > INT32_MAX / (width > kPaBN ? ceil_div(width, kPaBN) : 1))
     return fail(B200K_UNSUPPORTED, "more rows, pages or sequences than the kernel counts");
   return B200K_OK;
 }

@@ -698,7 +698,9 @@ int b200k_paged_kv_append(const b200k_paged_kv_append_args* args, b200k_stream s
  * table as its end; both are recorded in the status word.
  * Query head h reads key/value head h / (heads_q / heads_kv).  D a multiple of 8 up to 128;
  * page_size a multiple of 8; bases and strides of q and of the caches multiples of 16 bytes; at
- * most 128 query heads per key/value head and 65535 sequences.  Padding rows of out are left as
+ * most 128 query heads per key/value head and 65535 sequences; a table names up to 2^29 tokens, and
+ * batch * heads_kv * row tiles * ceil(max_pages * page_size / 128) stays below 2^31, where a row tile is
+ * up to 128 query rows of a key/value head, or 256 where there are more.  Padding rows of out are left as
  * they are, or become zero with `zero_padding`. */
 typedef struct {
   const void* q;                /* (batch, heads_q, tokens, D) */

@@ -121,6 +121,26 @@ def test_refusals_of_the_entry_point():
     assert call(tokens=0, q=None) == _lib.OK
 
 
+def test_the_limit_of_key_tiles_counts_full_tables():
+    h = _lib.lib()
+
+    def call(**change):
+        a = _lib.PagedAttentionArgs()
+        a.batch, a.tokens, a.heads_q, a.heads_kv, a.head_dim = 512, 2048, 32, 8, 128
+        a.dtype, a.page_size, a.max_pages, a.qk_scale = _lib.BF16, 16, 1 << 16, 0.125
+        a.q = a.k_cache = a.v_cache = a.out = a.page_table = a.cache_lens = 1 << 20
+        for name, value in change.items():
+            setattr(a, name, value)
+        return h.b200k_paged_attention(ctypes.byref(a), None)
+
+    # 512 x 8 items of 32 row tiles, tables of 2^20 tokens: 2^30 (refused for its lack of pages)
+    assert call() == _lib.INVALID_ARG
+    assert call(batch=1023) == _lib.INVALID_ARG
+    assert call(batch=1024) == _lib.UNSUPPORTED                       # 2^31
+    assert call(tokens=1 << 62, heads_q=8) == _lib.UNSUPPORTED        # counts whose product is no 64-bit number
+    assert call(tokens=1 << 14, batch=65535, page_size=8, max_pages=1 << 26) == _lib.UNSUPPORTED
+
+
 def test_refusals_of_the_wrapper():
     q = torch.zeros(1, 2, 3, 64).half()
     cache = torch.zeros(4, 2, 16, 64).half()
@@ -245,6 +265,19 @@ def test_more_items_than_a_grid_has_rows(t, hq, device_ok):
     got = c.run()
     c.check(got)
     assert bool((got.transpose(1, 2)[~c.real] == 0).all())
+
+
+@pytest.mark.gpu
+def test_wide_tables_with_many_row_tiles(device_ok):
+    # 8 x 4 items of 9 row tiles, tables of 2^29 tokens: more than 2^30 key tiles, were they full
+    c = Cache(8, 16, 4, 520, 8, torch.bfloat16, 4096, [0, 3, 900, 77, 128, 2000, 5, 4090])
+    want = c.run()
+    table = torch.zeros(8, 1 << 17, dtype=torch.int32, device="cuda")
+    table[:, :c.table.shape[1]] = c.table
+    c.table = table
+    got = c.run()
+    c.check(got)
+    assert torch.equal(got, want)
 
 
 @pytest.mark.gpu
