@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import argparse
 import concurrent.futures
+import importlib.metadata
 import importlib.util
 import os
 import shutil
@@ -25,6 +26,7 @@ OBJ_DIR = os.path.join(HERE, "build")
 LIB_PATH = os.path.join(HERE, "b200k", "libb200k.so")
 PLANS_SRC = os.path.join(CSRC, "launch_plans.cpp")
 PLANS_PATH = os.path.join(HERE, "b200k", "_plans.so")
+PLANS_STAMP = os.path.join(OBJ_DIR, "_plans.stamp")      # what _plans.so was built with
 
 NVCC_FLAGS = [
     "-std=c++17", "-O3", "-lineinfo",
@@ -69,13 +71,27 @@ def _plans_command(nvcc: str) -> list[str]:
             "-L", os.path.join(torch, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
 
 
+def _plans_stamp(nvcc: str) -> str:
+    """What the host module depends on besides its source: the command, this interpreter and the
+    torch whose classes it uses (they change their layout without changing their path)."""
+    return "\n".join([*_plans_command(nvcc), sys.version, importlib.metadata.version("torch")])
+
+
+def _plans_stale(nvcc: str) -> bool:
+    if _stale(PLANS_PATH, [PLANS_SRC]) or not os.path.exists(PLANS_STAMP):
+        return True
+    with open(PLANS_STAMP) as f:
+        return f.read() != _plans_stamp(nvcc)
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(OBJ_DIR, exist_ok=True)
     nvcc = _nvcc()
     hdrs = _headers()
     jobs = []
     objs = []
-    if force or _stale(PLANS_PATH, [PLANS_SRC]):
+    plans = force or _plans_stale(nvcc)
+    if plans:
         jobs.append(_plans_command(nvcc))
     for src in _sources():
         obj = os.path.join(OBJ_DIR, os.path.basename(src)[:-3] + ".o")
@@ -97,6 +113,9 @@ def build(force: bool = False, verbose: bool = False) -> str:
                     sys.stderr.write(" ".join(cmd) + "\n" + r.stdout + r.stderr)
                 if r.returncode != 0:
                     raise RuntimeError(f"compiling failed: {' '.join(cmd)}")
+    if plans:
+        with open(PLANS_STAMP, "w") as f:
+            f.write(_plans_stamp(nvcc))
     if jobs or force or _stale(LIB_PATH, objs):
         cmd = [nvcc, "-shared", "-o", LIB_PATH, *objs, "-cudart", "static"]
         r = subprocess.run(cmd, capture_output=True, text=True)

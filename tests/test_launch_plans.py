@@ -1,6 +1,8 @@
 """The host module that remembers checked calls by the layouts of their tensors: what makes a new
 plan and what does not, and that calls share nothing but plans."""
 import ctypes
+import importlib.util
+import os
 import shutil
 import subprocess
 import threading
@@ -205,3 +207,29 @@ def test_an_exception_in_an_entry_point_becomes_an_error(device_ok, tmp_path):
         with pytest.raises(RuntimeError, match="no room"):
             plans.call((x,), ())
     assert plans.size() == 1
+
+
+def _build_module():
+    spec = importlib.util.spec_from_file_location("b200k_build", os.path.join(os.path.dirname(b200k.__file__), "..", "build.py"))
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    return module
+
+
+def test_the_host_module_is_built_anew_for_another_torch_or_python(tmp_path, monkeypatch):
+    build = _build_module()
+    monkeypatch.setattr(build, "PLANS_STAMP", str(tmp_path / "stamp"))
+    monkeypatch.setattr(build, "PLANS_PATH", str(tmp_path / "_plans.so"))
+    (tmp_path / "_plans.so").write_text("")
+    assert build._plans_stale("nvcc")                          # built by nobody knows what
+    (tmp_path / "stamp").write_text(build._plans_stamp("nvcc"))
+    assert not build._plans_stale("nvcc")
+    with monkeypatch.context() as m:
+        m.setattr(build.importlib.metadata, "version", lambda name: "0.0")
+        assert build._plans_stale("nvcc")
+    with monkeypatch.context() as m:
+        m.setattr(build.sys, "version", "another")
+        assert build._plans_stale("nvcc")
+    assert not build._plans_stale("nvcc")
+    (tmp_path / "_plans.so").unlink()
+    assert build._plans_stale("nvcc")
