@@ -126,7 +126,7 @@ def aligned_table(cos, sin):
     """The tables themselves, or 16-byte aligned copies of a common layout."""
     if cos is None or sin is None or not cos.numel() or (
             (cos.data_ptr() | sin.data_ptr()) % 16 == 0 and cos.stride() == sin.stride()
-            and cos.stride(-1) == 1 and cos.stride(0) % 4 == 0):
+            and cos.stride(-1) == 1 and cos.stride(0) % 4 == 0 and cos.stride(0) >= cos.shape[1]):
         return cos, sin
     width = -(-cos.shape[1] // 4) * 4                # rows of whole 16-byte units
     return tuple(torch.empty(t.shape[0], width, dtype=t.dtype, device=t.device)[:, :t.shape[1]].copy_(t)

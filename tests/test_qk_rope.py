@@ -398,3 +398,11 @@ def test_positions_outside_the_table_name_late_tokens_as_such():
     b200k.qk_norm_rope(q[:, :, :65536], q[:, :, :65536], None, None, cos[:65534], sin[:65534])
     with pytest.raises(b200k.B200KError, match=r"token (65534\)|65535 or a later one)"):
         b200k.raise_on_device_error()
+
+
+@pytest.mark.gpu
+def test_tables_of_repeated_rows(device_ok):
+    # one row for all positions through a stride of zero, one row alone
+    q, k, qw, kw, cos, sin, pos = _make(2, 4, 2, 6, 64, torch.bfloat16, 64)
+    _check(q, k, qw, kw, cos[7:8].expand(512, 32), sin[7:8].expand(512, 32), pos)
+    _check(q, k, qw, kw, cos[7].expand(1, 32), sin[7].expand(1, 32), torch.zeros_like(pos))
