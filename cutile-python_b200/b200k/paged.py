@@ -72,12 +72,13 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
     ``q_out``, which may be q itself).
 
     ``positions`` (SeqLen,) or (Batch, SeqLen) are the tokens' positions where those are not their
-    places in the cache (drafts of one depth in a tree share a position).  Rows behind
-    new_lens[b] are padding: their cache slots stay as they are, as do their rows of a given
-    ``q_out``; in a q_out made here they are zero.  A token whose page lies outside the table
-    or the cache is not stored, and ``raise_on_device_error()`` names its sequence.  Sequences may
-    share the pages that they only read: of two tokens that a call stores in one slot, either may
-    stay.  Outputs overlap no input, but for q_out = q."""
+    places in the cache (drafts of one depth in a tree share a position); one outside the table
+    makes the rotated values of its rows NaN, in the cache too.  Rows behind new_lens[b] are
+    padding: their cache slots stay as they are, as do their rows of a given ``q_out``; in a q_out
+    made here they are zero.  A token whose page lies outside the table or the cache is not stored.
+    ``raise_on_device_error()`` names the token or the sequence.  Sequences may share the pages that
+    they only read: of two tokens that a call stores in one slot, either may stay.  Outputs overlap
+    no input, but for q_out = q."""
     tensors = (k, v, q, k_cache, v_cache, page_table, cache_lens, cos, sin, q_weight, k_weight, positions, new_lens, q_out)
     scalars = eps, interleaved
     done = _APPEND.call(tensors, scalars)

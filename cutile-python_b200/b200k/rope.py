@@ -171,8 +171,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor,
     A weight of None leaves that norm out (rotation alone).  ``cos`` / ``sin`` are tables by
     position (``rope_table``); ``positions`` is (SeqLen,) or (Batch, SeqLen), None = 0, 1, 2, ...
     Pairs are (i, i + rotary_dim / 2), or neighbours with ``interleaved``.  ``q_out`` / ``k_out``
-    may be q / k themselves and overlap nothing else.  A position outside the table gives NaN rows, and
-    ``raise_on_device_error()`` names it."""
+    may be q / k themselves and overlap nothing else.  A position outside the table makes the rotated
+    values of its rows NaN, and ``raise_on_device_error()`` names it."""
     tensors, scalars = (q, k, q_weight, k_weight, cos, sin, positions, q_out, k_out), (eps, interleaved)
     done = _FORWARD.call(tensors, scalars)
     if done is not NotImplemented:
@@ -209,7 +209,8 @@ def qk_norm_rope_backward(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k
     """Gradients (of q, of k, of q_weight, of k_weight) from the gradients ``dq``, ``dk`` of
     qk_norm_rope's outputs and its inputs (in-place outputs lose them).  The weights' gradients
     are summed in fp32 over all rows in a fixed order and rounded to the weights' dtype; None
-    for a weight of None."""
+    for a weight of None.  A position outside the table makes the gradients that depend on it NaN,
+    and ``raise_on_device_error()`` names it."""
     tensors, scalars = (dq, dk, q, k, q_weight, k_weight, cos, sin, positions), (eps, interleaved)
     done = _BACKWARD.call(tensors, scalars)
     if done is not NotImplemented:

@@ -256,7 +256,7 @@ __device__ __forceinline__ int64_t position_of(const RopeParams& p, int64_t b, i
 }
 
 // Cosines and sines of a position for the lane's pairs.  A position outside the table is recorded
-// in the status word and gives NaN rows: nothing is read out of range.
+// in the status word and makes the rotated values NaN: nothing is read out of range.
 template <typename T, bool INTER>
 __device__ __forceinline__ void load_angles(const RopeParams& p, int64_t pos, int64_t t, int unit,
                                             const LaneColumns<T>& col, Angles& g) {

@@ -597,8 +597,8 @@ int64_t b200k_fmha_workspace_bytes(const b200k_fmha_args* args);
  * rotary_dim a multiple of 16 up to D (0 = no rotation, the tables may then be NULL).  Either
  * head count may be 0.  q_out may be q and k_out may be k (same pointer and strides).
  * `positions` (batch, tokens) int32 or int64 through strides, NULL = 0, 1, 2, ... in every
- * sequence.  A position outside [0, table_rows) gives NaN rows and is recorded in the status
- * word. */
+ * sequence.  A position outside [0, table_rows) makes the rotated values of its rows NaN and is
+ * recorded in the status word. */
 typedef struct {
   const void* q;                /* (batch, heads_q, tokens, D) */
   const void* k;                /* (batch, heads_kv, tokens, D) */

@@ -406,3 +406,26 @@ def test_tables_of_repeated_rows(device_ok):
     q, k, qw, kw, cos, sin, pos = _make(2, 4, 2, 6, 64, torch.bfloat16, 64)
     _check(q, k, qw, kw, cos[7:8].expand(512, 32), sin[7:8].expand(512, 32), pos)
     _check(q, k, qw, kw, cos[7].expand(1, 32), sin[7].expand(1, 32), torch.zeros_like(pos))
+
+
+@pytest.mark.gpu
+def test_position_outside_the_table_leaves_what_is_not_rotated():
+    q, k, qw, kw, cos, sin, pos = _make(2, 2, 1, 4, 96, torch.bfloat16, 32)
+    pos[1, 2], pos[0, 0] = 512, -1
+    bad = torch.zeros(2, 1, 4, 96, dtype=torch.bool, device="cuda")
+    bad[1, :, 2, :32] = bad[0, :, 0, :32] = True
+    for inter in (False, True):
+        for x, w, y in zip((q, k), (qw, kw), b200k.qk_norm_rope(q, k, qw, kw, cos, sin, pos, interleaved=inter)):
+            want, scale = oracle.qk_rope_ref(x, w, cos, sin, pos, interleaved=inter)
+            assert torch.equal(torch.isnan(y), bad.expand_as(y))
+            good = ~torch.isnan(want)
+            _within(y[good], want[good], scale[good], 32)
+        with pytest.raises(b200k.B200KError, match="position outside"):
+            b200k.raise_on_device_error()
+        got = b200k.qk_norm_rope_backward(q, k, q, k, qw, kw, cos, sin, pos, interleaved=inter)
+        for dx, dw in (got[0::2], got[1::2]):
+            rows = torch.isnan(dx)
+            assert torch.equal(rows, bad.any(-1, keepdim=True).expand_as(dx))      # the mean over the row is NaN
+            assert bool(torch.isnan(dw[:32]).all()) and bool(torch.isfinite(dw[32:]).all())
+        with pytest.raises(b200k.B200KError, match="position outside"):
+            b200k.raise_on_device_error()
