@@ -13,6 +13,7 @@ import os
 import re
 import shutil
 import subprocess
+import textwrap
 
 import pytest
 import torch
@@ -429,3 +430,44 @@ def test_position_outside_the_table_leaves_what_is_not_rotated():
             assert bool(torch.isnan(dw[:32]).all()) and bool(torch.isfinite(dw[32:]).all())
         with pytest.raises(b200k.B200KError, match="position outside"):
             b200k.raise_on_device_error()
+
+
+def _documented_function():
+    """The autograd function of README.md."""
+    lines = open(os.path.join(ROOT, "README.md")).read().split("\n")
+    first = lines.index("    class QkNormRope(torch.autograd.Function):")
+    last = next(i for i in range(first, len(lines) + 1) if i == len(lines) or (lines[i] and not lines[i].startswith("    ")))
+    scope = {"torch": torch, "b200k": b200k}
+    exec(textwrap.dedent("\n".join(lines[first:last])), scope)
+    return scope["QkNormRope"]
+
+
+def test_the_documented_autograd_function_is_there():
+    assert issubclass(_documented_function(), torch.autograd.Function)
+
+
+@pytest.mark.gpu
+def test_the_documented_autograd_function(device_ok):
+    # a projection of queries and keys side by side, its gradient and the weights'
+    function = _documented_function()
+    g = torch.Generator().manual_seed(3)
+    qkv = torch.randn(2, 7, 8, 64, generator=g).bfloat16().cuda().requires_grad_()
+    weights = [(1 + 0.2 * torch.randn(64, generator=g)).bfloat16().cuda().requires_grad_() for _ in range(2)]
+    cos, sin = b200k.rope_table(16, 32, device="cuda")
+    pos = torch.randint(0, 16, (2, 7), generator=g).cuda()
+    q, k, _ = (x.transpose(1, 2) for x in qkv.split([4, 2, 2], dim=2))
+    qn, kn = function.apply(q, k, *weights, cos, sin, pos)
+    dq, dk = (torch.randn(x.shape, generator=g).bfloat16().cuda() for x in (qn, kn))
+    torch.autograd.backward((qn, kn), (dq, dk))
+    first = 0
+    for dy, x, w in ((dq, q, weights[0]), (dk, k, weights[1])):
+        want_x, want_w, scale_x, scale_w = oracle.qk_rope_grad_ref(dy, x.detach(), w.detach(), cos, sin, pos)
+        _within(qkv.grad[:, :, first:first + x.shape[1]].transpose(1, 2), want_x, scale_x, 64)
+        _within(w.grad, want_w, scale_w, 128)
+        first += x.shape[1]
+    assert bool((qkv.grad[:, :, first:] == 0).all())
+    qn, kn = function.apply(q, k, None, None, cos, sin)          # no norms, and keys that nothing uses
+    dx, = torch.autograd.grad(qn.float().sum(), q)
+    want, _, scale, _ = oracle.qk_rope_grad_ref(torch.ones_like(q), q.detach(), None, cos, sin,
+                                                torch.arange(7, device="cuda").expand(2, 7))
+    _within(dx, want, scale, 64)
