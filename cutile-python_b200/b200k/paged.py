@@ -166,7 +166,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     scores a tree of drafts.
 
     float16 or bfloat16, heads a multiple of the cache's, Dim a multiple of 8 up to 128, pages
-    of a multiple of 8 tokens, qk_scale positive (None: 1 / sqrt(Dim)); up to 65535 sequences, and
+    of a multiple of 8 tokens, qk_scale in (0, 2e38] (None: 1 / sqrt(Dim)); up to 65535 sequences, and
     their tables may name up to 2^38 tokens together, counted once per key/value head and 256 query
     rows of it (2^29 each).  A query that sees no token gives zeros.  Slots that hold none of the sequence's tokens are never used.  Rows behind
     new_lens[b] are padding: they stay as they are in a given ``out`` (which overlaps no input) and
@@ -216,8 +216,8 @@ def _attention_args(q, k_cache, v_cache, page_table, cache_lens, new_lens, tree_
     if k_cache.shape[2] % 8:
         raise ValueError("pages must hold a multiple of 8 tokens")
     qk_scale = 1.0 / math.sqrt(dim) if qk_scale is None else float(qk_scale)
-    if not 0.0 < qk_scale < 3.0e38:
-        raise ValueError("qk_scale must be positive and finite")
+    if not 0.0 < qk_scale <= 2.0e38:
+        raise ValueError("qk_scale must be positive and at most 2e38")
     for c, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
         if c.data_ptr() % 16 or any(s % 8 for s in c.stride()[:3]):
             raise ValueError(f"{name} must start on a 16-byte boundary with strides of whole 16-byte units")

@@ -1244,8 +1244,8 @@ int check_args(const b200k_paged_attention_args* a) {
   if (a->dtype != B200K_F16 && a->dtype != B200K_BF16) return fail(B200K_INVALID_ARG, "dtype must be f16 or bf16");
   if (a->head_dim <= 0 || a->head_dim > 128 || a->head_dim % 8 != 0)
     return fail(B200K_UNSUPPORTED, "head_dim must be a multiple of 8 up to 128 (got %d)", a->head_dim);
-  if (!(a->qk_scale > 0.f) || a->qk_scale > 3.0e38f)
-    return fail(B200K_INVALID_ARG, "qk_scale must be positive and finite");
+  if (!(a->qk_scale > 0.f) || a->qk_scale > 2.0e38f)   // times log2(e) it is finite, too
+    return fail(B200K_INVALID_ARG, "qk_scale must be positive and at most 2e38");
   if (a->page_size <= 0 || a->page_size % 8 != 0)
     return fail(B200K_UNSUPPORTED, "page_size must be a positive multiple of 8 (got %d)", a->page_size);
   const int64_t limit = int64_t(1) << 29;   // sums of two such counts fit 32 bits

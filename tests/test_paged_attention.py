@@ -121,6 +121,17 @@ def test_refusals_of_the_entry_point():
     assert call(tokens=0, q=None) == _lib.OK
 
 
+def test_scales_whose_product_with_log2_e_is_infinite_are_refused():
+    a = _lib.PagedAttentionArgs()
+    a.batch, a.tokens, a.heads_q, a.heads_kv, a.head_dim = 1, 4, 4, 2, 64
+    a.dtype, a.page_size, a.max_pages = _lib.BF16, 16, 4
+    a.q = a.k_cache = a.v_cache = a.out = a.page_table = a.cache_lens = 1 << 20
+    for scale, message in ((2.0e38, b"no pages"), (2.4e38, b"qk_scale"), (2.9e38, b"qk_scale")):
+        a.qk_scale = scale
+        assert _lib.lib().b200k_paged_attention(ctypes.byref(a), None) == _lib.INVALID_ARG
+        assert message in _lib.lib().b200k_last_error()
+
+
 def test_the_limit_of_key_tiles_counts_full_tables():
     h = _lib.lib()
 
