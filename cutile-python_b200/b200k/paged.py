@@ -77,8 +77,8 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
     padding: their cache slots stay as they are, as do their rows of a given ``q_out``; in a q_out
     made here they are zero.  A token whose page lies outside the table or the cache is not stored.
     ``raise_on_device_error()`` names the token or the sequence.  Sequences may share the pages that
-    they only read: of two tokens that a call stores in one slot, either may stay.  Outputs overlap
-    no input, but for q_out = q.
+    they only read: of two tokens that a call stores in one slot, parts of either may stay.  Outputs
+    overlap no input, but for q_out = q.
 
     Dim is a multiple of 8 up to 256 and pages hold any number of tokens; ``paged_attention`` reads
     caches of heads up to 128 and pages of a multiple of 8 tokens, and nothing else here reads others."""

@@ -651,8 +651,8 @@ int64_t b200k_qk_norm_rope_backward_workspace_bytes(const b200k_qk_norm_rope_arg
  * rotated queries to q_out in the same launch.  positions NULL = cache_lens[b] + t.  Slots of
  * padding tokens are left as they are; their q_out rows too, or become zero with
  * `zero_padding`.  A token whose page is outside [0, num_pages) or behind max_pages is not
- * stored and is recorded in the status word.  Tokens that share a slot (two sequences with the
- * same page) leave one of the two. */
+ * stored and is recorded in the status word.  Of tokens that a call stores in one slot (two
+ * sequences with the same page) parts of each may stay: nothing orders their pieces. */
 typedef struct {
   const void* k;                /* (batch, heads_kv, tokens, D) */
   const void* v;
