@@ -168,7 +168,12 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     float16 or bfloat16, heads a multiple of the cache's, Dim a multiple of 8 up to 128, pages
     of a multiple of 8 tokens, qk_scale in (0, 2e38] (None: 1 / sqrt(Dim)); up to 65535 sequences, and
     their tables may name up to 2^38 tokens together, counted once per key/value head and 256 query
-    rows of it (2^29 each).  A query that sees no token gives zeros.  Slots that hold none of the sequence's tokens are never used.  Rows behind
+    rows of it (2^29 each).  Scores, maxima, sums and the output's sum are fp32; the weights are
+    rounded to the inputs' type before they multiply V, and where more than 128 queries share a
+    cache head every fourth pair of them is computed to 7.5e-5.
+
+    A query that sees no token gives zeros.  Slots that hold none of the sequence's tokens are never
+    used; NaN and infinities of the step's tokens reach only the queries that see them.  Rows behind
     new_lens[b] are padding: they stay as they are in a given ``out`` (which overlaps no input) and
     are zero in one made here.  Sequences may share pages.  A length or page outside the table or
     the cache is not followed: that sequence's rows mean nothing, and ``raise_on_device_error()``

@@ -22,9 +22,9 @@
 //                               maximum, sum and O; the group of a run's last tile joins the two
 //                               states at its end, while the other already works on the next
 //                               run's first tile, whose S was issued before (Q has two places)
-//   quad   (at most 16 rows)    split, with the rows four times in the tile: warp q of a group takes
-//                               keys [32 q, 32 q + 32) of every tile, its P is zero elsewhere, and
-//                               its rows are a partial state of their own.  A warp's 128
+//   quad   (at most 16 rows,    split, with the rows four times in the tile: warp q of a group takes
+//          many items: see      keys [32 q, 32 q + 32) of every tile, its P is zero elsewhere, and
+//          lay_out_rows)        its rows are a partial state of their own.  A warp's 128
 //                               exponentials, 1000 cycles of the special-function unit whether
 //                               one lane has a row or all, become 32, on four schedulers
 //   pair   (more rows)          A and B are two row tiles of 128, every key tile serves both
@@ -34,17 +34,19 @@
 //   warp 1       MMA issuer: S_x = Q K^T, O_x += P_x V (P from tensor memory)
 //   warps 2..5   softmax group A, warps 6..9 group B: a query row per thread
 //
-// What a run does once (masks, Q rows that are not aligned, tokens that are not finite) is kept in
+// What a run does once (masks, values that are not finite) is kept in
 // rolled loops: unrolled, the kernel was 180 KB of code, more than the instruction cache.
 //
-// Measured (bf16, heads of 128, 32 on 8): 32 sequences of 2048 - 8192 keys, a token each, 115 us = 5.9 TB/s,
-// 0.89 of a copy (quad; a tile of 64 KB every 2230 cycles); 8 x 16 drafts of the same lengths 44 us =
-// 3.9 TB/s, where the first copies, the last softmax and the join are a third; 4 x 64 drafts of 8192 -
+// Measured (bf16, heads of 128, 32 on 8): 32 sequences of 2048 - 8192 keys, a token each, 115 - 119 us =
+// 5.7 - 5.9 TB/s, 0.87 - 0.89 of a copy (quad; a tile of 64 KB every 2230 cycles); 8 x 16 drafts of the
+// same lengths 44 us = 3.9 TB/s, where the first copies, the last softmax and the join are a third; 4 x 64 drafts of 8192 -
 // 32768 keys 124 us: 2.0 - 2.2 us for a tile of 256 rows (pair), bound by the chain S, softmax, P V of a row
-// tile.  One token of 32 heads and 1024 keys (fp16) 13.5 us: launch, lengths -> pages -> K, join.
+// tile.  One token of 32 heads and 1024 keys (fp16) 13.0 us: launch, lengths -> pages -> K, join.
 //
 // Slots behind a sequence's last token may hold anything: their scores are masked by index and
-// their rows of V are cleared in shared memory, since 0 * NaN is not 0.
+// their rows of V are cleared in shared memory, since 0 * NaN is not 0.  Values of the step's own tokens
+// that are not finite are cleared too, and added to the rows that see them.  A row that sees no key is
+// zero; NaN in a query, or in a key that the row sees, makes it NaN, whoever finishes or joins it.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -896,7 +898,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                 for (int k = 0; k < 32; ++k) {
                   const float2 y = __ffma2_rn(make_float2(s[2 * k], s[2 * k + 1]), scale2, negm2);
                   // pair: every fourth pair on the FMA pipe, as two row tiles keep the special-function
-                  // unit busier than the tensor cores (133 -> 130 us); split waits for memory
+                  // unit busier than the tensor cores (133 -> 130 us); split waits for memory.  7.5e-5 of a
+                  // weight, where its rounding to 16 bits below takes up to 2^-8 or 2^-11
                   const bool poly = PAIR && k % kFmhaPolyEvery == kFmhaPolyEvery - 1;
                   const float2 e = poly ? exp2_poly_pair<true>(y) : make_float2(fast_exp2(y.x), fast_exp2(y.y));
                   sum2[k & 3] = __fadd2_rn(sum2[k & 3], e);
@@ -1202,8 +1205,8 @@ paged_attention_join_kernel(const __grid_constant__ PagedParams p) {
 int padded_dim(const b200k_paged_attention_args* a) { return a->head_dim <= 64 ? 64 : 128; }
 
 // The rows that share a key/value head, token by token, and how they are cut: one 128-row half
-// ("split", up to 32 of them "quad"), or tiles of two halves ("pair") where there are more.  A half
-// holds whole tokens.
+// ("split"; "quad" where there are few rows and many items), or tiles of two halves ("pair") where there
+// are more.  A half holds whole tokens.
 struct Rows {
   Mode mode;
   int64_t half_tokens, tiles, per_tile;      // per_tile: rows of a partial state

@@ -693,6 +693,8 @@ int b200k_paged_kv_append(const b200k_paged_kv_append_args* args, b200k_stream s
  * new_lens[b] of the call for which tree_mask[b][t][j] is not 0 (NULL: j <= t), so that a tree
  * of drafted tokens, a chunk of a prompt and a single token are the same call.
  *   out = sum_p softmax_p(qk_scale * q . k_p) v_p        (a row that sees no key gives 0)
+ * in fp32, but for the weights, which are rounded to the inputs' type before they multiply v_p and, with
+ * more than 128 query rows per key/value head, every fourth pair of which is computed to 7.5e-5.
  * qk_scale lies in (0, 2e38].  What lies in slots that no token of the sequence occupies is never
  * used, whatever it is.  A page outside [0, num_pages) counts as zeros, lengths beyond the page
  * table as its end; both are recorded in the status word.
