@@ -173,7 +173,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     cache head every fourth pair of them is computed to 7.5e-5.
 
     A query that sees no token gives zeros.  Slots that hold none of the sequence's tokens are never
-    used; NaN and infinities of the step's tokens reach only the queries that see them.  Rows behind
+    used; NaN and infinities of the step's tokens reach only the queries that see them.  (An infinite
+    value of an earlier token gives infinity, or NaN where its weight rounds to zero.)  Rows behind
     new_lens[b] are padding: they stay as they are in a given ``out`` (which overlaps no input) and
     are zero in one made here.  Sequences may share pages.  A length or page outside the table or
     the cache is not followed: that sequence's rows mean nothing, and ``raise_on_device_error()``
