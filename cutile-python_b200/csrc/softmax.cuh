@@ -27,10 +27,12 @@ __device__ __forceinline__ float fmax_or_nan(float a, float b) {
 // of P to 16 bits.  0 disables the polynomial path.
 //
 // Arguments far below zero: without EXACT_ENDS they give 2^-125, which a row that sees something
-// does not notice, and so does NaN.  With it the power of two is a factor of its own, so that
+// does not notice, and NaN gives the largest number, whose rounding to 16 bits is infinite, so that
+// the row is not finite either.  With it the power of two is a factor of its own, so that
 // arguments from -127 down (a masked score's -inf) give the bits of 2^-127, a zero: rows that see
-// nothing keep a sum of zero, and a masked value no weight.  NaN stays NaN.  One more product per pair (4 x 64 drafts over 8192 - 32768 keys
-// 127 us as before); the contiguous attention, whose rows all see something, keeps the shorter form.
+// nothing keep a sum of zero, and a masked value no weight.  NaN stays NaN.  One more product per pair
+// (4 x 64 drafts over 8192 - 32768 keys 127 us as before); the contiguous attention, whose rows all see
+// something, keeps the shorter form (4 x 16 heads of 64, 4096 tokens, bf16: 456 us, 468 with the product).
 #ifndef B200K_FMHA_POLY
 #define B200K_FMHA_POLY 4
 #endif
@@ -40,13 +42,9 @@ template <bool EXACT_ENDS = false>
 __device__ __forceinline__ float2 exp2_poly_pair(float2 x) {
   const float2 magic = make_float2(12582912.0f, 12582912.0f);       // 1.5 * 2^23
   const float2 neg_magic = make_float2(-12582912.0f, -12582912.0f);
-  if constexpr (EXACT_ENDS) {
-    x.x = fmax_or_nan(x.x, -127.0f);
-    x.y = fmax_or_nan(x.y, -127.0f);
-  } else {
-    x.x = fmaxf(x.x, -125.0f);
-    x.y = fmaxf(x.y, -125.0f);
-  }
+  constexpr float kLeast = EXACT_ENDS ? -127.0f : -125.0f;
+  x.x = fmax_or_nan(x.x, kLeast);
+  x.y = fmax_or_nan(x.y, kLeast);
   const float2 t = __fadd2_rn(x, magic);            // integer part lands in the low mantissa bits
   const float2 i = __fadd2_rn(t, neg_magic);
   const float2 f = __fadd2_rn(x, make_float2(-i.x, -i.y));   // in [-0.5, 0.5]

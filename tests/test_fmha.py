@@ -176,3 +176,18 @@ def test_fmha_baseline_shape_slice(device_ok):
     ones = torch.ones_like(v)
     const = b200k.cutile_fmha(q.cuda(), k.cuda(), ones.cuda(), causal=True).float().cpu()
     torch.testing.assert_close(const, torch.ones_like(const), atol=1e-2, rtol=1e-2)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("residue", range(8))
+@pytest.mark.parametrize("sq,d", [(200, 64), (200, 128), (2048, 128)])
+def test_a_key_of_nan_reaches_every_row_that_sees_it(dtype, residue, sq, d, device_ok):
+    # at every place of the eight scores that one round of exponentials takes
+    q, k, v = (x.cuda() for x in _qkv(2, 4, 4, sq, sq, d, dtype, 7))
+    at = sq // 2 // 8 * 8 + residue
+    clean = b200k.cutile_fmha(q, k, v, causal=True)
+    k[:, :, at, 3] = math.nan
+    out = b200k.cutile_fmha(q, k, v, causal=True)
+    assert torch.equal(out[:, :, :at], clean[:, :, :at])
+    assert not bool(torch.isfinite(out[:, :, at:]).any())
+    assert not bool(torch.isfinite(b200k.cutile_fmha(q, k, v, causal=False)).any())
